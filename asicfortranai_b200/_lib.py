@@ -17,6 +17,9 @@ Q35_FMT_INT4 = 1
 Q35_LAYOUT_COLMAJOR = 0
 Q35_LAYOUT_ROWMAJOR = 1
 
+DTYPES = {"f32": 0, "bf16": 1, "f16": 2}      # Q35_DT_*
+CODES = {"int8": 0, "e4m3": 1}                # Q35_CODE_*
+
 _vp, _i32, _i64, _sz = C.c_void_p, C.c_int32, C.c_int64, C.c_size_t
 
 # name -> (restype, argtypes); every symbol include/q35.h declares
@@ -73,6 +76,14 @@ SIGNATURES = {
     "q35_sample_top_k": (C.c_int, [_vp, _vp, _i32, _i32, C.c_float, _vp]),
     "q35_sample_top_p": (C.c_int, [_vp, _vp, _i32, C.c_float, C.c_float, _vp]),
     "q35_sample_dev": (C.c_int, [_vp, _i32, _vp, _i32, _i32, C.c_float, _i32, C.c_float, _vp, _vp]),
+    "q35_sample_filtered_dev": (C.c_int, [_vp, C.c_int, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "q35_rms_norm_quant_dev": (C.c_int, [_vp, C.c_int, _vp, _i64, _vp, _i64, _vp, _i64, _vp, C.c_float, _i32, _i32,
+                                         C.c_int, _i32, _vp, _i64, _vp]),
+    "q35_fp8_gemm_dev": (C.c_int, [_vp, _vp, _i64, _vp, _vp, _i64, _vp, C.c_int, _vp, _i64, _i32, _i32, _i32]),
+    "q35_kv8_append_dev": (C.c_int, [_vp, _vp, C.c_int, _vp, _vp, _i64, _vp, _vp, _i32, _i32]),
+    "q35_kv8_attention_dev": (C.c_int, [_vp, _vp, C.c_int, _vp, _i64, _i32, _vp, _i64, _vp, _vp, _i32, _i32,
+                                        C.c_float, _vp, _sz]),
+    "q35_kv8_attention_workspace": (C.c_int64, [_vp, _i32, _i32, _i32]),
     "q35_model_set_sampling": (C.c_int, [_vp, _vp]),
     "q35_model_create": (C.c_int, [_vp, _vp, C.POINTER(_vp)]),
     "q35_model_create_tp": (C.c_int, [_vp, _vp, _vp, C.POINTER(_vp)]),
@@ -98,6 +109,16 @@ _lib = None
 
 class Q35Error(RuntimeError):
     pass
+
+
+def dtype_code(dtype) -> int:
+    """Q35_DT_* of "f32", "bf16" or "f16" (other values go to the library, which refuses them)."""
+    return DTYPES.get(dtype, dtype if isinstance(dtype, int) else -1)
+
+
+def code_of(code) -> int:
+    """Q35_CODE_* of "int8" or "e4m3"."""
+    return CODES.get(code, code if isinstance(code, int) else -1)
 
 
 def load():

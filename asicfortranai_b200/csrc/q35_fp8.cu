@@ -1,0 +1,508 @@
+// q35_fp8.cu -- matrix product in 8-bit floating point (e4m3) with a scale for each block of
+// 128 along k of every row of x, and for each 128 x 128 block of w:
+//   y[m][n] = sum_b xs[m][b] ws[n / 128][b] sum_{k in block b} x[m][k] w[n][k]
+//
+// Tile: 128 rows of w (the MMA's M: one row of scale blocks, so ws is one number per tile
+// and k-block) x BN rows of x (the MMA's N).  Per 128-k block:
+//   * producer (warp 0, one thread): two 2D TMA loads, 128 bytes of k x 128 rows of w and
+//     x BN rows of x, 128-byte swizzle (rows past the edges and k past K read as zero);
+//   * scale loader (warp 2): xs[m][b] * ws[b] of the tile's BN rows into the stage;
+//   * MMA issuer (warp 1, one thread): 4 x tcgen05.mma kind::f8f6f4 (K = 32 each) into one
+//     of several accumulators in tensor memory.  The sum over one block is a tensor-core
+//     fp32 sum of exact products;
+//   * promotion (warps 4 ..): tcgen05.ld of the block's sums, acc = fma(sum, scale, acc)
+//     with acc in registers -- a thread owns one row of w, the scales are read as broadcast
+//     pairs and two sums take one packed fma (fma.rn.f32x2).
+// A k-block's accumulator is handed over through mbarriers, so the MMAs of the next blocks
+// run under the promotion of this one.
+//
+// Few tiles (decode batches) are split along k over the CTAs of a cluster; each CTA then adds
+// up its share of the tile's columns from every CTA's shared memory, in CTA order, so the
+// result does not depend on timing.  Many tiles run on a persistent grid, the row tiles of
+// one w tile side by side so that w comes from HBM once.
+//
+// With w in the MMA's M position a warp stores 32 consecutive n of a row of y, whatever y's
+// stride and type, without staging.
+//
+// Every wait is bounded: a wait that gives up records Q35_ERR_TIMEOUT in the context's error
+// word and raises an abort flag that ends the other roles' waits; copies and MMAs in flight
+// are waited for (bounded) before the CTA leaves.
+#include <cuda.h>
+
+#include <algorithm>
+
+#include "q35_q8.cuh"
+
+namespace q35 {
+namespace {
+
+constexpr int F8_TN = 128;                 // rows of w per tile
+constexpr int F8_KB = 128;                 // k per block (bytes per row of a stage)
+constexpr uint32_t F8_WAIT = 1u << 26;
+
+struct F8Params {
+    const float *xs, *ws;                  // [M][KB], [ceil(N/128)][KB]
+    void *y;
+    int64_t ldy;
+    int32_t M, N, KB;
+    int32_t BN, mt, nt;                    // rows of x per tile, tiles along m and n
+    int32_t split;                         // CTAs (of a cluster) per tile
+    int32_t stages, bufs;
+    uint32_t tmem_cols, buf_cols;
+    uint32_t off_sc, off_bar;
+    int *err;
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred P1;\n\t"
+                 "mbarrier.try_wait.parity.shared::cta.b64 P1, [%1], %2;\n\t"
+                 "selp.b32 %0, 1, 0, P1;\n\t}"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+// bounded wait; gives up when the limit passes or another role raised the abort flag
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag) {
+    for (uint32_t i = 0; i < F8_WAIT; ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((i & 255u) == 255u && *abort_flag) return false;
+    }
+    return false;
+}
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map, int32_t x, int32_t y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+                 " [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tc_mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tc_ld16(uint32_t taddr, float (&v)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32"
+                 " {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]),
+                   "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]),
+                   "=f"(v[14]), "=f"(v[15])
+                 : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// K-major operand, 128-byte swizzle: 8-row atoms of 1024 bytes
+__device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t addr) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// D fp32, A and B e4m3, both K-major, M = 128
+__host__ __device__ constexpr uint32_t idesc_f8(int BN) {
+    return (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(F8_TN >> 4) << 24);
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t rank, float v) {
+    asm volatile("{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %0, %1;\n\t"
+                 "st.shared::cluster.f32 [ra], %2;\n\t}" ::"r"(addr), "r"(rank), "f"(v) : "memory");
+}
+
+struct Ring {
+    int i = 0;
+    uint32_t ph = 0;
+    __device__ __forceinline__ void next(int n) {
+        if (++i == n) { i = 0; ph ^= 1u; }
+    }
+};
+
+// NB: accumulator registers (x rows) per promotion thread; 4 or 8 promotion warps, the second
+// four taking the upper half of the tile's columns
+template <typename T, int NB, int PW>
+__global__ void __launch_bounds__(128 + 32 * PW, 1)
+fp8_gemm_kernel(const F8Params p, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap) {
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    uint8_t *sbase = smem_raw + (base - raw);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int S = p.stages, NBUF = p.bufs, BN = p.BN;
+    const uint32_t stage_bytes = (uint32_t)(F8_TN + BN) * F8_KB;
+    const uint32_t bars = base + p.off_bar;
+    auto full = [&](int i) { return bars + 8u * i; };                       // TMA bytes
+    auto sc_full = [&](int i) { return bars + 8u * (S + i); };              // scale loader
+    auto empty = [&](int i) { return bars + 8u * (2 * S + i); };            // commit + promotion warps
+    auto acc_full = [&](int i) { return bars + 8u * (3 * S + i); };         // commit
+    auto acc_empty = [&](int i) { return bars + 8u * (3 * S + NBUF + i); }; // promotion warps
+    const uint32_t drain = bars + 8u * (3 * S + 2 * NBUF);
+    uint8_t *misc = sbase + p.off_bar + 8 * (3 * S + 2 * NBUF + 1);
+    volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(misc);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(misc + 4);
+
+    if (tid == 0) {
+        for (int i = 0; i < S; ++i) { mbar_init(full(i), 1); mbar_init(sc_full(i), 1); mbar_init(empty(i), 1 + PW); }
+        for (int i = 0; i < NBUF; ++i) { mbar_init(acc_full(i), 1); mbar_init(acc_empty(i), PW); }
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_u32((const void *)tmem_slot)), "r"(p.tmem_cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    const int rank = p.split > 1 ? (int)cluster_rank() : 0;
+    const int first_tile = blockIdx.x / p.split, step = gridDim.x / p.split;
+    const int tiles = p.mt * p.nt;
+    const int kb0 = (int)((int64_t)p.KB * rank / p.split), kb1 = (int)((int64_t)p.KB * (rank + 1) / p.split);
+    bool ok = true;
+    auto fail = [&]() {
+        ok = false;
+        *abort_flag = 1;
+        atomicExch(p.err, Q35_ERR_TIMEOUT);
+    };
+
+    constexpr int HB = NB;                       // columns per promotion thread
+    float2 acc[HB / 2];
+    if (warp == 0) {
+        if (lane == 0) {
+            Ring st{};
+            int64_t issued = 0;
+            for (int tile = first_tile; tile < tiles && ok; tile += step) {
+                const int nt = tile / p.mt, mt = tile - nt * p.mt;
+                for (int kb = kb0; kb < kb1; ++kb) {
+                    if (!mbar_wait(empty(st.i), st.ph ^ 1u, abort_flag)) { fail(); break; }
+                    mbar_expect_tx(full(st.i), stage_bytes);
+                    const uint32_t dst = base + (uint32_t)st.i * stage_bytes;
+                    tma_load_2d(dst, &wmap, kb * F8_KB, nt * F8_TN, full(st.i));
+                    tma_load_2d(dst + F8_TN * F8_KB, &xmap, kb * F8_KB, mt * BN, full(st.i));
+                    st.next(S);
+                    ++issued;
+                }
+            }
+            // every copy has landed before the CTA leaves (after a failure too)
+            for (int64_t j = issued < S ? issued : S; j > 0; --j) {
+                const int i = st.i >= j ? st.i - (int)j : st.i - (int)j + S;
+                const uint32_t ph = st.i >= j ? st.ph : st.ph ^ 1u;
+                for (uint32_t n = 0; n < (1u << 20) && !mbar_try_wait(full(i), ph); ++n) {}
+            }
+        }
+    } else if (warp == 2) {
+        // scales of a stage: xs[m][kb] * ws[nt][kb], four k-blocks' loads in flight at once
+        constexpr int SN = NB * (PW / 4), SL = (SN + 31) / 32, SB = 4;
+        Ring st{};
+        for (int tile = first_tile; tile < tiles && ok; tile += step) {
+            const int nt = tile / p.mt, mt = tile - nt * p.mt;
+            for (int kb = kb0; kb < kb1 && ok; kb += SB) {
+                float v[SB][SL];
+#pragma unroll
+                for (int b = 0; b < SB; ++b) {
+                    const bool live = kb + b < kb1;
+                    const float w = live ? p.ws[(int64_t)nt * p.KB + kb + b] : 0.0f;
+#pragma unroll
+                    for (int i = 0; i < SL; ++i) {
+                        const int j = lane + 32 * i, m = mt * BN + j;
+                        v[b][i] = live && j < BN && m < p.M ? p.xs[(int64_t)m * p.KB + kb + b] * w : 0.0f;
+                    }
+                }
+#pragma unroll
+                for (int b = 0; b < SB; ++b) {
+                    if (kb + b >= kb1) break;
+                    if (!__all_sync(0xffffffffu, mbar_wait(empty(st.i), st.ph ^ 1u, abort_flag))) { fail(); break; }
+                    float *sc = reinterpret_cast<float *>(sbase + p.off_sc) + st.i * SN;
+#pragma unroll
+                    for (int i = 0; i < SL; ++i)
+                        if (lane + 32 * i < SN) sc[lane + 32 * i] = v[b][i];
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(sc_full(st.i));
+                    st.next(S);
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            const uint32_t idesc = idesc_f8(BN);
+            Ring st{}, ab{};
+            for (int tile = first_tile; tile < tiles && ok; tile += step) {
+                for (int kb = kb0; kb < kb1; ++kb) {
+                    if (!mbar_wait(acc_empty(ab.i), ab.ph ^ 1u, abort_flag) || !mbar_wait(full(st.i), st.ph, abort_flag)) {
+                        fail();
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t a0 = base + (uint32_t)st.i * stage_bytes, b0 = a0 + F8_TN * F8_KB;
+                    const uint32_t d = tmem + (uint32_t)ab.i * p.buf_cols;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        tc_mma_f8(d, smem_desc_sw128(a0 + 32u * j), smem_desc_sw128(b0 + 32u * j), idesc, j > 0 ? 1u : 0u);
+                    tc_commit(empty(st.i));
+                    tc_commit(acc_full(ab.i));
+                    st.next(S);
+                    ab.next(NBUF);
+                }
+            }
+            // every MMA issued has completed before the CTA moves on
+            tc_commit(drain);
+            if (!mbar_wait(drain, 0, abort_flag)) fail();
+        }
+    } else if (warp >= 4) {
+        const int q = warp & 3, half = (warp - 4) >> 2;
+        const int c0 = half * NB;                       // first column of this thread
+        Ring st{}, ab{};
+        for (int tile = first_tile; tile < tiles && ok; tile += step) {
+            const int nt = tile / p.mt, mt = tile - nt * p.mt;
+#pragma unroll
+            for (int i = 0; i < HB / 2; ++i) acc[i] = make_float2(0.0f, 0.0f);
+            for (int kb = kb0; kb < kb1; ++kb) {
+                // (the stage cannot be refilled before this warp arrives on it, so its phase
+                // is still the one to wait for)
+                if (!__all_sync(0xffffffffu, mbar_wait(acc_full(ab.i), ab.ph, abort_flag) &&
+                                                 mbar_wait(sc_full(st.i), st.ph, abort_flag))) { fail(); break; }
+                tc_fence_after();
+                const float *sc = reinterpret_cast<const float *>(sbase + p.off_sc) + st.i * (NB * (PW / 4)) + c0;
+                const uint32_t ta = tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)ab.i * p.buf_cols + (uint32_t)c0;
+#pragma unroll
+                for (int j = 0; j < NB / 16; ++j) {
+                    if (c0 + 16 * j >= BN) break;
+                    float v[16];
+                    tc_ld16(ta + 16u * j, v);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 8; i += 2) {
+                        const float4 s4 = *reinterpret_cast<const float4 *>(sc + 16 * j + 2 * i);
+                        float2 &A0 = acc[8 * j + i], &A1 = acc[8 * j + i + 1];
+                        asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%0, %1};\n\t"
+                            "fma.rn.f32x2 c, a, b, c;\n\tmov.b64 {%0, %1}, c;\n\t}"
+                            : "+f"(A0.x), "+f"(A0.y) : "f"(v[2 * i]), "f"(v[2 * i + 1]), "f"(s4.x), "f"(s4.y));
+                        asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%0, %1};\n\t"
+                            "fma.rn.f32x2 c, a, b, c;\n\tmov.b64 {%0, %1}, c;\n\t}"
+                            : "+f"(A1.x), "+f"(A1.y) : "f"(v[2 * i + 2]), "f"(v[2 * i + 3]), "f"(s4.z), "f"(s4.w));
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) { mbar_arrive(acc_empty(ab.i)); mbar_arrive(empty(st.i)); }
+                st.next(S);
+                ab.next(NBUF);
+            }
+            if (p.split == 1 && ok) {
+                const int n = nt * F8_TN + 32 * q + lane;
+                T *y = static_cast<T *>(p.y) + n;
+#pragma unroll
+                for (int j = 0; j < HB; ++j) {
+                    const int m = mt * BN + c0 + j;
+                    if (c0 + j < BN && m < p.M && n < p.N) y[(int64_t)m * p.ldy] = from_f32<T>(j & 1 ? acc[j / 2].y : acc[j / 2].x);
+                }
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1) {
+        __syncwarp();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_cols) : "memory");
+    }
+    if (p.split > 1) {
+        // column j of the tile belongs to the cluster's CTA j / cols, which receives every
+        // CTA's partial sums in its stage memory (each CTA has drained its copies and MMAs
+        // when it passes the first barrier) and adds them in CTA order
+        const int cols = (BN + p.split - 1) / p.split;
+        const int tile = first_tile, nt = tile / p.mt, mt = tile - nt * p.mt;
+        cluster_sync();
+        if (warp >= 4) {
+            const int q = warp & 3, c0 = ((warp - 4) >> 2) * NB;
+#pragma unroll
+            for (int j = 0; j < HB; ++j) {
+                const int col = c0 + j;
+                if (col < BN) {
+                    const int to = col / cols;
+                    st_cluster(base + 4u * (uint32_t)((rank * cols + (col - to * cols)) * F8_TN + 32 * q + lane),
+                               (uint32_t)to, j & 1 ? acc[j / 2].y : acc[j / 2].x);
+                }
+            }
+        }
+        cluster_sync();
+        const float *part = reinterpret_cast<const float *>(sbase);
+        const int mine = min(cols, BN - rank * cols);
+        for (int e = tid; e < mine * F8_TN; e += blockDim.x) {
+            const int j = e / F8_TN, r = e - j * F8_TN;
+            float v = 0.0f;
+            for (int s = 0; s < p.split; ++s) v += part[(s * cols + j) * F8_TN + r];
+            const int m = mt * BN + rank * cols + j, n = nt * F8_TN + r;
+            if (m < p.M && n < p.N) static_cast<T *>(p.y)[(int64_t)m * p.ldy + n] = from_f32<T>(v);
+        }
+    }
+}
+
+// ---- host side -------------------------------------------------------------------------
+
+using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                              const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// the driver entry point, looked up through the runtime (as in q35_mma.cu)
+int tma_encoder(EncodeFn *out) {
+    static EncodeFn encode = nullptr;
+    if (!encode) {
+        void *fn = nullptr;
+        cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+        cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q);
+        if (e != cudaSuccess || q != cudaDriverEntryPointSuccess || !fn)
+            return set_error(Q35_ERR_CUDA, "fp8_gemm: cuTensorMapEncodeTiled not available");
+        encode = reinterpret_cast<EncodeFn>(fn);
+    }
+    *out = encode;
+    return Q35_OK;
+}
+
+int byte_map(EncodeFn encode, CUtensorMap *map, const void *p, int64_t rows, int64_t K, int64_t ld, int box_rows) {
+    const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)ld};
+    const cuuint32_t box[2] = {(cuuint32_t)F8_KB, (cuuint32_t)box_rows};
+    const cuuint32_t estr[2] = {1u, 1u};
+    CUresult cr = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(p), dims, strides, box, estr,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return cr == CUDA_SUCCESS ? Q35_OK : set_error(Q35_ERR_CUDA, "fp8_gemm: cuTensorMapEncodeTiled failed");
+}
+
+struct F8Plan {
+    int NB, PW, BN, mt, nt, split, stages, bufs, grid;
+    uint32_t tmem_cols, buf_cols, off_sc, off_bar;
+    size_t smem;
+};
+
+F8Plan plan_f8(int32_t M, int32_t N, int32_t KB) {
+    constexpr int SMS = 148;
+    F8Plan pl{};
+    pl.mt = (int)ceil_div(M, 256);
+    pl.BN = (int)round_up(ceil_div(M, pl.mt), 16);
+    pl.nt = (int)ceil_div(N, F8_TN);
+    pl.NB = pl.BN <= 16 ? 16 : pl.BN <= 32 ? 32 : pl.BN <= 64 ? 64 : 128;
+    pl.PW = pl.BN <= 128 ? 4 : 8;
+    const int tiles = pl.mt * pl.nt;
+    pl.split = 1;
+    while (pl.split < 8 && 2 * pl.split <= KB && (int64_t)tiles * 2 * pl.split <= SMS) pl.split *= 2;
+    pl.grid = pl.split > 1 ? tiles * pl.split : std::min(tiles, SMS);
+    pl.buf_cols = (uint32_t)(pl.NB * (pl.PW / 4));
+    pl.bufs = std::min<int>(8, 512 / pl.buf_cols);
+    pl.tmem_cols = 32;
+    while (pl.tmem_cols < pl.bufs * pl.buf_cols) pl.tmem_cols *= 2;
+    const size_t stage = (size_t)(F8_TN + pl.BN) * F8_KB, sc = pl.buf_cols * 4;
+    const size_t budget = 227 * 1024 - 1024 - 512;
+    pl.stages = (int)std::min<size_t>(16, budget / (stage + sc));
+    // the split exchange reuses the stages: split * ceil(BN / split) columns of 128 floats
+    pl.off_sc = (uint32_t)(pl.stages * stage);
+    pl.off_bar = (uint32_t)round_up((int64_t)(pl.off_sc + pl.stages * sc), 8);
+    pl.smem = 1024 + pl.off_bar + 8 * (3 * pl.stages + 2 * pl.bufs + 1) + 16;
+    return pl;
+}
+
+template <typename T, int NB, int PW>
+int launch_f8(const F8Params &p, const F8Plan &pl, const CUtensorMap &wm, const CUtensorMap &xm, int dev, cudaStream_t s) {
+    auto kern = fp8_gemm_kernel<T, NB, PW>;
+    static bool configured[64] = {};
+    if (!configured[dev]) {
+        Q35_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+        configured[dev] = true;
+    }
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)pl.split;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)pl.grid);
+    cfg.blockDim = dim3(128 + 32 * PW);
+    cfg.dynamicSmemBytes = pl.smem;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    Q35_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, p, wm, xm));
+    return Q35_OK;
+}
+
+template <typename T>
+int launch_f8(const F8Params &p, const F8Plan &pl, const CUtensorMap &wm, const CUtensorMap &xm, int dev, cudaStream_t s) {
+    if (pl.PW == 8) return launch_f8<T, 128, 8>(p, pl, wm, xm, dev, s);
+    switch (pl.NB) {
+    case 16: return launch_f8<T, 16, 4>(p, pl, wm, xm, dev, s);
+    case 32: return launch_f8<T, 32, 4>(p, pl, wm, xm, dev, s);
+    case 64: return launch_f8<T, 64, 4>(p, pl, wm, xm, dev, s);
+    default: return launch_f8<T, 128, 4>(p, pl, wm, xm, dev, s);
+    }
+}
+
+}  // namespace
+}  // namespace q35
+
+using namespace q35;
+
+extern "C" int q35_fp8_gemm_dev(q35_ctx ctx, const void *x, int64_t ldx, const float *x_scales, const void *w,
+                                int64_t ldw, const float *w_scales, int dtype, void *y, int64_t ldy, int32_t M,
+                                int32_t N, int32_t K) {
+    if (!ctx) return set_error(Q35_ERR_INVALID, "fp8_gemm: ctx is NULL");
+    int st = check_dtype(dtype);
+    if (st) return st;
+    if (M < 0 || M > GEMM_MAX_M) return set_error(Q35_ERR_INVALID, "fp8_gemm: M must be in [0,65536]");
+    if (N < 0 || N > (1 << 24)) return set_error(Q35_ERR_INVALID, "fp8_gemm: N must be in [0,2^24]");
+    if (K < 1 || K > GEMM_MAX_K) return set_error(Q35_ERR_INVALID, "fp8_gemm: K must be in [1,131072]");
+    if (M == 0 || N == 0) return Q35_OK;
+    if (!x || !x_scales || !w || !w_scales || !y) return set_error(Q35_ERR_INVALID, "fp8_gemm: NULL argument");
+    if (ldx < K || ldw < K || ldy < N) return set_error(Q35_ERR_INVALID, "fp8_gemm: a row stride is below the row's length");
+    if (ldx % 16 || ldw % 16 || !aligned_to(x, 16) || !aligned_to(w, 16))
+        return set_error(Q35_ERR_INVALID, "fp8_gemm: rows of x and w must start on 16-byte boundaries");
+    if (!aligned_to(x_scales, 4) || !aligned_to(w_scales, 4) || !aligned_to(y, dtype_size(dtype)))
+        return set_error(Q35_ERR_INVALID, "fp8_gemm: a pointer is not aligned to its elements");
+    if (ctx->device < 0 || ctx->device >= 64) return set_error(Q35_ERR_INVALID, "fp8_gemm: device ordinal out of range");
+    DeviceGuard g(ctx->device);
+    st = ensure_workspace(ctx, 0, 0);
+    if (st) return st;
+    EncodeFn encode = nullptr;
+    st = tma_encoder(&encode);
+    if (st) return st;
+    const int KB = (int)ceil_div(K, F8_KB);
+    const F8Plan pl = plan_f8(M, N, KB);
+    CUtensorMap wm, xm;
+    st = byte_map(encode, &wm, w, N, K, ldw, F8_TN);
+    if (!st) st = byte_map(encode, &xm, x, M, K, ldx, pl.BN);
+    if (st) return st;
+    F8Params p;
+    p.xs = x_scales; p.ws = w_scales;
+    p.y = y; p.ldy = ldy;
+    p.M = M; p.N = N; p.KB = KB;
+    p.BN = pl.BN; p.mt = pl.mt; p.nt = pl.nt;
+    p.split = pl.split; p.stages = pl.stages; p.bufs = pl.bufs;
+    p.tmem_cols = pl.tmem_cols; p.buf_cols = pl.buf_cols;
+    p.off_sc = pl.off_sc; p.off_bar = pl.off_bar;
+    p.err = ctx->ws.err;
+    switch (dtype) {
+    case Q35_DT_F32: return launch_f8<float>(p, pl, wm, xm, ctx->device, ctx->stream);
+    case Q35_DT_BF16: return launch_f8<__nv_bfloat16>(p, pl, wm, xm, ctx->device, ctx->stream);
+    default: return launch_f8<__half>(p, pl, wm, xm, ctx->device, ctx->stream);
+    }
+}

@@ -1,0 +1,733 @@
+// q35_kv8.cu -- a KV cache held in 8 bits with a scale for each block of tokens and head:
+// the append that fills it and the causal grouped-query attention that reads it.
+//
+//   codes  k, v [seq][kv_head][max_seq][head_dim], one byte each (int8 or e4m3)
+//   scales k_scale, v_scale [seq][kv_head][ceil(max_seq / block)], block of 16..128 tokens
+//
+// Append.  Tokens that join a block can be larger than the ones it holds, so the block's
+// scale is s' = max(s, max |new| / Q) (s = 0 for a block without older tokens); where it
+// grew, the older codes become the codes nearest to (code * s) / s'.  One CTA per (block,
+// head, k or v): it alone reads and writes the block, so nothing races.  Non-finite input
+// does not enter the maximum; infinities are stored as +-Q, NaN as 0.
+//
+// Attention.  o = sum_j softmax_j(scale q . k_j) v_j over the row's own position and all
+// before it.  The group's query heads read a kv head's codes once: its (row, head) pairs
+// are the 16 rows of an m16n8k16 tensor-core tile.  Codes become fp16 exactly (both codes
+// fit its 11 bits), the scale multiplies the fp32 scores of its block, and v's scale the
+// probabilities, relative to the largest v scale seen so far (at most 1), so no range is
+// lost.  A query row is scaled by a power of two to use fp16's range; fp32 queries and their
+// probabilities take two fp16 terms each (22 bits).  Maximum, sum and outputs are fp32.
+//
+// No shared-memory staging of codes: a lane's 16 consecutive bytes of a key serve four
+// k-steps of Q K^T (the order of the d indices is free as long as Q uses the same), and its
+// 16 bytes of each of four keys serve 16 column tiles of P V (the order of the output
+// columns is free), so every load is a 16-byte register load and there is no transpose.
+#include <algorithm>
+#include <type_traits>
+
+#include "q35_kv8.cuh"
+
+namespace q35 {
+namespace {
+
+struct AppendParams {
+    const void *x[2];          // k, v rows
+    uint8_t *codes[2];
+    float *scales[2];
+    int64_t ld;                // elements between rows of x
+    int64_t seq_stride, scale_seq_stride;
+    const int32_t *row_start, *past;
+    int32_t rows, max_rows, G, max_seq, nblk;
+    int *err;
+};
+
+// the rows of sequence s: first row, count (0 with the error word set when the tables are
+// inconsistent or the cache would overflow) and the tokens before them
+struct SeqRows { int r0, n, past; };
+__device__ __forceinline__ SeqRows seq_rows(const int32_t *row_start, const int32_t *past, int s, int rows,
+                                            int max_rows, int max_seq, int *err) {
+    SeqRows q;
+    q.r0 = row_start[s];
+    const int r1 = row_start[s + 1];
+    q.n = r1 - q.r0;
+    q.past = past[s];
+    const bool ok = q.r0 >= 0 && r1 >= q.r0 && r1 <= rows && q.n <= max_rows && q.past >= 0 &&
+                    (int64_t)q.past + q.n <= max_seq;
+    if (!ok) {
+        if (threadIdx.x == 0) atomicExch(err, Q35_ERR_INVALID);
+        q.n = 0;
+    }
+    return q;
+}
+
+constexpr int APPEND_THREADS = 256;
+
+template <typename T, int CODE, int D, int TB>
+__global__ void __launch_bounds__(APPEND_THREADS) kv8_append_kernel(const AppendParams p) {
+    __shared__ float part[APPEND_THREADS / 32];
+    const int s = blockIdx.z >> 1, which = blockIdx.z & 1, head = blockIdx.y;
+    const SeqRows q = seq_rows(p.row_start, p.past, s, p.rows, p.max_rows, p.max_seq, p.err);
+    if (q.n == 0) return;
+    const int blk = q.past / TB + blockIdx.x;
+    const int t0 = blk * TB;                              // first token of the block
+    const int first = max(t0, q.past), last = min(t0 + TB, q.past + q.n);   // new tokens [first, last)
+    if (first >= last) return;
+    const T *x = static_cast<const T *>(p.x[which]) + (int64_t)(q.r0 + first - q.past) * p.ld + (int64_t)head * D;
+    uint8_t *codes = p.codes[which] + s * p.seq_stride + ((int64_t)head * p.max_seq + t0) * D;
+    float *scale = p.scales[which] + s * p.scale_seq_stride + (int64_t)head * p.nblk + blk;
+    const int held = first - t0, fresh = last - first;
+
+    float amax = 0.0f;
+    for (int e = threadIdx.x; e < fresh * D; e += APPEND_THREADS) {
+        const float a = fabsf(to_f32<T>(x[(int64_t)(e / D) * p.ld + e % D]));
+        if (a <= 3.402823466e38f) amax = fmaxf(amax, a);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = amax;
+    const float old = held ? *scale : 0.0f;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < APPEND_THREADS / 32; ++w) amax = fmaxf(amax, part[w]);
+    const float now = fmaxf(old, __fdiv_rn(amax, code_max<CODE>()));
+    if (threadIdx.x == 0) *scale = now;
+    if (held && now != old)
+        for (int e = threadIdx.x; e < held * D; e += APPEND_THREADS)
+            codes[e] = encode8<CODE>(__fdiv_rn(__fmul_rn(decode8<CODE>(codes[e]), old), now));
+    codes += held * D;
+    for (int e = threadIdx.x; e < fresh * D; e += APPEND_THREADS) {
+        const float v = to_f32<T>(x[(int64_t)(e / D) * p.ld + e % D]);
+        codes[e] = now == 0.0f || v != v ? 0 : encode8<CODE>(__fdiv_rn(v, now));
+    }
+}
+
+// ---- attention ------------------------------------------------------------------------
+
+constexpr int ATT_WARPS = 8;
+constexpr int ATT_THREADS = 32 * ATT_WARPS;
+constexpr int ATT_M = 16;                 // (row, head) pairs per CTA
+
+struct AttnParams {
+    const void *q;
+    void *out;
+    int8_t *out_q;
+    const uint8_t *k, *v;
+    const float *ks, *vs;
+    int64_t ldq, ldo, seq_stride, scale_seq_stride;
+    const int32_t *row_start, *past;
+    int32_t rows, max_rows, H, G, max_seq, nblk;   // G: heads per kv head
+    int32_t splits, tiles;
+    int32_t block_shift;                           // log2 of the tokens per scale
+    float scale;
+    float *part_o;                                 // [tile][split][16][D] unnormalised outputs
+    float2 *part_ml;                               // [tile][split][16] maximum (log2 units) and sum
+    int *err;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ uint4 ldg16(const uint8_t *p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint2 ldg8(const uint8_t *p) {
+    uint2 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    return v;
+}
+// four codes to two fp16 pairs (bytes 0,1 and 2,3)
+template <int CODE> __device__ __forceinline__ void codes_f16(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    if (CODE == Q35_CODE_INT8) {
+        // 0x64xx is the fp16 number 1024 + xx: biased bytes, minus 1024 + 128, exactly
+        const uint32_t u = w ^ 0x80808080u;
+        const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+        asm("sub.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(a), "r"(0x64806480u));
+        asm("sub.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(b), "r"(0x64806480u));
+    } else {
+        asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+            : "=r"(lo), "=r"(hi) : "r"(w));
+    }
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9},"
+                 " {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+
+template <int D> struct AttnShape {
+    static constexpr int KC = 4096 / D;        // keys per warp and step: 64, 32, 16
+    static constexpr int KS = D / 16;          // k-steps of Q K^T
+    static constexpr int ROWS_O = D + 4;       // padded row of the merge buffer, floats
+};
+template <int D> constexpr size_t attn_smem(int terms) {
+    // Q fragments, then (after the key loop) the merge buffer, in the same bytes
+    const size_t qf = (size_t)terms * AttnShape<D>::KS * 32 * 16;
+    const size_t mg = (size_t)ATT_WARPS * ATT_M * AttnShape<D>::ROWS_O * 4;
+    return qf > mg ? qf : mg;
+}
+
+// quant127's caller-visible form: int8 trunc(127 o), clamped
+template <typename T, int D>
+__device__ __forceinline__ void store_out(const AttnParams &p, int64_t row, int head, int d, float v) {
+    if (p.out_q) p.out_q[(row * p.H + head) * D + d] = quant127(v);
+    else static_cast<T *>(p.out)[row * p.ldo + (int64_t)head * D + d] = from_f32<T>(v);
+}
+
+// grid (split, tile of 16 (row, head) pairs, seq * kv_heads + kv head)
+template <typename T, int CODE, int D>
+__global__ void __launch_bounds__(ATT_THREADS, 1) kv8_attn_kernel(const AttnParams p) {
+    constexpr int TERMS = std::is_same<T, float>::value ? 2 : 1;
+    constexpr int KC = AttnShape<D>::KC, KS = AttnShape<D>::KS, NT = KC / 8, VT = D / 8;
+    constexpr int RO = AttnShape<D>::ROWS_O;
+    extern __shared__ __align__(16) uint8_t sm[];
+    __shared__ float qscale[ATT_M];
+    __shared__ float2 ml[ATT_WARPS][ATT_M];
+    uint32_t *qf = reinterpret_cast<uint32_t *>(sm);   // [TERMS][KS][32][4]
+    float *mg = reinterpret_cast<float *>(sm);         // [ATT_WARPS][16][RO]
+
+    const int split = blockIdx.x, mt = blockIdx.y;
+    const int KVH = p.H / p.G;
+    const int seq = blockIdx.z / KVH, kvh = blockIdx.z - seq * KVH;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const SeqRows sr = seq_rows(p.row_start, p.past, seq, p.rows, p.max_rows, p.max_seq, p.err);
+    const int f0 = mt * ATT_M;                          // first (row, head) pair of the tile
+    const int fn = min(ATT_M, sr.n * p.G - f0);
+    if (fn <= 0) return;
+    const int64_t tile = (int64_t)blockIdx.z * gridDim.y + mt;
+
+    // keys of this CTA: an equal share of the keys the tile's last row sees
+    const int kend_all = sr.past + (f0 + fn - 1) / p.G + 1;
+    const int steps = (kend_all + KC - 1) / KC;
+    const int k0 = (int)((int64_t)steps * split / p.splits) * KC;
+    const int k1 = min(kend_all, (int)((int64_t)steps * (split + 1) / p.splits) * KC);
+
+    // Q rows: a power of two brings each row's largest element to 2^13..2^14
+    for (int r = warp; r < ATT_M; r += ATT_WARPS) {
+        const int f = f0 + r;
+        const bool live = r < fn;
+        const T *src = static_cast<const T *>(p.q) + (live ? (int64_t)(sr.r0 + f / p.G) * p.ldq +
+                                                                 (int64_t)(kvh * p.G + f % p.G) * D : 0);
+        float x[D / 32], a = 0.0f;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+            x[i] = live ? to_f32<T>(src[lane + 32 * i]) : 0.0f;
+            a = fmaxf(a, fabsf(x[i]));
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+        const int e = min(126, 13 - ((int)(__float_as_uint(a) >> 23) - 127));
+        const float up = a > 0.0f ? __uint_as_float((uint32_t)(e + 127) << 23) : 1.0f;
+        if (lane == 0) qscale[r] = p.scale * 1.4426950408889634f * (a > 0.0f ? __uint_as_float((uint32_t)(127 - e) << 23) : 1.0f);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+            const int d = lane + 32 * i;
+            const int ks = (d / 64) * 4 + (d % 16) / 4, ln = (r % 8) * 4 + (d % 64) / 16;
+            const int reg = (d & 2) + (r >> 3), half = d & 1;
+            const float y = x[i] * up;
+            const __half hi = __float2half_rn(y);
+            __half *dst = reinterpret_cast<__half *>(qf + ((ks * 32 + ln) * 4 + reg)) + half;
+            *dst = hi;
+            if (TERMS == 2) dst[KS * 32 * 8] = __float2half_rn(y - __half2float(hi));
+        }
+    }
+    __syncthreads();
+
+    // rows g and g + 8 of the tile: limits, scales, running maximum and sum
+    int lim[2];
+    float qs[2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int r = g + 8 * h;
+        lim[h] = r < fn ? sr.past + (f0 + r) / p.G + 1 : 0;
+        qs[h] = qscale[r];
+    }
+    const int64_t hb = seq * p.seq_stride + (int64_t)kvh * p.max_seq * D;
+    const uint8_t *kb = p.k + hb, *vb = p.v + hb;
+    const int64_t sb = seq * p.scale_seq_stride + (int64_t)kvh * p.nblk;
+    const float *ksb = p.ks + sb, *vsb = p.vs + sb;
+
+    float o[VT][4];
+#pragma unroll
+    for (int t = 0; t < VT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[t][i] = 0.0f;
+    float vref = 0.0f, vinv = 0.0f;             // largest v scale so far and its reciprocal
+
+    constexpr int KL = D / 64;                  // 16-byte loads per key and lane: 1, 2, 4
+    uint4 kr[NT][KL];                           // K codes of a step: key 8t + g, bytes 64 j + 16 c ..
+    constexpr int VW = D == 64 ? 2 : 4;         // words per V load
+    constexpr int VL = D == 256 ? 2 : 1;
+    uint32_t vr[NT / 2][4][VL][VW];             // V codes: keys 16 s + 2c, +1, +8, +9, bytes 16 g (8 g) ..
+
+    auto load_k = [&](int kk) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const uint8_t *a = kb + (int64_t)min(kk + 8 * t + g, k1 - 1) * D + 16 * c;
+#pragma unroll
+            for (int j = 0; j < KL; ++j) kr[t][j] = ldg16(a + 64 * j);
+        }
+    };
+    auto load_v = [&](int kk) {
+#pragma unroll
+        for (int s = 0; s < NT / 2; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int key = kk + 16 * s + 2 * c + (i & 1) + 8 * (i >> 1);
+                const uint8_t *a = vb + (int64_t)min(key, k1 - 1) * D;
+                if constexpr (D == 64) {
+                    const uint2 u = ldg8(a + 8 * g);
+                    vr[s][i][0][0] = u.x; vr[s][i][0][1] = u.y;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < VL; ++j) {
+                        const uint4 u = ldg16(a + 128 * j + 16 * g);
+                        vr[s][i][j][0] = u.x; vr[s][i][j][1] = u.y; vr[s][i][j][2] = u.z; vr[s][i][j][3] = u.w;
+                    }
+                }
+                if (key >= k1) {                // past the last key: whatever is stored there must not count
+#pragma unroll
+                    for (int j = 0; j < VL; ++j)
+#pragma unroll
+                        for (int w = 0; w < VW; ++w) vr[s][i][j][w] = 0u;
+                }
+            }
+    };
+
+    int kk = k0 + warp * KC;
+    if (kk < k1) { load_k(kk); load_v(kk); }
+    for (; kk < k1; kk += ATT_WARPS * KC) {
+        const int nk = kk + ATT_WARPS * KC;
+        float s[NT][4];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[t][i] = 0.0f;
+        // scores: k-step (j, i) takes byte quad i of load j
+#pragma unroll
+        for (int j = 0; j < KL; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint4 qa = *reinterpret_cast<const uint4 *>(qf + ((j * 4 + i) * 32 + lane) * 4);
+                uint4 ql;
+                if (TERMS == 2) ql = *reinterpret_cast<const uint4 *>(qf + ((KS + j * 4 + i) * 32 + lane) * 4);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    uint32_t b0, b1;
+                    codes_f16<CODE>(i == 0 ? kr[t][j].x : i == 1 ? kr[t][j].y : i == 2 ? kr[t][j].z : kr[t][j].w, b0, b1);
+                    mma16816(s[t], qa, b0, b1);
+                    if (TERMS == 2) mma16816(s[t], ql, b0, b1);
+                }
+            }
+        // scales of the step's 16-key pieces (blocks hold 16 tokens or more)
+        float ksc[NT / 2], vsc[NT / 2], vtop = vref;
+#pragma unroll
+        for (int u = 0; u < NT / 2; ++u) {
+            const int key = kk + 16 * u;
+            ksc[u] = key < k1 ? ksb[key >> p.block_shift] : 0.0f;
+            vsc[u] = key < k1 ? vsb[key >> p.block_shift] : 0.0f;
+            vtop = fmaxf(vtop, vsc[u]);
+        }
+        if (nk < k1) load_k(nk);
+        float mx[2] = {m[0], m[1]};
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int key = kk + 8 * t + 2 * c + (i & 1), h = i >> 1;
+                s[t][i] = key < lim[h] && key < k1 ? s[t][i] * (qs[h] * ksc[t / 2]) : -INFINITY;
+                mx[h] = fmaxf(mx[h], s[t][i]);
+            }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+        }
+        // the outputs so far move to the new maximum and the new reference v scale
+        if (vtop > vref) vinv = 1.0f / vtop;
+        const float vdown = vtop > vref ? vref * vinv : 1.0f;
+        vref = vtop;
+        float mu[2], down[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            mu[h] = mx[h] == -INFINITY ? 0.0f : mx[h];     // a row that has seen no key yet
+            down[h] = ex2(m[h] - mu[h]);
+            l[h] *= down[h];
+            down[h] *= vdown;
+            m[h] = mx[h];
+        }
+#pragma unroll
+        for (int t = 0; t < VT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[t][i] *= down[i >> 1];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float e = ex2(s[t][i] - mu[i >> 1]);
+                l[i >> 1] += e;
+                s[t][i] = e;
+            }
+        // outputs
+#pragma unroll
+        for (int u = 0; u < NT / 2; ++u) {
+            const float w = vsc[u] == vref ? 1.0f : vsc[u] * vinv;
+            uint4 pa, pl;
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { x[i] = s[2 * u][i] * w; x[4 + i] = s[2 * u + 1][i] * w; }
+            pa = make_uint4(pack2<__half>(x[0], x[1]), pack2<__half>(x[2], x[3]), pack2<__half>(x[4], x[5]),
+                            pack2<__half>(x[6], x[7]));
+            if (TERMS == 2) {
+                uint32_t *hp = reinterpret_cast<uint32_t *>(&pa), *lp = reinterpret_cast<uint32_t *>(&pl);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 hf = __half22float2(*reinterpret_cast<const __half2 *>(&hp[i]));
+                    lp[i] = pack2<__half>((x[2 * i] - hf.x) * 2048.0f, (x[2 * i + 1] - hf.y) * 2048.0f);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < VL; ++j)
+#pragma unroll
+                for (int w4 = 0; w4 < VW; ++w4) {
+                    // keys 2c, 2c+1 interleaved byte by byte, and keys 2c+8, 2c+9
+                    const uint32_t a0 = vr[u][0][j][w4], a1 = vr[u][1][j][w4], a2 = vr[u][2][j][w4], a3 = vr[u][3][j][w4];
+#pragma unroll
+                    for (int hh = 0; hh < 2; ++hh) {
+                        uint32_t b0, b1, b2, b3;
+                        codes_f16<CODE>(__byte_perm(a0, a1, hh ? 0x7362 : 0x5140), b0, b1);
+                        codes_f16<CODE>(__byte_perm(a2, a3, hh ? 0x7362 : 0x5140), b2, b3);
+                        const int t = (j * VW + w4) * 4 + 2 * hh;
+                        mma16816(o[t], pa, b0, b2);
+                        mma16816(o[t + 1], pa, b1, b3);
+                        if (TERMS == 2) {
+                            // the low terms carry a factor 2^11 that keeps them in fp16's normal range
+                            float lo0[4] = {0, 0, 0, 0}, lo1[4] = {0, 0, 0, 0};
+                            mma16816(lo0, pl, b0, b2);
+                            mma16816(lo1, pl, b1, b3);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                o[t][i] = fmaf(lo0[i], 1.0f / 2048.0f, o[t][i]);
+                                o[t + 1][i] = fmaf(lo1[i], 1.0f / 2048.0f, o[t + 1][i]);
+                            }
+                        }
+                    }
+                }
+        }
+        if (nk < k1) load_v(nk);
+    }
+
+    // merge the warps: every warp's rows relative to its own maximum
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+        if (c == 0) ml[warp][g + 8 * h] = make_float2(m[h], l[h]);
+    }
+    __syncthreads();       // Q fragments are read no more
+#pragma unroll
+    for (int t = 0; t < VT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int n = 2 * c + (i & 1);      // column tile t, column n: see load_v
+            const int d = D == 64 ? n * 8 + t : (t / 16) * 128 + n * 16 + t % 16;
+            mg[(warp * ATT_M + g + 8 * (i >> 1)) * RO + d] = o[t][i] * vref;
+        }
+    __syncthreads();
+    for (int r = warp; r < fn; r += ATT_WARPS) {
+        float mm = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < ATT_WARPS; ++w) mm = fmaxf(mm, ml[w][r].x);
+        const float mu = mm == -INFINITY ? 0.0f : mm;
+        float sum = 0.0f, f[ATT_WARPS];
+#pragma unroll
+        for (int w = 0; w < ATT_WARPS; ++w) {
+            f[w] = ex2(ml[w][r].x - mu);
+            sum = fmaf(ml[w][r].y, f[w], sum);
+        }
+        const int fr = f0 + r;
+        const int64_t slot = (tile * p.splits + split) * ATT_M + r;
+        if (p.splits > 1 && lane == 0) p.part_ml[slot] = make_float2(mm, sum);
+        const float inv = 1.0f / sum;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+            const int d = lane + 32 * i;
+            float v = 0.0f;
+#pragma unroll
+            for (int w = 0; w < ATT_WARPS; ++w) v = fmaf(mg[(w * ATT_M + r) * RO + d], f[w], v);
+            if (p.splits > 1) p.part_o[slot * D + d] = v;
+            else store_out<T, D>(p, sr.r0 + fr / p.G, kvh * p.G + fr % p.G, d, v * inv);
+        }
+    }
+}
+
+// joins the splits of a tile: grid (16 rows of a tile, tile, seq * kv_heads + kv head), one warp
+template <typename T, int D>
+__global__ void __launch_bounds__(32) kv8_combine_kernel(const AttnParams p) {
+    const int r = blockIdx.x, mt = blockIdx.y, lane = threadIdx.x;
+    const int KVH = p.H / p.G;
+    const int seq = blockIdx.z / KVH, kvh = blockIdx.z - seq * KVH;
+    const SeqRows sr = seq_rows(p.row_start, p.past, seq, p.rows, p.max_rows, p.max_seq, p.err);
+    const int f = mt * ATT_M + r;
+    if (f >= sr.n * p.G) return;
+    const int64_t tile = (int64_t)blockIdx.z * gridDim.y + mt;
+    const int64_t slot0 = tile * p.splits * ATT_M + r;
+    float mm = -INFINITY;
+    for (int s = 0; s < p.splits; ++s) mm = fmaxf(mm, p.part_ml[slot0 + (int64_t)s * ATT_M].x);
+    float sum = 0.0f, v[D / 32] = {};
+    for (int s = 0; s < p.splits; ++s) {
+        const int64_t slot = slot0 + (int64_t)s * ATT_M;
+        const float2 a = p.part_ml[slot];
+        const float f2 = ex2(a.x - mm);
+        sum = fmaf(a.y, f2, sum);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) v[i] = fmaf(p.part_o[slot * D + lane + 32 * i], f2, v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+        store_out<T, D>(p, sr.r0 + f / p.G, kvh * p.G + f % p.G, lane + 32 * i, v[i] / sum);
+}
+
+
+struct AttnPlan { int mtiles, splits; int64_t tiles; size_t ml_bytes, o_bytes; };
+
+// splits: enough CTAs for every SM, at least one step of every warp each
+AttnPlan attn_plan(const q35_kv8_cache &c, int32_t heads, int32_t max_rows) {
+    AttnPlan pl;
+    const int G = heads / c.kv_heads;
+    pl.mtiles = (int)ceil_div((int64_t)max_rows * G, ATT_M);
+    pl.tiles = (int64_t)pl.mtiles * c.seqs * c.kv_heads;
+    const int64_t keys = (int64_t)ATT_WARPS * (4096 / c.head_dim);
+    pl.splits = (int)std::max<int64_t>(1, std::min<int64_t>(148 / std::max<int64_t>(1, pl.tiles), ceil_div(c.max_seq, keys)));
+    const int64_t slots = pl.splits > 1 ? pl.tiles * pl.splits * ATT_M : 0;
+    pl.ml_bytes = (size_t)round_up(slots * (int64_t)sizeof(float2), 256);
+    pl.o_bytes = (size_t)slots * c.head_dim * sizeof(float);
+    return pl;
+}
+
+template <typename T, int CODE, int D>
+int launch_attn(const AttnParams &p, const AttnPlan &pl, int zs, cudaStream_t s) {
+    const size_t smem = attn_smem<D>(std::is_same<T, float>::value ? 2 : 1);
+    static bool configured[64] = {};
+    int dev = 0;
+    Q35_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !configured[dev]) {
+        Q35_CUDA_TRY(cudaFuncSetAttribute(kv8_attn_kernel<T, CODE, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        if (dev >= 0 && dev < 64) configured[dev] = true;
+    }
+    kv8_attn_kernel<T, CODE, D><<<dim3(pl.splits, pl.mtiles, zs), ATT_THREADS, smem, s>>>(p);
+    Q35_CUDA_TRY(cudaGetLastError());
+    if (pl.splits > 1) {
+        kv8_combine_kernel<T, D><<<dim3(ATT_M, pl.mtiles, zs), 32, 0, s>>>(p);
+        Q35_CUDA_TRY(cudaGetLastError());
+    }
+    return Q35_OK;
+}
+
+template <typename T, int CODE>
+int launch_attn(const AttnParams &p, const AttnPlan &pl, int D, int zs, cudaStream_t s) {
+    if (D == 64) return launch_attn<T, CODE, 64>(p, pl, zs, s);
+    if (D == 128) return launch_attn<T, CODE, 128>(p, pl, zs, s);
+    return launch_attn<T, CODE, 256>(p, pl, zs, s);
+}
+template <typename T>
+int launch_attn(const AttnParams &p, const AttnPlan &pl, int code, int D, int zs, cudaStream_t s) {
+    return code == Q35_CODE_INT8 ? launch_attn<T, Q35_CODE_INT8>(p, pl, D, zs, s) : launch_attn<T, Q35_CODE_E4M3>(p, pl, D, zs, s);
+}
+
+template <typename T, int CODE, int D>
+int launch_append_b(const AppendParams &p, int block, dim3 grid, cudaStream_t s) {
+    switch (block) {
+    case 16: kv8_append_kernel<T, CODE, D, 16><<<grid, APPEND_THREADS, 0, s>>>(p); break;
+    case 32: kv8_append_kernel<T, CODE, D, 32><<<grid, APPEND_THREADS, 0, s>>>(p); break;
+    case 64: kv8_append_kernel<T, CODE, D, 64><<<grid, APPEND_THREADS, 0, s>>>(p); break;
+    default: kv8_append_kernel<T, CODE, D, 128><<<grid, APPEND_THREADS, 0, s>>>(p); break;
+    }
+    Q35_CUDA_TRY(cudaGetLastError());
+    return Q35_OK;
+}
+template <typename T, int CODE>
+int launch_append_d(const AppendParams &p, int D, int block, dim3 grid, cudaStream_t s) {
+    if (D == 64) return launch_append_b<T, CODE, 64>(p, block, grid, s);
+    if (D == 128) return launch_append_b<T, CODE, 128>(p, block, grid, s);
+    return launch_append_b<T, CODE, 256>(p, block, grid, s);
+}
+template <typename T>
+int launch_append_c(const AppendParams &p, int code, int D, int block, dim3 grid, cudaStream_t s) {
+    return code == Q35_CODE_INT8 ? launch_append_d<T, Q35_CODE_INT8>(p, D, block, grid, s)
+                                 : launch_append_d<T, Q35_CODE_E4M3>(p, D, block, grid, s);
+}
+
+int nblk(const q35_kv8_cache &c) { return (int)ceil_div(c.max_seq, c.block); }
+int64_t seq_stride(const q35_kv8_cache &c) {
+    return c.seq_stride ? c.seq_stride : (int64_t)c.kv_heads * c.max_seq * c.head_dim;
+}
+int64_t scale_seq_stride(const q35_kv8_cache &c) {
+    return c.scale_seq_stride ? c.scale_seq_stride : (int64_t)c.kv_heads * nblk(c);
+}
+
+int check_rows(const q35_kv8_cache &c, const Kv8Rows &r) {
+    if (r.rows < 0 || r.max_rows < 0 || r.max_rows > r.rows)
+        return set_error(Q35_ERR_INVALID, "kv8: rows and max_rows must satisfy 0 <= max_rows <= rows");
+    if (r.rows > 0 && r.max_rows == 0) return set_error(Q35_ERR_INVALID, "kv8: max_rows is 0");
+    if (r.max_rows > c.max_seq) return set_error(Q35_ERR_INVALID, "kv8: more rows than the cache has positions");
+    if (r.rows > 0 && (!r.row_start || !r.past)) return set_error(Q35_ERR_INVALID, "kv8: NULL row table");
+    return Q35_OK;
+}
+
+}  // namespace
+
+int kv8_check(const q35_kv8_cache *c) {
+    if (!c) return set_error(Q35_ERR_INVALID, "kv8: cache is NULL");
+    int st = check_code(c->code);
+    if (st) return st;
+    if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
+        return set_error(Q35_ERR_INVALID, "kv8: head_dim must be 64, 128 or 256");
+    if (c->block != 16 && c->block != 32 && c->block != 64 && c->block != 128)
+        return set_error(Q35_ERR_INVALID, "kv8: block must be 16, 32, 64 or 128 tokens");
+    if (c->seqs < 1 || c->kv_heads < 1 || c->max_seq < 1) return set_error(Q35_ERR_INVALID, "kv8: non-positive size");
+    if ((int64_t)c->seqs * c->kv_heads > 32767) return set_error(Q35_ERR_INVALID, "kv8: more than 32767 sequences x kv heads");
+    if (c->max_seq > (1 << 30)) return set_error(Q35_ERR_INVALID, "kv8: max_seq above 2^30");
+    if (!c->k || !c->v || !c->k_scale || !c->v_scale) return set_error(Q35_ERR_INVALID, "kv8: NULL cache array");
+    if (!aligned_to(c->k, 16) || !aligned_to(c->v, 16) || seq_stride(*c) % 16)
+        return set_error(Q35_ERR_INVALID, "kv8: codes must start on 16-byte boundaries");
+    if (!aligned_to(c->k_scale, 4) || !aligned_to(c->v_scale, 4))
+        return set_error(Q35_ERR_INVALID, "kv8: scales are not aligned");
+    if (c->seqs > 1 && (seq_stride(*c) < (int64_t)c->kv_heads * c->max_seq * c->head_dim ||
+                        scale_seq_stride(*c) < (int64_t)c->kv_heads * nblk(*c)))
+        return set_error(Q35_ERR_INVALID, "kv8: a sequence stride is below a sequence's size");
+    return Q35_OK;
+}
+
+int launch_kv8_append(const q35_kv8_cache &c, int dtype, const void *k, const void *v, int64_t ld, const Kv8Rows &r,
+                      int *err, cudaStream_t s) {
+    if (r.rows == 0) return Q35_OK;
+    AppendParams p;
+    p.x[0] = k; p.x[1] = v;
+    p.codes[0] = static_cast<uint8_t *>(c.k); p.codes[1] = static_cast<uint8_t *>(c.v);
+    p.scales[0] = c.k_scale; p.scales[1] = c.v_scale;
+    p.ld = ld;
+    p.seq_stride = seq_stride(c); p.scale_seq_stride = scale_seq_stride(c);
+    p.row_start = r.row_start; p.past = r.past;
+    p.rows = r.rows; p.max_rows = r.max_rows;
+    p.G = c.kv_heads; p.max_seq = c.max_seq; p.nblk = nblk(c);
+    p.err = err;
+    // blocks a run of max_rows tokens can touch, wherever it starts
+    const int bx = (int)((r.max_rows + (int64_t)c.block - 2) / c.block + 1);
+    const dim3 grid((unsigned)bx, (unsigned)c.kv_heads, (unsigned)(2 * c.seqs));
+    switch (dtype) {
+    case Q35_DT_F32: return launch_append_c<float>(p, c.code, c.head_dim, c.block, grid, s);
+    case Q35_DT_BF16: return launch_append_c<__nv_bfloat16>(p, c.code, c.head_dim, c.block, grid, s);
+    default: return launch_append_c<__half>(p, c.code, c.head_dim, c.block, grid, s);
+    }
+}
+
+size_t kv8_attention_workspace(const q35_kv8_cache &c, int32_t heads, int32_t rows, int32_t max_rows) {
+    if (rows <= 0) return 0;
+    const AttnPlan pl = attn_plan(c, heads, max_rows);
+    return pl.ml_bytes + pl.o_bytes;
+}
+
+int launch_kv8_attention(const q35_kv8_cache &c, int dtype, const void *q, int64_t ldq, int32_t heads, void *out,
+                         int64_t ldo, int8_t *out_q, const Kv8Rows &r, float scale, void *workspace, int *err,
+                         cudaStream_t s) {
+    if (r.rows == 0) return Q35_OK;
+    const AttnPlan pl = attn_plan(c, heads, r.max_rows);
+    if (pl.mtiles > 65535) return set_error(Q35_ERR_INVALID, "kv8: too many rows in one call");
+    AttnParams p;
+    p.q = q; p.out = out; p.out_q = out_q;
+    p.k = static_cast<const uint8_t *>(c.k); p.v = static_cast<const uint8_t *>(c.v);
+    p.ks = c.k_scale; p.vs = c.v_scale;
+    p.ldq = ldq; p.ldo = ldo;
+    p.seq_stride = seq_stride(c); p.scale_seq_stride = scale_seq_stride(c);
+    p.row_start = r.row_start; p.past = r.past;
+    p.rows = r.rows; p.max_rows = r.max_rows;
+    p.H = heads; p.G = heads / c.kv_heads; p.max_seq = c.max_seq; p.nblk = nblk(c);
+    p.splits = pl.splits; p.tiles = (int32_t)pl.tiles;
+    p.block_shift = c.block == 16 ? 4 : c.block == 32 ? 5 : c.block == 64 ? 6 : 7;
+    p.scale = scale;
+    p.part_ml = static_cast<float2 *>(workspace);
+    p.part_o = reinterpret_cast<float *>(static_cast<char *>(workspace) + pl.ml_bytes);
+    p.err = err;
+    const int zs = c.seqs * c.kv_heads;
+    switch (dtype) {
+    case Q35_DT_F32: return launch_attn<float>(p, pl, c.code, c.head_dim, zs, s);
+    case Q35_DT_BF16: return launch_attn<__nv_bfloat16>(p, pl, c.code, c.head_dim, zs, s);
+    default: return launch_attn<__half>(p, pl, c.code, c.head_dim, zs, s);
+    }
+}
+
+}  // namespace q35
+
+using namespace q35;
+
+extern "C" {
+
+int q35_kv8_append_dev(q35_ctx ctx, const q35_kv8_cache *cache, int dtype, const void *k, const void *v, int64_t ld,
+                       const int32_t *row_start, const int32_t *past, int32_t rows, int32_t max_rows) {
+    if (!ctx) return set_error(Q35_ERR_INVALID, "kv8_append: ctx is NULL");
+    int st = kv8_check(cache);
+    if (!st) st = check_dtype(dtype);
+    if (st) return st;
+    const Kv8Rows r{row_start, past, rows, max_rows};
+    st = check_rows(*cache, r);
+    if (st) return st;
+    if (rows == 0) return Q35_OK;
+    if (!k || !v) return set_error(Q35_ERR_INVALID, "kv8_append: NULL argument");
+    if (ld < (int64_t)cache->kv_heads * cache->head_dim)
+        return set_error(Q35_ERR_INVALID, "kv8_append: the row stride is below kv_heads * head_dim");
+    if (!aligned_to(k, dtype_size(dtype)) || !aligned_to(v, dtype_size(dtype)))
+        return set_error(Q35_ERR_INVALID, "kv8_append: a pointer is not aligned to its elements");
+    DeviceGuard g(ctx->device);
+    st = ensure_workspace(ctx, 0, 0);
+    if (st) return st;
+    return launch_kv8_append(*cache, dtype, k, v, ld, r, ctx->ws.err, ctx->stream);
+}
+
+int64_t q35_kv8_attention_workspace(const q35_kv8_cache *cache, int32_t heads, int32_t rows, int32_t max_rows) {
+    if (kv8_check(cache)) return -1;
+    if (heads < 1 || heads % cache->kv_heads) {
+        set_error(Q35_ERR_INVALID, "kv8_attention: heads must be a multiple of kv_heads");
+        return -1;
+    }
+    const int32_t dummy = 0;
+    if (check_rows(*cache, Kv8Rows{&dummy, &dummy, rows, max_rows})) return -1;
+    return (int64_t)kv8_attention_workspace(*cache, heads, rows, max_rows);
+}
+
+int q35_kv8_attention_dev(q35_ctx ctx, const q35_kv8_cache *cache, int dtype, const void *q, int64_t ldq,
+                          int32_t heads, void *out, int64_t ldo, const int32_t *row_start, const int32_t *past,
+                          int32_t rows, int32_t max_rows, float scale, void *workspace, size_t workspace_bytes) {
+    if (!ctx) return set_error(Q35_ERR_INVALID, "kv8_attention: ctx is NULL");
+    int st = kv8_check(cache);
+    if (!st) st = check_dtype(dtype);
+    if (st) return st;
+    if (heads < 1 || heads % cache->kv_heads)
+        return set_error(Q35_ERR_INVALID, "kv8_attention: heads must be a multiple of kv_heads");
+    const Kv8Rows r{row_start, past, rows, max_rows};
+    st = check_rows(*cache, r);
+    if (st) return st;
+    if (rows == 0) return Q35_OK;
+    if (!q || !out) return set_error(Q35_ERR_INVALID, "kv8_attention: NULL argument");
+    const int64_t width = (int64_t)heads * cache->head_dim;
+    if (ldq < width || ldo < width) return set_error(Q35_ERR_INVALID, "kv8_attention: a row stride is below heads * head_dim");
+    if (!aligned_to(q, dtype_size(dtype)) || !aligned_to(out, dtype_size(dtype)))
+        return set_error(Q35_ERR_INVALID, "kv8_attention: a pointer is not aligned to its elements");
+    if (!(scale == scale) || scale > 3.402823466e38f || scale < -3.402823466e38f)
+        return set_error(Q35_ERR_INVALID, "kv8_attention: scale is not finite");
+    const size_t need = kv8_attention_workspace(*cache, heads, rows, max_rows);
+    if (need > 0 && (!workspace || workspace_bytes < need || !aligned_to(workspace, 16)))
+        return set_error(Q35_ERR_INVALID, "kv8_attention: workspace missing, too small or not 16-byte aligned");
+    DeviceGuard g(ctx->device);
+    st = ensure_workspace(ctx, 0, 0);
+    if (st) return st;
+    return launch_kv8_attention(*cache, dtype, q, ldq, heads, out, ldo, nullptr, r, scale, workspace, ctx->ws.err,
+                                ctx->stream);
+}
+
+}  // extern "C"

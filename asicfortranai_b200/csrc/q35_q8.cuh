@@ -1,0 +1,72 @@
+// q35_q8.cuh -- what the 8-bit operators share (q35_norm8.cu, q35_fp8.cu, q35_kv8.cu,
+// q35_sample_filtered.cu): element types, the two 8-bit codes and their rounding,
+// argument checks.
+//
+// A code stands for code * scale.  scale = amax / Q in binary32 (Q = 127 for int8, 448 for
+// e4m3), and a value x is stored as the code nearest to x / scale: the binary32 quotient,
+// correctly rounded, then rounded to the code with ties to even and clamped to [-Q, Q].
+// Every step is an IEEE operation, so a plain program in binary32 gets the same codes.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "q35_internal.cuh"
+
+namespace q35 {
+
+constexpr int Q8_BLOCK = 128;   // elements per scale along a row (norm output, e4m3 product)
+
+inline size_t dtype_size(int dtype) { return dtype == Q35_DT_F32 ? 4 : 2; }
+inline int check_dtype(int dtype) {
+    if (dtype != Q35_DT_F32 && dtype != Q35_DT_BF16 && dtype != Q35_DT_F16)
+        return set_error(Q35_ERR_INVALID, "unknown element type");
+    return Q35_OK;
+}
+inline int check_code(int code) {
+    if (code != Q35_CODE_INT8 && code != Q35_CODE_E4M3) return set_error(Q35_ERR_INVALID, "unknown 8-bit code");
+    return Q35_OK;
+}
+inline bool aligned_to(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+#ifdef __CUDACC__
+template <typename T> __device__ __forceinline__ float to_f32(T v);
+template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <> __device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+
+// two floats to the packed pair of a 16-bit type (low half first)
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+
+template <int CODE> __device__ __forceinline__ constexpr float code_max() {
+    return CODE == Q35_CODE_INT8 ? 127.0f : 448.0f;
+}
+
+// the code nearest to v (ties to even, clamped); NaN gives 0 (int8) or NaN (e4m3)
+template <int CODE> __device__ __forceinline__ uint8_t encode8(float v) {
+    if (CODE == Q35_CODE_INT8) {
+        const int q = __float2int_rn(v);               // saturates; NaN gives 0
+        return (uint8_t)(int8_t)max(-127, min(127, q));
+    }
+    return (uint8_t)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
+}
+template <int CODE> __device__ __forceinline__ float decode8(uint8_t c) {
+    if (CODE == Q35_CODE_INT8) return (float)(int8_t)c;
+    const __half_raw h = __nv_cvt_fp8_to_halfraw(c, __NV_E4M3);
+    return __half2float(__half(h));
+}
+#endif
+
+}  // namespace q35

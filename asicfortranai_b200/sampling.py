@@ -6,11 +6,13 @@ draw runs on the GPU in one fused kernel (q35_sample.cu).
     tok = sample_top_k(logits, vocab_size, 40)            # :123-176
     tok = sample_top_p(logits, vocab_size, 0.95)          # :181-259
     toks = sample_rows(ctx, "top_p", logits_dev, u_dev, top_p=0.95)   # device rows
+    sample_filtered_rows(ctx, logits_dev, rows, vocab, u_dev, tokens_dev, temperature=..., top_k=...,
+                         top_p=..., min_p=...)   # all filters at once, parameters per row
 
 Tokens are 1-based, as in the reference.  ``random_number`` is replaced by the uniform
 draw ``u`` in [0, 1): pass it for a reproducible draw, or leave it None to take one from
 ``rng`` (a numpy Generator; numpy's default generator when None).  Vocabularies up to
-32,768.
+32,768 (sample_filtered_rows: 4,194,304).
 """
 from __future__ import annotations
 
@@ -72,3 +74,19 @@ def sample_rows(ctx, mode, logits_ptr: int, rows: int, vocab: int, u_ptr: int, t
     m = MODES[mode] if isinstance(mode, str) else int(mode)
     _lib.check(_lib.load().q35_sample_dev(ctx.h, m, logits_ptr, rows, vocab, temperature, top_k, top_p,
                                           u_ptr, tokens_ptr), "q35_sample_dev")
+
+
+def sample_filtered_rows(ctx, logits_ptr: int, rows: int, vocab: int, u_ptr: int, tokens_ptr: int,
+                         temperature: int | None = None, top_k: int | None = None, top_p: int | None = None,
+                         min_p: int | None = None, probs: int | None = None, dtype: str = "f32",
+                         ld: int | None = None) -> None:
+    """Temperature, top-k, top-p and min-p together (q35_sample_filtered_dev): every argument
+    but the sizes is a device pointer; temperature, top_p, min_p, u (fp32) and top_k (int32)
+    hold one value per row, None turns a filter off.  tokens[rows] int32 gets 1-based tokens
+    (0 where every logit is -inf or NaN), probs[rows] fp32 their probabilities among the kept
+    ones.  dtype of the logits: "f32", "bf16" or "f16"; rows ld elements apart (default
+    vocab).  Enqueued on ctx's stream."""
+    _lib.check(_lib.load().q35_sample_filtered_dev(ctx.h, _lib.dtype_code(dtype), logits_ptr,
+                                                   vocab if ld is None else ld, rows, vocab, temperature, top_k,
+                                                   top_p, min_p, u_ptr, tokens_ptr, probs),
+               "q35_sample_filtered_dev")

@@ -54,6 +54,15 @@ enum {
     Q35_SAMPLE_TOP_P = 3         /* sample_top_p, :181-259 */
 };
 
+/* element types of the 8-bit operators' activations, outputs and logits */
+enum { Q35_DT_F32 = 0, Q35_DT_BF16 = 1, Q35_DT_F16 = 2 };
+
+/* 8-bit codes; a code stands for code * scale */
+enum {
+    Q35_CODE_INT8 = 0,  /* -127 .. 127 */
+    Q35_CODE_E4M3 = 1   /* 8-bit float, 4 exponent and 3 mantissa bits, largest 448 */
+};
+
 typedef struct q35_ctx_s *q35_ctx;         /* device, stream, split-K workspace */
 typedef struct q35_weights_s *q35_weights; /* one device-resident quantized matrix */
 typedef struct q35_graph_s *q35_graph;     /* an instantiated CUDA graph of captured calls */
@@ -211,6 +220,95 @@ int q35_sample_top_p(q35_ctx ctx, const float *logits, int32_t vocab, float p, f
  * enqueued on ctx's stream, no synchronisation */
 int q35_sample_dev(q35_ctx ctx, int32_t mode, const float *logits, int32_t rows, int32_t vocab, float temperature,
                    int32_t top_k, float top_p, const float *u, int32_t *tokens);
+
+/* Sampling with temperature, top-k, top-p and min-p together, per row, on the device (no
+ * counterpart in the reference, whose strategies exclude one another).  logits[rows][ld] of
+ * dtype (Q35_DT_*), vocab of them used, vocab <= 4,194,304.  Per row r, from device arrays
+ * (NULL: the filter is off for every row):
+ *   temperature[r] (NULL: 1; <= 0 or NaN: the first maximum);
+ *   top_k[r]: the k largest logits, equal ones lowest index first (<= 0: off);
+ *   top_p[r]: of those, in descending order, the shortest prefix whose mass reaches p times
+ *             theirs (>= 1: off; <= 0: the first maximum);
+ *   min_p[r]: of those, the ones with at least min_p times the largest probability (<= 0:
+ *             off; above 1: the first maximum);
+ * then the first kept index, in index order, whose running mass passes u[r] times the kept
+ * mass, u in [0,1).  tokens[r] is 1-based; probs[r] (may be NULL) gets the token's
+ * probability among the kept ones.  -infinity and NaN logits are never drawn; a row of
+ * nothing else gives token 0 and probability 0.  Masses are exact sums of 2^-40 of the
+ * largest weight.  Enqueued on ctx's stream, no synchronisation, no workspace. */
+int q35_sample_filtered_dev(q35_ctx ctx, int dtype, const void *logits, int64_t ld, int32_t rows,
+                            int32_t vocab, const float *temperature, const int32_t *top_k,
+                            const float *top_p, const float *min_p, const float *u, int32_t *tokens,
+                            float *probs);
+
+/* ---- 8-bit operators of a serving step on device arrays (no counterpart in the reference) ----
+ * All are enqueued on ctx's stream without synchronisation and allocate nothing after the
+ * context's first call, so they can be captured into graphs. */
+
+/* RMSNorm of x + residual with an 8-bit output:
+ *   h = x + residual (residual NULL: h = x), in fp32; stored rounded to dtype in residual_out
+ *   (may be NULL; may be x or residual themselves);
+ *   y = h / sqrt(mean(h^2) + eps) * weight;
+ *   scales[row][g] = max |y| over group g / (127 or 448), q = the code nearest to y / scale
+ *   (ties to even; scale 0: codes 0).  A row with a NaN or infinite element gets NaN scales.
+ * x, residual, residual_out: dtype, [rows] of dim elements ldx, ldr, ldo apart; q: codes, ldq
+ * apart; weight fp32 [dim]; group: 128 elements (scales [rows][ceil(dim/128)], the x_scales of
+ * q35_fp8_gemm_dev) or 0, the whole row (scales [rows]).  dim <= 32768. */
+int q35_rms_norm_quant_dev(q35_ctx ctx, int dtype, const void *x, int64_t ldx, const void *residual,
+                           int64_t ldr, void *residual_out, int64_t ldo, const float *weight, float eps,
+                           int32_t rows, int32_t dim, int code, int32_t group, void *q, int64_t ldq,
+                           float *scales);
+
+/* Matrix product in e4m3 with a scale for each block of 128:
+ *   y[m][n] = sum_b x_scales[m][b] * w_scales[n/128][b] * sum over k in block b of x[m][k] w[n][k]
+ * x [M] rows of K codes ldx apart with x_scales [M][ceil(K/128)]; w [N] rows of K codes ldw
+ * apart with w_scales [ceil(N/128)][ceil(K/128)]; y dtype, [M] rows of N elements ldy apart.
+ * Rows of x and w start on 16-byte boundaries (base and stride); K need not be a multiple of
+ * anything (bytes between K and the stride are not used).  M <= 65536, K <= 131072,
+ * N <= 2^24; M = 0 or N = 0 does nothing. */
+int q35_fp8_gemm_dev(q35_ctx ctx, const void *x, int64_t ldx, const float *x_scales, const void *w,
+                     int64_t ldw, const float *w_scales, int dtype, void *y, int64_t ldy, int32_t M,
+                     int32_t N, int32_t K);
+
+/* A KV cache held in 8 bits with a scale for each block of tokens and head.  The arrays are
+ * the caller's, on the device. */
+typedef struct {
+    int32_t code;                     /* Q35_CODE_* */
+    int32_t seqs, kv_heads, head_dim; /* head_dim 64, 128 or 256 */
+    int32_t max_seq, block;           /* positions; tokens per scale: 16, 32, 64 or 128 */
+    void *k, *v;                      /* codes [seq][kv_head][max_seq][head_dim], 16-byte aligned */
+    float *k_scale, *v_scale;         /* [seq][kv_head][ceil(max_seq / block)] */
+    int64_t seq_stride;               /* codes between sequences (multiple of 16; 0: dense) */
+    int64_t scale_seq_stride;         /* scales between sequences (0: dense) */
+} q35_kv8_cache;
+
+/* Rows of several sequences: row_start[seqs + 1] and past[seqs] on the device; rows
+ * row_start[s] .. row_start[s+1]-1 are the tokens of sequence s at positions past[s], past[s]+1,
+ * ...; a sequence may have none.  rows: how many in all, max_rows: at least the most of one
+ * sequence.  A sequence whose entries contradict this, or whose tokens would pass max_seq, is
+ * left out and recorded (Q35_ERR_INVALID from q35_ctx_device_error).
+ *
+ * Appends k and v (dtype, [rows] of kv_heads * head_dim elements, ld apart).  A block's scale
+ * becomes max(scale, max |new| / (127 or 448)), counting from 0 for a block without older
+ * tokens; where it grew the block's older codes are rounded again.  Infinities are stored as
+ * the largest code, NaN as 0.  q35_kv8_append_dev neither reads nor writes anything behind a
+ * sequence's last token but the scale of its last block. */
+int q35_kv8_append_dev(q35_ctx ctx, const q35_kv8_cache *cache, int dtype, const void *k, const void *v,
+                       int64_t ld, const int32_t *row_start, const int32_t *past, int32_t rows,
+                       int32_t max_rows);
+/* Causal attention of the rows' queries over the cache, which already holds the rows' own
+ * tokens: out[row][h] = sum_j softmax_j(scale * q[row][h] . k[h / (heads/kv_heads)][j]) v[..][j]
+ * over positions j up to the row's own.  q, out: dtype, [rows] of heads * head_dim elements, ldq
+ * and ldo apart; heads a multiple of kv_heads.  workspace: device memory of
+ * q35_kv8_attention_workspace bytes (16-byte aligned; may be NULL when that is 0), used by this
+ * call alone while it runs.  Nothing behind a sequence's last token counts, whatever it holds. */
+int q35_kv8_attention_dev(q35_ctx ctx, const q35_kv8_cache *cache, int dtype, const void *q, int64_t ldq,
+                          int32_t heads, void *out, int64_t ldo, const int32_t *row_start,
+                          const int32_t *past, int32_t rows, int32_t max_rows, float scale,
+                          void *workspace, size_t workspace_bytes);
+/* bytes of workspace for such a call, -1 for bad arguments */
+int64_t q35_kv8_attention_workspace(const q35_kv8_cache *cache, int32_t heads, int32_t rows,
+                                    int32_t max_rows);
 
 /* ---- LLaMA model (llama_model.f90, transformer_layer.f90, llama_generate.f90) ---- */
 typedef struct {
