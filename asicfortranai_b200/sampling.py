@@ -12,7 +12,7 @@ draw runs on the GPU in one fused kernel (q35_sample.cu).
 Tokens are 1-based, as in the reference.  ``random_number`` is replaced by the uniform
 draw ``u`` in [0, 1): pass it for a reproducible draw, or leave it None to take one from
 ``rng`` (a numpy Generator; numpy's default generator when None).  Vocabularies up to
-32,768 (sample_filtered_rows: 4,194,304).
+32,768 (sample_filtered_rows: 401,408).
 """
 from __future__ import annotations
 

@@ -223,7 +223,7 @@ int q35_sample_dev(q35_ctx ctx, int32_t mode, const float *logits, int32_t rows,
 
 /* Sampling with temperature, top-k, top-p and min-p together, per row, on the device (no
  * counterpart in the reference, whose strategies exclude one another).  logits[rows][ld] of
- * dtype (Q35_DT_*), vocab of them used, vocab <= 4,194,304.  Per row r, from device arrays
+ * dtype (Q35_DT_*), vocab of them used, vocab <= 401,408.  Per row r, from device arrays
  * (NULL: the filter is off for every row):
  *   temperature[r] (NULL: 1; <= 0 or NaN: the first maximum);
  *   top_k[r]: the k largest logits, equal ones lowest index first (<= 0: off);

@@ -530,10 +530,10 @@ ONE_MINUS = float(np.nextafter(F(1), F(0)))
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("V", [1, 2, 31, 33, 1000, 4097, 32000, 100277])
-def test_sampler(ctx, dtype, V):
+@pytest.mark.parametrize("V,R", [(1, 48), (2, 48), (31, 48), (33, 48), (1000, 48), (4097, 48), (32000, 48), (100277, 48),
+                                 (9000, 200), (131072, 5), (400001, 5), (401408, 5)])
+def test_sampler(ctx, dtype, V, R):
     rng = np.random.default_rng(V)
-    R = 48
     lg = rng.normal(0, 2.5, (R, V))
     lg[::5] = np.round(lg[::5] * 2) / 2                        # ties
     lg[1::7] = rng.normal(0, 0.01, (len(lg[1::7]), V))         # flat
