@@ -2,27 +2,30 @@
 // 128 along k of every row of x, and for each 128 x 128 block of w:
 //   y[m][n] = sum_b xs[m][b] ws[n / 128][b] sum_{k in block b} x[m][k] w[n][k]
 //
-// Tile: 128 rows of w (the MMA's M: one row of scale blocks, so ws is one number per tile
-// and k-block) x BN rows of x (the MMA's N).  Per 128-k block:
-//   * producer (warp 0, one thread): two 2D TMA loads, 128 bytes of k x 128 rows of w and
-//     x BN rows of x, 128-byte swizzle (rows past the edges and k past K read as zero);
-//   * scale loader (warp 2): xs[m][b] * ws[b] of the tile's BN rows into the stage;
+// Both kernels below run the same pipeline, per 128-k block:
+//   * producer (warp 0, one thread): two 2D TMA loads, 128 bytes of k x the tile's rows of w and
+//     of x, 128-byte swizzle (rows past the edges and k past K read as zero);
+//   * scale loader (warp 2): the products xs * ws of the tile's rows of x into the stage;
 //   * MMA issuer (warp 1, one thread): 4 x tcgen05.mma kind::f8f6f4 (K = 32 each) into one
 //     of several accumulators in tensor memory.  The sum over one block is a tensor-core
 //     fp32 sum of exact products;
 //   * promotion (warps 4 ..): tcgen05.ld of the block's sums, acc = fma(sum, scale, acc)
-//     with acc in registers -- a thread owns one row of w, the scales are read as broadcast
-//     pairs and two sums take one packed fma (fma.rn.f32x2).
+//     with acc in registers, two sums per packed fma (fma.rn.f32x2), the next columns' load
+//     on its way meanwhile.
 // A k-block's accumulator is handed over through mbarriers, so the MMAs of the next blocks
 // run under the promotion of this one.
 //
-// Few tiles (decode batches) are split along k over the CTAs of a cluster; each CTA then adds
-// up its share of the tile's columns from every CTA's shared memory, in CTA order, so the
-// result does not depend on timing.  Many tiles run on a persistent grid, the row tiles of
-// one w tile side by side so that w comes from HBM once.
+// fp8_gemm_kernel (few rows of x): w in the MMA's M position, 128 rows of w (one row of scale
+// blocks, so ws is one number per tile and k-block) x BN <= 256 rows of x; a thread owns a row
+// of w and reads the scales of x's rows as broadcast vectors.  Few tiles are split along k over
+// the CTAs of a cluster; each CTA then adds up its share of the tile's columns from every CTA's
+// shared memory, in CTA order, so the result does not depend on timing.
 //
-// With w in the MMA's M position a warp stores 32 consecutive n of a row of y, whatever y's
-// stride and type, without staging.
+// fp8_gemm_pair_kernel (many rows): two CTAs on one 256 x 256 tile (cta_group::2), x in the M
+// position, each CTA holding 128 rows of x and half of the tile's rows of w, so that an SM
+// reads 32 KB a k-block instead of 48 (shared memory's and L2's rates, not the MMAs, bound
+// the one-CTA form: 128 x 256 x 128 takes the tensor cores 512 clocks, 48 KB through 128 bytes a
+// clock in and out 768); a thread owns a row of x and one scale covers its 128 columns.
 //
 // Every wait is bounded: a wait that gives up records Q35_ERR_TIMEOUT in the context's error
 // word and raises an abort flag that ends the other roles' waits; copies and MMAs in flight
@@ -38,7 +41,7 @@ namespace {
 
 constexpr int F8_TN = 128;                 // rows of w per tile
 constexpr int F8_KB = 128;                 // k per block (bytes per row of a stage)
-constexpr uint32_t F8_WAIT = 1u << 26;
+constexpr uint32_t F8_WAIT = 1u << 24;
 
 struct F8Params {
     const float *xs, *ws;                  // [M][KB], [ceil(N/128)][KB]
@@ -103,15 +106,34 @@ __device__ __forceinline__ void tc_ld16(uint32_t taddr, float (&v)[16]) {
                    "=f"(v[14]), "=f"(v[15])
                  : "r"(taddr) : "memory");
 }
+__device__ __forceinline__ void tc_ld32(uint32_t taddr, float (&v)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32"
+                 " {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15,"
+                 " %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+                   "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]),
+                   "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]),
+                   "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]),
+                   "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+                 : "r"(taddr) : "memory");
+}
+// acc.x += a * s, acc.y += b * t in one packed instruction
+__device__ __forceinline__ void fma2(float2 &acc, float a, float b, float s, float t) {
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%0, %1};\n\t"
+        "fma.rn.f32x2 z, x, y, z;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "+f"(acc.x), "+f"(acc.y) : "f"(a), "f"(b), "f"(s), "f"(t));
+}
+template <int R> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R)); }
+template <int R> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 // K-major operand, 128-byte swizzle: 8-row atoms of 1024 bytes
 __device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t addr) {
     return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
            ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
-// D fp32, A and B e4m3, both K-major, M = 128
-__host__ __device__ constexpr uint32_t idesc_f8(int BN) {
-    return (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(F8_TN >> 4) << 24);
+// D fp32, A and B e4m3, both K-major
+__host__ __device__ constexpr uint32_t idesc_f8(int m, int n) {
+    return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
@@ -119,7 +141,14 @@ __device__ __forceinline__ uint32_t cluster_rank() {
     return r;
 }
 __device__ __forceinline__ void cluster_sync() {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// the address of a shared variable of this CTA in CTA rank's shared memory
+__device__ __forceinline__ uint32_t at_rank(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
 }
 __device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t rank, float v) {
     asm volatile("{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %0, %1;\n\t"
@@ -135,9 +164,10 @@ struct Ring {
 };
 
 // NB: accumulator registers (x rows) per promotion thread; 4 or 8 promotion warps, the second
-// four taking the upper half of the tile's columns
+// four taking the upper half of the tile's columns.  Tiles of up to 32 rows leave room for
+// two CTAs on an SM.
 template <typename T, int NB, int PW>
-__global__ void __launch_bounds__(128 + 32 * PW, 1)
+__global__ void __launch_bounds__(128 + 32 * PW, NB <= 32 ? 2 : 1)
 fp8_gemm_kernel(const F8Params p, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap) {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
@@ -173,6 +203,8 @@ fp8_gemm_kernel(const F8Params p, const __grid_constant__ CUtensorMap wmap, cons
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    dependency_trigger();
+    dependency_wait();
 
     const int rank = p.split > 1 ? (int)cluster_rank() : 0;
     const int first_tile = blockIdx.x / p.split, step = gridDim.x / p.split;
@@ -185,121 +217,138 @@ fp8_gemm_kernel(const F8Params p, const __grid_constant__ CUtensorMap wmap, cons
         atomicExch(p.err, Q35_ERR_TIMEOUT);
     };
 
-    constexpr int HB = NB;                       // columns per promotion thread
-    float2 acc[HB / 2];
-    if (warp == 0) {
-        if (lane == 0) {
+    // registers: 4 x 32 x 56 + 8 x 32 x 224 = 384 x 168
+    if (warp < 4) {
+        if (PW == 8) regs_down<56>();
+        if (warp == 0) {
+            if (lane == 0) {
+                Ring st{};
+                int64_t issued = 0;
+                for (int tile = first_tile; tile < tiles && ok; tile += step) {
+                    const int nt = tile / p.mt, mt = tile - nt * p.mt;
+                    for (int kb = kb0; kb < kb1; ++kb) {
+                        if (!mbar_wait(empty(st.i), st.ph ^ 1u, abort_flag)) { fail(); break; }
+                        mbar_expect_tx(full(st.i), stage_bytes);
+                        const uint32_t dst = base + (uint32_t)st.i * stage_bytes;
+                        tma_load_2d(dst, &wmap, kb * F8_KB, nt * F8_TN, full(st.i));
+                        tma_load_2d(dst + F8_TN * F8_KB, &xmap, kb * F8_KB, mt * BN, full(st.i));
+                        st.next(S);
+                        ++issued;
+                    }
+                }
+                // every copy has landed before the CTA leaves (after a failure too)
+                for (int64_t j = issued < S ? issued : S; j > 0; --j) {
+                    const int i = st.i >= j ? st.i - (int)j : st.i - (int)j + S;
+                    const uint32_t ph = st.i >= j ? st.ph : st.ph ^ 1u;
+                    for (uint32_t n = 0; n < (1u << 20) && !mbar_try_wait(full(i), ph); ++n) {}
+                }
+            }
+        } else if (warp == 2) {
+            // scales of a stage: xs[m][kb] * ws[nt][kb], several k-blocks' loads in flight at once
+            constexpr int SN = NB * (PW / 4), SL = (SN + 31) / 32, SB = SL > 4 ? 2 : 4;
             Ring st{};
-            int64_t issued = 0;
             for (int tile = first_tile; tile < tiles && ok; tile += step) {
                 const int nt = tile / p.mt, mt = tile - nt * p.mt;
-                for (int kb = kb0; kb < kb1; ++kb) {
-                    if (!mbar_wait(empty(st.i), st.ph ^ 1u, abort_flag)) { fail(); break; }
-                    mbar_expect_tx(full(st.i), stage_bytes);
-                    const uint32_t dst = base + (uint32_t)st.i * stage_bytes;
-                    tma_load_2d(dst, &wmap, kb * F8_KB, nt * F8_TN, full(st.i));
-                    tma_load_2d(dst + F8_TN * F8_KB, &xmap, kb * F8_KB, mt * BN, full(st.i));
-                    st.next(S);
-                    ++issued;
-                }
-            }
-            // every copy has landed before the CTA leaves (after a failure too)
-            for (int64_t j = issued < S ? issued : S; j > 0; --j) {
-                const int i = st.i >= j ? st.i - (int)j : st.i - (int)j + S;
-                const uint32_t ph = st.i >= j ? st.ph : st.ph ^ 1u;
-                for (uint32_t n = 0; n < (1u << 20) && !mbar_try_wait(full(i), ph); ++n) {}
-            }
-        }
-    } else if (warp == 2) {
-        // scales of a stage: xs[m][kb] * ws[nt][kb], four k-blocks' loads in flight at once
-        constexpr int SN = NB * (PW / 4), SL = (SN + 31) / 32, SB = 4;
-        Ring st{};
-        for (int tile = first_tile; tile < tiles && ok; tile += step) {
-            const int nt = tile / p.mt, mt = tile - nt * p.mt;
-            for (int kb = kb0; kb < kb1 && ok; kb += SB) {
-                float v[SB][SL];
+                for (int kb = kb0; kb < kb1 && ok; kb += SB) {
+                    float v[SB][SL];
 #pragma unroll
-                for (int b = 0; b < SB; ++b) {
-                    const bool live = kb + b < kb1;
-                    const float w = live ? p.ws[(int64_t)nt * p.KB + kb + b] : 0.0f;
+                    for (int b = 0; b < SB; ++b) {
+                        const bool live = kb + b < kb1;
+                        const float w = live ? p.ws[(int64_t)nt * p.KB + kb + b] : 0.0f;
 #pragma unroll
-                    for (int i = 0; i < SL; ++i) {
-                        const int j = lane + 32 * i, m = mt * BN + j;
-                        v[b][i] = live && j < BN && m < p.M ? p.xs[(int64_t)m * p.KB + kb + b] * w : 0.0f;
+                        for (int i = 0; i < SL; ++i) {
+                            const int j = lane + 32 * i, m = mt * BN + j;
+                            v[b][i] = live && j < BN && m < p.M ? p.xs[(int64_t)m * p.KB + kb + b] * w : 0.0f;
+                        }
+                    }
+#pragma unroll
+                    for (int b = 0; b < SB; ++b) {
+                        if (kb + b >= kb1) break;
+                        if (!__all_sync(0xffffffffu, mbar_wait(empty(st.i), st.ph ^ 1u, abort_flag))) { fail(); break; }
+                        float *sc = reinterpret_cast<float *>(sbase + p.off_sc) + st.i * SN;
+#pragma unroll
+                        for (int i = 0; i < SL; ++i)
+                            if (lane + 32 * i < SN) sc[lane + 32 * i] = v[b][i];
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(sc_full(st.i));
+                        st.next(S);
                     }
                 }
-#pragma unroll
-                for (int b = 0; b < SB; ++b) {
-                    if (kb + b >= kb1) break;
-                    if (!__all_sync(0xffffffffu, mbar_wait(empty(st.i), st.ph ^ 1u, abort_flag))) { fail(); break; }
-                    float *sc = reinterpret_cast<float *>(sbase + p.off_sc) + st.i * SN;
-#pragma unroll
-                    for (int i = 0; i < SL; ++i)
-                        if (lane + 32 * i < SN) sc[lane + 32 * i] = v[b][i];
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(sc_full(st.i));
-                    st.next(S);
-                }
             }
-        }
-    } else if (warp == 1) {
-        if (lane == 0) {
-            const uint32_t idesc = idesc_f8(BN);
-            Ring st{}, ab{};
-            for (int tile = first_tile; tile < tiles && ok; tile += step) {
-                for (int kb = kb0; kb < kb1; ++kb) {
-                    if (!mbar_wait(acc_empty(ab.i), ab.ph ^ 1u, abort_flag) || !mbar_wait(full(st.i), st.ph, abort_flag)) {
-                        fail();
-                        break;
+        } else if (warp == 1) {
+            if (lane == 0) {
+                const uint32_t idesc = idesc_f8(F8_TN, BN);
+                Ring st{}, ab{};
+                for (int tile = first_tile; tile < tiles && ok; tile += step) {
+                    for (int kb = kb0; kb < kb1; ++kb) {
+                        if (!mbar_wait(acc_empty(ab.i), ab.ph ^ 1u, abort_flag) || !mbar_wait(full(st.i), st.ph, abort_flag)) {
+                            fail();
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint32_t a0 = base + (uint32_t)st.i * stage_bytes, b0 = a0 + F8_TN * F8_KB;
+                        const uint32_t d = tmem + (uint32_t)ab.i * p.buf_cols;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            tc_mma_f8(d, smem_desc_sw128(a0 + 32u * j), smem_desc_sw128(b0 + 32u * j), idesc, j > 0 ? 1u : 0u);
+                        tc_commit(empty(st.i));
+                        tc_commit(acc_full(ab.i));
+                        st.next(S);
+                        ab.next(NBUF);
                     }
-                    tc_fence_after();
-                    const uint32_t a0 = base + (uint32_t)st.i * stage_bytes, b0 = a0 + F8_TN * F8_KB;
-                    const uint32_t d = tmem + (uint32_t)ab.i * p.buf_cols;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        tc_mma_f8(d, smem_desc_sw128(a0 + 32u * j), smem_desc_sw128(b0 + 32u * j), idesc, j > 0 ? 1u : 0u);
-                    tc_commit(empty(st.i));
-                    tc_commit(acc_full(ab.i));
-                    st.next(S);
-                    ab.next(NBUF);
                 }
+                // every MMA issued has completed before the CTA moves on
+                tc_commit(drain);
+                if (!mbar_wait(drain, 0, abort_flag)) fail();
             }
-            // every MMA issued has completed before the CTA moves on
-            tc_commit(drain);
-            if (!mbar_wait(drain, 0, abort_flag)) fail();
         }
-    } else if (warp >= 4) {
+        if (p.split > 1) {
+            cluster_sync();
+            cluster_sync();
+        }
+    } else {
+        if (PW == 8) regs_up<224>();
         const int q = warp & 3, half = (warp - 4) >> 2;
         const int c0 = half * NB;                       // first column of this thread
+        float2 acc[NB / 2];
         Ring st{}, ab{};
         for (int tile = first_tile; tile < tiles && ok; tile += step) {
             const int nt = tile / p.mt, mt = tile - nt * p.mt;
 #pragma unroll
-            for (int i = 0; i < HB / 2; ++i) acc[i] = make_float2(0.0f, 0.0f);
+            for (int i = 0; i < NB / 2; ++i) acc[i] = make_float2(0.0f, 0.0f);
             for (int kb = kb0; kb < kb1; ++kb) {
                 // (the stage cannot be refilled before this warp arrives on it, so its phase
                 // is still the one to wait for)
-                if (!__all_sync(0xffffffffu, mbar_wait(acc_full(ab.i), ab.ph, abort_flag) &&
-                                                 mbar_wait(sc_full(st.i), st.ph, abort_flag))) { fail(); break; }
+                if (!__all_sync(0xffffffffu, mbar_wait(sc_full(st.i), st.ph, abort_flag) &&
+                                                 mbar_wait(acc_full(ab.i), ab.ph, abort_flag))) { fail(); break; }
                 tc_fence_after();
                 const float *sc = reinterpret_cast<const float *>(sbase + p.off_sc) + st.i * (NB * (PW / 4)) + c0;
                 const uint32_t ta = tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)ab.i * p.buf_cols + (uint32_t)c0;
-#pragma unroll
-                for (int j = 0; j < NB / 16; ++j) {
-                    if (c0 + 16 * j >= BN) break;
+                if constexpr (NB == 16) {
                     float v[16];
-                    tc_ld16(ta + 16u * j, v);
+                    tc_ld16(ta, v);
                     tc_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 8; i += 2) {
-                        const float4 s4 = *reinterpret_cast<const float4 *>(sc + 16 * j + 2 * i);
-                        float2 &A0 = acc[8 * j + i], &A1 = acc[8 * j + i + 1];
-                        asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%0, %1};\n\t"
-                            "fma.rn.f32x2 c, a, b, c;\n\tmov.b64 {%0, %1}, c;\n\t}"
-                            : "+f"(A0.x), "+f"(A0.y) : "f"(v[2 * i]), "f"(v[2 * i + 1]), "f"(s4.x), "f"(s4.y));
-                        asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%0, %1};\n\t"
-                            "fma.rn.f32x2 c, a, b, c;\n\tmov.b64 {%0, %1}, c;\n\t}"
-                            : "+f"(A1.x), "+f"(A1.y) : "f"(v[2 * i + 2]), "f"(v[2 * i + 3]), "f"(s4.z), "f"(s4.w));
+                    for (int i = 0; i < 16; i += 4) {
+                        const float4 s4 = *reinterpret_cast<const float4 *>(sc + i);
+                        fma2(acc[i / 2], v[i], v[i + 1], s4.x, s4.y);
+                        fma2(acc[i / 2 + 1], v[i + 2], v[i + 3], s4.z, s4.w);
+                    }
+                } else {
+                    // 32 columns at a time, the next ones on their way while these are added
+                    // (columns from BN on hold whatever was there; they are not stored)
+                    float v[2][32];
+                    tc_ld32(ta, v[0]);
+#pragma unroll
+                    for (int j = 0; j < NB / 32; ++j) {
+                        tc_wait_ld();
+                        if (j + 1 < NB / 32) tc_ld32(ta + 32u * (j + 1), v[(j + 1) & 1]);
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            const float4 s4 = *reinterpret_cast<const float4 *>(sc + 32 * j + i);
+                            fma2(acc[16 * j + i / 2], v[j & 1][i], v[j & 1][i + 1], s4.x, s4.y);
+                            fma2(acc[16 * j + i / 2 + 1], v[j & 1][i + 2], v[j & 1][i + 3], s4.z, s4.w);
+                        }
                     }
                 }
                 tc_fence_before();
@@ -312,10 +361,37 @@ fp8_gemm_kernel(const F8Params p, const __grid_constant__ CUtensorMap wmap, cons
                 const int n = nt * F8_TN + 32 * q + lane;
                 T *y = static_cast<T *>(p.y) + n;
 #pragma unroll
-                for (int j = 0; j < HB; ++j) {
+                for (int j = 0; j < NB; ++j) {
                     const int m = mt * BN + c0 + j;
                     if (c0 + j < BN && m < p.M && n < p.N) y[(int64_t)m * p.ldy] = from_f32<T>(j & 1 ? acc[j / 2].y : acc[j / 2].x);
                 }
+            }
+        }
+        if (p.split > 1) {
+            // column j of the tile belongs to the cluster's CTA j / cols, which receives every
+            // CTA's partial sums in its stage memory (each CTA has drained its copies and MMAs
+            // when it passes the first barrier) and adds them in CTA order
+            const int cols = (BN + p.split - 1) / p.split;
+            const int nt = first_tile / p.mt, mt = first_tile - nt * p.mt;
+            cluster_sync();
+#pragma unroll
+            for (int j = 0; j < NB; ++j) {
+                const int col = c0 + j;
+                if (col < BN) {
+                    const int to = col / cols;
+                    st_cluster(base + 4u * (uint32_t)((rank * cols + (col - to * cols)) * F8_TN + 32 * q + lane),
+                               (uint32_t)to, j & 1 ? acc[j / 2].y : acc[j / 2].x);
+                }
+            }
+            cluster_sync();
+            const float *part = reinterpret_cast<const float *>(sbase);
+            const int mine = min(cols, BN - rank * cols);
+            for (int e = tid - 128; e < mine * F8_TN; e += 32 * PW) {
+                const int j = e / F8_TN, r = e - j * F8_TN;
+                float v = 0.0f;
+                for (int s = 0; s < p.split; ++s) v += part[(s * cols + j) * F8_TN + r];
+                const int m = mt * BN + rank * cols + j, n = nt * F8_TN + r;
+                if (m < p.M && n < p.N) static_cast<T *>(p.y)[(int64_t)m * p.ldy + n] = from_f32<T>(v);
             }
         }
     }
@@ -327,35 +403,249 @@ fp8_gemm_kernel(const F8Params p, const __grid_constant__ CUtensorMap wmap, cons
         __syncwarp();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_cols) : "memory");
     }
-    if (p.split > 1) {
-        // column j of the tile belongs to the cluster's CTA j / cols, which receives every
-        // CTA's partial sums in its stage memory (each CTA has drained its copies and MMAs
-        // when it passes the first barrier) and adds them in CTA order
-        const int cols = (BN + p.split - 1) / p.split;
-        const int tile = first_tile, nt = tile / p.mt, mt = tile - nt * p.mt;
-        cluster_sync();
-        if (warp >= 4) {
-            const int q = warp & 3, c0 = ((warp - 4) >> 2) * NB;
+}
+
+// ---- two CTAs on one tile ----------------------------------------------------------------
+
+constexpr int F8P_T = 256;                 // rows of x and of w per tile
+constexpr int F8P_STAGES = 6;
+constexpr uint32_t F8P_STAGE = 2 * 128 * F8_KB;      // one CTA's bytes of a stage: 128 rows of x, 128 of w
+constexpr uint32_t F8P_SC = F8P_STAGES * F8P_STAGE;  // scales: 256 floats a stage
+constexpr uint32_t F8P_BAR = F8P_SC + F8P_STAGES * 1024;
+constexpr size_t F8P_SMEM = 1024 + F8P_BAR + 8 * (3 * F8P_STAGES + 4 + 1) + 16;
+
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap *map, int32_t x, int32_t y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2"
+                 " [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void tc_mma_f8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// arrives on the barrier at this offset in both CTAs
+__device__ __forceinline__ void tc_commit_pair(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_at(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred P1;\n\t"
+                 "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 P1, [%1], %2;\n\t"
+                 "selp.b32 %0, 1, 0, P1;\n\t}"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, volatile int *abort_flag) {
+    for (uint32_t i = 0; i < F8_WAIT; ++i) {
+        if (mbar_try_wait_cluster(bar, parity)) return true;
+        if ((i & 255u) == 255u && *abort_flag) return false;
+    }
+    return false;
+}
+
+// Cluster of two: rank 0 leads (it issues the MMAs of both).  The leader's `full` barrier
+// counts both CTAs' copies; commits arrive in both CTAs; both CTAs' promotion warps free an
+// accumulator on the leader's acc_empty.  Registers as above: 384 x 168 at launch.
+template <typename T>
+__global__ void __launch_bounds__(384, 1)
+fp8_gemm_pair_kernel(const F8Params p, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap) {
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    uint8_t *sbase = smem_raw + (base - raw);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    constexpr int S = F8P_STAGES;
+    const uint32_t bars = base + F8P_BAR;
+    auto full = [&](int i) { return bars + 8u * i; };                 // both CTAs' bytes (the leader's)
+    auto sc_full = [&](int i) { return bars + 8u * (S + i); };        // scale loader
+    auto empty = [&](int i) { return bars + 8u * (2 * S + i); };      // commit + promotion warps
+    auto acc_full = [&](int i) { return bars + 8u * (3 * S + i); };   // commit
+    auto acc_empty = [&](int i) { return bars + 8u * (3 * S + 2 + i); };   // both CTAs' promotion warps (the leader's)
+    const uint32_t drain = bars + 8u * (3 * S + 4);
+    uint8_t *misc = sbase + F8P_BAR + 8 * (3 * S + 5);
+    volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(misc);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(misc + 4);
+    const uint32_t rank = cluster_rank();
+
+    if (tid == 0) {
+        for (int i = 0; i < S; ++i) { mbar_init(full(i), 1); mbar_init(sc_full(i), 1); mbar_init(empty(i), 1 + 8); }
+        for (int i = 0; i < 2; ++i) { mbar_init(acc_full(i), 1); mbar_init(acc_empty(i), 16); }
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_u32((const void *)tmem_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();                       // both CTAs' barriers stand
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    dependency_trigger();
+    dependency_wait();
+
+    const int tiles = p.mt * p.nt, step = gridDim.x / 2;
+    bool ok = true;
+    auto fail = [&]() {
+        ok = false;
+        *abort_flag = 1;
+        atomicExch(p.err, Q35_ERR_TIMEOUT);
+    };
+
+    if (warp < 4) {
+        regs_down<56>();
+        if (warp == 0 && lane == 0) {
+            Ring st{};
+            for (int tile = blockIdx.x / 2; tile < tiles && ok; tile += step) {
+                const int nt = tile / p.mt, mt = tile - nt * p.mt;
+                for (int kb = 0; kb < p.KB; ++kb) {
+                    if (!mbar_wait(empty(st.i), st.ph ^ 1u, abort_flag)) { fail(); break; }
+                    if (rank == 0) mbar_expect_tx(full(st.i), 2 * F8P_STAGE);
+                    const uint32_t dst = base + (uint32_t)st.i * F8P_STAGE, bar = at_rank(full(st.i), 0);
+                    tma_load_pair(dst, &xmap, kb * F8_KB, mt * F8P_T + 128 * (int)rank, bar);
+                    tma_load_pair(dst + 128 * F8_KB, &wmap, kb * F8_KB, nt * F8P_T + 128 * (int)rank, bar);
+                    st.next(S);
+                }
+            }
+            // (every copy has landed when the leader's MMAs have: see the end)
+        } else if (warp == 2) {
+            // xs[m][kb] * ws[nb][kb] for this CTA's 128 rows and the tile's two blocks of w's rows
+            constexpr int SB = 2;
+            const int wb = (p.N + F8_TN - 1) / F8_TN;
+            Ring st{};
+            for (int tile = blockIdx.x / 2; tile < tiles && ok; tile += step) {
+                const int nt = tile / p.mt, mt = tile - nt * p.mt;
+                const int n1 = min(2 * nt + 1, wb - 1);
+                for (int kb = 0; kb < p.KB && ok; kb += SB) {
+                    float v[SB][4], w[SB][2];
 #pragma unroll
-            for (int j = 0; j < HB; ++j) {
-                const int col = c0 + j;
-                if (col < BN) {
-                    const int to = col / cols;
-                    st_cluster(base + 4u * (uint32_t)((rank * cols + (col - to * cols)) * F8_TN + 32 * q + lane),
-                               (uint32_t)to, j & 1 ? acc[j / 2].y : acc[j / 2].x);
+                    for (int b = 0; b < SB; ++b) {
+                        const bool live = kb + b < p.KB;
+                        w[b][0] = live ? p.ws[(int64_t)(2 * nt) * p.KB + kb + b] : 0.0f;
+                        w[b][1] = live ? p.ws[(int64_t)n1 * p.KB + kb + b] : 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int m = mt * F8P_T + 128 * (int)rank + lane + 32 * i;
+                            v[b][i] = live && m < p.M ? p.xs[(int64_t)m * p.KB + kb + b] : 0.0f;
+                        }
+                    }
+#pragma unroll
+                    for (int b = 0; b < SB; ++b) {
+                        if (kb + b >= p.KB) break;
+                        if (!__all_sync(0xffffffffu, mbar_wait(empty(st.i), st.ph ^ 1u, abort_flag))) { fail(); break; }
+                        float *sc = reinterpret_cast<float *>(sbase + F8P_SC) + st.i * 256;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            sc[lane + 32 * i] = v[b][i] * w[b][0];
+                            sc[128 + lane + 32 * i] = v[b][i] * w[b][1];
+                        }
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(sc_full(st.i));
+                        st.next(S);
+                    }
+                }
+            }
+        } else if (warp == 1 && lane == 0 && rank == 0) {
+            const uint32_t idesc = idesc_f8(F8P_T, F8P_T);
+            Ring st{}, ab{};
+            for (int tile = blockIdx.x / 2; tile < tiles && ok; tile += step) {
+                for (int kb = 0; kb < p.KB; ++kb) {
+                    if (!mbar_wait_cluster(acc_empty(ab.i), ab.ph ^ 1u, abort_flag) ||
+                        !mbar_wait_cluster(full(st.i), st.ph, abort_flag)) { fail(); break; }
+                    tc_fence_after();
+                    const uint32_t a0 = base + (uint32_t)st.i * F8P_STAGE, b0 = a0 + 128 * F8_KB;
+                    const uint32_t d = tmem + (uint32_t)ab.i * 256u;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        tc_mma_f8_pair(d, smem_desc_sw128(a0 + 32u * j), smem_desc_sw128(b0 + 32u * j), idesc, j > 0 ? 1u : 0u);
+                    tc_commit_pair(empty(st.i));
+                    tc_commit_pair(acc_full(ab.i));
+                    st.next(S);
+                    ab.next(2);
                 }
             }
         }
-        cluster_sync();
-        const float *part = reinterpret_cast<const float *>(sbase);
-        const int mine = min(cols, BN - rank * cols);
-        for (int e = tid; e < mine * F8_TN; e += blockDim.x) {
-            const int j = e / F8_TN, r = e - j * F8_TN;
-            float v = 0.0f;
-            for (int s = 0; s < p.split; ++s) v += part[(s * cols + j) * F8_TN + r];
-            const int m = mt * BN + rank * cols + j, n = nt * F8_TN + r;
-            if (m < p.M && n < p.N) static_cast<T *>(p.y)[(int64_t)m * p.ldy + n] = from_f32<T>(v);
+        // every MMA has completed, so every copy it read has landed, in both CTAs
+        if (warp == 1 && lane == 0) {
+            if (rank == 0) tc_commit_pair(drain);
+            if (!mbar_wait_cluster(drain, 0, abort_flag)) fail();
         }
+    } else {
+        regs_up<224>();
+        const int q = warp & 3, half = (warp - 4) >> 2;
+        float2 acc[64];
+        Ring st{}, ab{};
+        for (int tile = blockIdx.x / 2; tile < tiles && ok; tile += step) {
+            const int nt = tile / p.mt, mt = tile - nt * p.mt;
+#pragma unroll
+            for (int i = 0; i < 64; ++i) acc[i] = make_float2(0.0f, 0.0f);
+            for (int kb = 0; kb < p.KB; ++kb) {
+                if (!__all_sync(0xffffffffu, mbar_wait(sc_full(st.i), st.ph, abort_flag) &&
+                                                 mbar_wait(acc_full(ab.i), ab.ph, abort_flag))) { fail(); break; }
+                tc_fence_after();
+                const float s = reinterpret_cast<const float *>(sbase + F8P_SC)[st.i * 256 + half * 128 + 32 * q + lane];
+                const uint32_t ta = tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)ab.i * 256u + (uint32_t)half * 128u;
+                float v[2][32];
+                tc_ld32(ta, v[0]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    tc_wait_ld();
+                    if (j < 3) tc_ld32(ta + 32u * (j + 1), v[(j + 1) & 1]);
+                    else {
+                        // all of the accumulator has been read
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) { mbar_arrive_at(at_rank(acc_empty(ab.i), 0)); mbar_arrive(empty(st.i)); }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) fma2(acc[16 * j + i / 2], v[j & 1][i], v[j & 1][i + 1], s, s);
+                }
+                st.next(S);
+                ab.next(2);
+            }
+            if (!ok) break;
+            const int m = mt * F8P_T + 128 * (int)rank + 32 * q + lane, n0 = nt * F8P_T + 128 * half;
+            if (m < p.M) {
+                T *y = static_cast<T *>(p.y) + (int64_t)m * p.ldy + n0;
+                constexpr int V = 16 / sizeof(T);
+                if (n0 + 128 <= p.N && (reinterpret_cast<uintptr_t>(y) & 15) == 0) {
+#pragma unroll
+                    for (int j = 0; j < 128; j += V) {
+                        uint4 u;
+                        if constexpr (sizeof(T) == 4) {
+                            u = make_uint4(__float_as_uint(acc[j / 2].x), __float_as_uint(acc[j / 2].y),
+                                           __float_as_uint(acc[j / 2 + 1].x), __float_as_uint(acc[j / 2 + 1].y));
+                        } else {
+                            u = make_uint4(pack2<T>(acc[j / 2].x, acc[j / 2].y), pack2<T>(acc[j / 2 + 1].x, acc[j / 2 + 1].y),
+                                           pack2<T>(acc[j / 2 + 2].x, acc[j / 2 + 2].y), pack2<T>(acc[j / 2 + 3].x, acc[j / 2 + 3].y));
+                        }
+                        *reinterpret_cast<uint4 *>(y + j) = u;
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 128; ++j)
+                        if (n0 + j < p.N) y[j] = from_f32<T>(j & 1 ? acc[j / 2].y : acc[j / 2].x);
+                }
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();                       // neither CTA leaves while the other may arrive on its barriers
+    tc_fence_after();
+    if (warp == 1) {
+        __syncwarp();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     }
 }
 
@@ -392,6 +682,7 @@ int byte_map(EncodeFn encode, CUtensorMap *map, const void *p, int64_t rows, int
 }
 
 struct F8Plan {
+    bool pair = false;
     int NB, PW, BN, mt, nt, split, stages, bufs, grid;
     uint32_t tmem_cols, buf_cols, off_sc, off_bar;
     size_t smem;
@@ -400,21 +691,32 @@ struct F8Plan {
 F8Plan plan_f8(int32_t M, int32_t N, int32_t KB) {
     constexpr int SMS = 148;
     F8Plan pl{};
+    // a tile for every pair of SMs: two CTAs per tile
+    if (M > 128 && ceil_div(M, F8P_T) * ceil_div(N, F8P_T) >= SMS / 2) {
+        pl.pair = true;
+        pl.mt = (int)ceil_div(M, F8P_T);
+        pl.nt = (int)ceil_div(N, F8P_T);
+        pl.split = 1;
+        pl.grid = SMS;
+        pl.BN = 128;
+        return pl;
+    }
     pl.mt = (int)ceil_div(M, 256);
     pl.BN = (int)round_up(ceil_div(M, pl.mt), 16);
     pl.nt = (int)ceil_div(N, F8_TN);
     pl.NB = pl.BN <= 16 ? 16 : pl.BN <= 32 ? 32 : pl.BN <= 64 ? 64 : 128;
     pl.PW = pl.BN <= 128 ? 4 : 8;
     const int tiles = pl.mt * pl.nt;
-    pl.split = 1;
-    while (pl.split < 8 && 2 * pl.split <= KB && (int64_t)tiles * 2 * pl.split <= SMS) pl.split *= 2;
-    pl.grid = pl.split > 1 ? tiles * pl.split : std::min(tiles, SMS);
+    const int per_sm = pl.NB <= 32 ? 2 : 1;
+    // as many CTAs per tile as give every slot one, at least four k-blocks each
+    pl.split = std::max(1, std::min({8, KB / 4, per_sm * SMS / tiles}));
+    pl.grid = pl.split > 1 ? tiles * pl.split : std::min(tiles, per_sm * SMS);
     pl.buf_cols = (uint32_t)(pl.NB * (pl.PW / 4));
-    pl.bufs = std::min<int>(8, 512 / pl.buf_cols);
+    pl.bufs = std::min<int>(8, 512 / per_sm / pl.buf_cols);
     pl.tmem_cols = 32;
     while (pl.tmem_cols < pl.bufs * pl.buf_cols) pl.tmem_cols *= 2;
     const size_t stage = (size_t)(F8_TN + pl.BN) * F8_KB, sc = pl.buf_cols * 4;
-    const size_t budget = 227 * 1024 - 1024 - 512;
+    const size_t budget = (227 * 1024 - (per_sm - 1) * 1024) / per_sm - 1024 - 512;
     pl.stages = (int)std::min<size_t>(16, budget / (stage + sc));
     // the split exchange reuses the stages: split * ceil(BN / split) columns of 128 floats
     pl.off_sc = (uint32_t)(pl.stages * stage);
@@ -431,23 +733,25 @@ int launch_f8(const F8Params &p, const F8Plan &pl, const CUtensorMap &wm, const 
         Q35_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
         configured[dev] = true;
     }
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)pl.split;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)pl.grid);
-    cfg.blockDim = dim3(128 + 32 * PW);
-    cfg.dynamicSmemBytes = pl.smem;
-    cfg.stream = s;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    Q35_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, p, wm, xm));
+    Q35_CUDA_TRY(launch_dependent(kern, dim3((unsigned)pl.grid), 128 + 32 * PW, pl.smem, s, pl.split, p, wm, xm));
+    return Q35_OK;
+}
+
+template <typename T>
+int launch_f8_pair(const F8Params &p, const F8Plan &pl, const CUtensorMap &wm, const CUtensorMap &xm, int dev, cudaStream_t s) {
+    auto kern = fp8_gemm_pair_kernel<T>;
+    static bool configured[64] = {};
+    if (!configured[dev]) {
+        Q35_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)F8P_SMEM));
+        configured[dev] = true;
+    }
+    Q35_CUDA_TRY(launch_dependent(kern, dim3((unsigned)pl.grid), 384, F8P_SMEM, s, 2, p, wm, xm));
     return Q35_OK;
 }
 
 template <typename T>
 int launch_f8(const F8Params &p, const F8Plan &pl, const CUtensorMap &wm, const CUtensorMap &xm, int dev, cudaStream_t s) {
+    if (pl.pair) return launch_f8_pair<T>(p, pl, wm, xm, dev, s);
     if (pl.PW == 8) return launch_f8<T, 128, 8>(p, pl, wm, xm, dev, s);
     switch (pl.NB) {
     case 16: return launch_f8<T, 16, 4>(p, pl, wm, xm, dev, s);

@@ -193,6 +193,17 @@ def test_product(ctx, dtype, M, N, K):
     assert torch.equal(y, again)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("M,N,K", [(129, 19001, 300), (513, 9500, 1000), (2048, 8192, 1024), (300, 10240, 130), (256, 28672, 16),
+                                   (1025, 5120, 512), (12, 128, 65536), (197, 5120, 1500), (40, 20000, 512), (90, 640, 9000)])
+def test_product_of_many_tiles_and_of_split_ones(ctx, dtype, M, N, K):
+    """Two CTAs per tile (a tile for every pair of SMs), persistent grids, and clusters along k."""
+    x, xs, w, ws, ld = make_product(M, N, K, M + 3 * N + K)
+    ref, mag = product_ref(x, xs, w, ws, N, K)
+    for pad in (0, 1, 8):
+        check_product(run_product(ctx, x, xs, w, ws, ld, M, N, K, dtype, pad=pad), ref, mag, K, dtype)
+
+
 def test_product_scales_of_very_different_size(ctx):
     M, N, K = 40, 512, 2048
     x, xs, w, ws, ld = make_product(M, N, K, 9, spread=20)
