@@ -10,8 +10,8 @@
 //     of several accumulators in tensor memory.  The sum over one block is a tensor-core
 //     fp32 sum of exact products;
 //   * promotion (warps 4 ..): tcgen05.ld of the block's sums, acc = fma(sum, scale, acc)
-//     with acc in registers, two sums per packed fma (fma.rn.f32x2), the next columns' load
-//     on its way meanwhile.
+//     with acc in registers, the next columns' load on its way meanwhile (packed fma.rn.f32x2
+//     was slower: the pairs had to be moved together).
 // A k-block's accumulator is handed over through mbarriers, so the MMAs of the next blocks
 // run under the promotion of this one.
 //
@@ -116,12 +116,6 @@ __device__ __forceinline__ void tc_ld32(uint32_t taddr, float (&v)[32]) {
                    "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]),
                    "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
                  : "r"(taddr) : "memory");
-}
-// acc.x += a * s, acc.y += b * t in one packed instruction
-__device__ __forceinline__ void fma2(float2 &acc, float a, float b, float s, float t) {
-    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%0, %1};\n\t"
-        "fma.rn.f32x2 z, x, y, z;\n\tmov.b64 {%0, %1}, z;\n\t}"
-        : "+f"(acc.x), "+f"(acc.y) : "f"(a), "f"(b), "f"(s), "f"(t));
 }
 template <int R> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R)); }
 template <int R> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
@@ -310,52 +304,60 @@ fp8_gemm_kernel(const F8Params p, const __grid_constant__ CUtensorMap wmap, cons
         if (PW == 8) regs_up<224>();
         const int q = warp & 3, half = (warp - 4) >> 2;
         const int c0 = half * NB;                       // first column of this thread
-        float2 acc[NB / 2];
+        constexpr int W = NB < 32 ? NB : 32, NJ = NB / W;   // columns per load, loads per k-block
+        float acc[NB];
         Ring st{}, ab{};
         for (int tile = first_tile; tile < tiles && ok; tile += step) {
             const int nt = tile / p.mt, mt = tile - nt * p.mt;
 #pragma unroll
-            for (int i = 0; i < NB / 2; ++i) acc[i] = make_float2(0.0f, 0.0f);
-            for (int kb = kb0; kb < kb1; ++kb) {
-                // (the stage cannot be refilled before this warp arrives on it, so its phase
-                // is still the one to wait for)
+            for (int i = 0; i < NB; ++i) acc[i] = 0.0f;
+            // W columns at a time, the next ones on their way while these are added (columns from BN on hold whatever was there; they are not stored)
+            float v[2][W];
+            auto ready = [&]() {                       // the k-block at (st, ab): its scales and sums
+                // (the stage cannot be refilled before this warp arrives on it, so its phase is
+                // still the one to wait for)
                 if (!__all_sync(0xffffffffu, mbar_wait(sc_full(st.i), st.ph, abort_flag) &&
-                                                 mbar_wait(acc_full(ab.i), ab.ph, abort_flag))) { fail(); break; }
+                                                 mbar_wait(acc_full(ab.i), ab.ph, abort_flag))) { fail(); return false; }
                 tc_fence_after();
+                return true;
+            };
+            auto load = [&](int j, float (&to)[W]) {
+                const uint32_t ta = tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)ab.i * p.buf_cols + (uint32_t)(c0 + W * j);
+                if constexpr (W == 16) tc_ld16(ta, to);
+                else tc_ld32(ta, to);
+            };
+            if (!ready()) break;
+            load(0, v[0]);
+            const int nkb = kb1 - kb0;
+            for (int kb = 0; kb < nkb && ok; ++kb) {
                 const float *sc = reinterpret_cast<const float *>(sbase + p.off_sc) + st.i * (NB * (PW / 4)) + c0;
-                const uint32_t ta = tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)ab.i * p.buf_cols + (uint32_t)c0;
-                if constexpr (NB == 16) {
-                    float v[16];
-                    tc_ld16(ta, v);
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    float (&now)[W] = v[j & 1];
                     tc_wait_ld();
-#pragma unroll
-                    for (int i = 0; i < 16; i += 4) {
-                        const float4 s4 = *reinterpret_cast<const float4 *>(sc + i);
-                        fma2(acc[i / 2], v[i], v[i + 1], s4.x, s4.y);
-                        fma2(acc[i / 2 + 1], v[i + 2], v[i + 3], s4.z, s4.w);
+                    if (j + 1 < NJ) {
+                        load(j + 1, v[(j + 1) & 1]);
+                    } else {
+                        // all of the accumulator has been read
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(acc_empty(ab.i));
                     }
-                } else {
-                    // 32 columns at a time, the next ones on their way while these are added
-                    // (columns from BN on hold whatever was there; they are not stored)
-                    float v[2][32];
-                    tc_ld32(ta, v[0]);
 #pragma unroll
-                    for (int j = 0; j < NB / 32; ++j) {
-                        tc_wait_ld();
-                        if (j + 1 < NB / 32) tc_ld32(ta + 32u * (j + 1), v[(j + 1) & 1]);
-#pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
-                            const float4 s4 = *reinterpret_cast<const float4 *>(sc + 32 * j + i);
-                            fma2(acc[16 * j + i / 2], v[j & 1][i], v[j & 1][i + 1], s4.x, s4.y);
-                            fma2(acc[16 * j + i / 2 + 1], v[j & 1][i + 2], v[j & 1][i + 3], s4.z, s4.w);
-                        }
+                    for (int i = 0; i < W / 4; ++i) {
+                        const float4 s = reinterpret_cast<const float4 *>(sc + W * j)[i];
+                        acc[W * j + 4 * i] = fmaf(now[4 * i], s.x, acc[W * j + 4 * i]);
+                        acc[W * j + 4 * i + 1] = fmaf(now[4 * i + 1], s.y, acc[W * j + 4 * i + 1]);
+                        acc[W * j + 4 * i + 2] = fmaf(now[4 * i + 2], s.z, acc[W * j + 4 * i + 2]);
+                        acc[W * j + 4 * i + 3] = fmaf(now[4 * i + 3], s.w, acc[W * j + 4 * i + 3]);
                     }
                 }
-                tc_fence_before();
+                // (the scales have been used)
                 __syncwarp();
-                if (lane == 0) { mbar_arrive(acc_empty(ab.i)); mbar_arrive(empty(st.i)); }
+                if (lane == 0) mbar_arrive(empty(st.i));
                 st.next(S);
                 ab.next(NBUF);
+                if (kb + 1 < nkb && ready()) load(0, v[0]);
             }
             if (p.split == 1 && ok) {
                 const int n = nt * F8_TN + 32 * q + lane;
@@ -363,7 +365,7 @@ fp8_gemm_kernel(const F8Params p, const __grid_constant__ CUtensorMap wmap, cons
 #pragma unroll
                 for (int j = 0; j < NB; ++j) {
                     const int m = mt * BN + c0 + j;
-                    if (c0 + j < BN && m < p.M && n < p.N) y[(int64_t)m * p.ldy] = from_f32<T>(j & 1 ? acc[j / 2].y : acc[j / 2].x);
+                    if (c0 + j < BN && m < p.M && n < p.N) y[(int64_t)m * p.ldy] = from_f32<T>(acc[j]);
                 }
             }
         }
@@ -380,7 +382,7 @@ fp8_gemm_kernel(const F8Params p, const __grid_constant__ CUtensorMap wmap, cons
                 if (col < BN) {
                     const int to = col / cols;
                     st_cluster(base + 4u * (uint32_t)((rank * cols + (col - to * cols)) * F8_TN + 32 * q + lane),
-                               (uint32_t)to, j & 1 ? acc[j / 2].y : acc[j / 2].x);
+                               (uint32_t)to, acc[j]);
                 }
             }
             cluster_sync();
@@ -582,35 +584,43 @@ fp8_gemm_pair_kernel(const F8Params p, const __grid_constant__ CUtensorMap wmap,
     } else {
         regs_up<224>();
         const int q = warp & 3, half = (warp - 4) >> 2;
-        float2 acc[64];
+        float acc[128];
         Ring st{}, ab{};
         for (int tile = blockIdx.x / 2; tile < tiles && ok; tile += step) {
             const int nt = tile / p.mt, mt = tile - nt * p.mt;
 #pragma unroll
-            for (int i = 0; i < 64; ++i) acc[i] = make_float2(0.0f, 0.0f);
-            for (int kb = 0; kb < p.KB; ++kb) {
+            for (int i = 0; i < 128; ++i) acc[i] = 0.0f;
+            // 32 columns at a time; the next ones (of the next k-block too) are on their way
+            // while these are added
+            float v[2][32], s = 0.0f;
+            auto ready = [&]() {                       // the k-block at (st, ab): its scale and sums
                 if (!__all_sync(0xffffffffu, mbar_wait(sc_full(st.i), st.ph, abort_flag) &&
-                                                 mbar_wait(acc_full(ab.i), ab.ph, abort_flag))) { fail(); break; }
+                                                 mbar_wait(acc_full(ab.i), ab.ph, abort_flag))) { fail(); return false; }
                 tc_fence_after();
-                const float s = reinterpret_cast<const float *>(sbase + F8P_SC)[st.i * 256 + half * 128 + 32 * q + lane];
-                const uint32_t ta = tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)ab.i * 256u + (uint32_t)half * 128u;
-                float v[2][32];
-                tc_ld32(ta, v[0]);
+                return true;
+            };
+            auto columns = [&](int j) { return tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)ab.i * 256u + (uint32_t)(half * 128 + 32 * j); };
+            if (!ready()) break;
+            tc_ld32(columns(0), v[0]);
+            for (int kb = 0; kb < p.KB && ok; ++kb) {
+                s = reinterpret_cast<const float *>(sbase + F8P_SC)[st.i * 256 + half * 128 + 32 * q + lane];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     tc_wait_ld();
-                    if (j < 3) tc_ld32(ta + 32u * (j + 1), v[(j + 1) & 1]);
-                    else {
+                    if (j < 3) {
+                        tc_ld32(columns(j + 1), v[(j + 1) & 1]);
+                    } else {
                         // all of the accumulator has been read
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) { mbar_arrive_at(at_rank(acc_empty(ab.i), 0)); mbar_arrive(empty(st.i)); }
+                        st.next(S);
+                        ab.next(2);
+                        if (kb + 1 < p.KB && ready()) tc_ld32(columns(0), v[0]);
                     }
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) fma2(acc[16 * j + i / 2], v[j & 1][i], v[j & 1][i + 1], s, s);
+                    for (int i = 0; i < 32; ++i) acc[32 * j + i] = fmaf(v[j & 1][i], s, acc[32 * j + i]);
                 }
-                st.next(S);
-                ab.next(2);
             }
             if (!ok) break;
             const int m = mt * F8P_T + 128 * (int)rank + 32 * q + lane, n0 = nt * F8P_T + 128 * half;
@@ -621,19 +631,18 @@ fp8_gemm_pair_kernel(const F8Params p, const __grid_constant__ CUtensorMap wmap,
 #pragma unroll
                     for (int j = 0; j < 128; j += V) {
                         uint4 u;
-                        if constexpr (sizeof(T) == 4) {
-                            u = make_uint4(__float_as_uint(acc[j / 2].x), __float_as_uint(acc[j / 2].y),
-                                           __float_as_uint(acc[j / 2 + 1].x), __float_as_uint(acc[j / 2 + 1].y));
-                        } else {
-                            u = make_uint4(pack2<T>(acc[j / 2].x, acc[j / 2].y), pack2<T>(acc[j / 2 + 1].x, acc[j / 2 + 1].y),
-                                           pack2<T>(acc[j / 2 + 2].x, acc[j / 2 + 2].y), pack2<T>(acc[j / 2 + 3].x, acc[j / 2 + 3].y));
-                        }
+                        if constexpr (sizeof(T) == 4)
+                            u = make_uint4(__float_as_uint(acc[j]), __float_as_uint(acc[j + 1]), __float_as_uint(acc[j + 2]),
+                                           __float_as_uint(acc[j + 3]));
+                        else
+                            u = make_uint4(pack2<T>(acc[j], acc[j + 1]), pack2<T>(acc[j + 2], acc[j + 3]),
+                                           pack2<T>(acc[j + 4], acc[j + 5]), pack2<T>(acc[j + 6], acc[j + 7]));
                         *reinterpret_cast<uint4 *>(y + j) = u;
                     }
                 } else {
 #pragma unroll
                     for (int j = 0; j < 128; ++j)
-                        if (n0 + j < p.N) y[j] = from_f32<T>(j & 1 ? acc[j / 2].y : acc[j / 2].x);
+                        if (n0 + j < p.N) y[j] = from_f32<T>(acc[j]);
                 }
             }
         }
