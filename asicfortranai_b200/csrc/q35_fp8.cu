@@ -15,17 +15,19 @@
 // A k-block's accumulator is handed over through mbarriers, so the MMAs of the next blocks
 // run under the promotion of this one.
 //
-// fp8_gemm_kernel (few rows of x): w in the MMA's M position, 128 rows of w (one row of scale
-// blocks, so ws is one number per tile and k-block) x BN <= 256 rows of x; a thread owns a row
-// of w and reads the scales of x's rows as broadcast vectors.  Few tiles are split along k over
-// the CTAs of a cluster; each CTA then adds up its share of the tile's columns from every CTA's
-// shared memory, in CTA order, so the result does not depend on timing.
+// fp8_gemm_kernel (up to 128 rows of x): w in the MMA's M position, 128 rows of w (one row of
+// scale blocks, so ws is one number per tile and k-block) x BN <= 128 rows of x; a thread owns a
+// row of w and reads the scales of x's rows as broadcast vectors.
 //
-// fp8_gemm_pair_kernel (many rows): two CTAs on one 256 x 256 tile (cta_group::2), x in the M
+// fp8_gemm_pair_kernel (more rows): two CTAs on one 256 x 256 tile (cta_group::2), x in the M
 // position, each CTA holding 128 rows of x and half of the tile's rows of w, so that an SM
-// reads 32 KB a k-block instead of 48 (shared memory's and L2's rates, not the MMAs, bound
-// the one-CTA form: 128 x 256 x 128 takes the tensor cores 512 clocks, 48 KB through 128 bytes a
-// clock in and out 768); a thread owns a row of x and one scale covers its 128 columns.
+// reads 32 KB a k-block instead of 48; a thread owns a row of x and one scale covers its 128
+// columns.  (An accumulator, issuer and hand-over of its own for each of the two blocks of w's
+// rows was slower, 573 against 522 us at 2048 x 28672 x 8192: x's rows are then read twice.)
+//
+// Few tiles are split along k over the CTAs (pairs) of a cluster; each CTA then adds up its
+// share of the tile's columns from every CTA's shared memory, in CTA order, so the result does
+// not depend on timing.
 //
 // Every wait is bounded: a wait that gives up records Q35_ERR_TIMEOUT in the context's error
 // word and raises an abort flag that ends the other roles' waits; copies and MMAs in flight
@@ -119,7 +121,23 @@ __device__ __forceinline__ void tc_ld32(uint32_t taddr, float (&v)[32]) {
 }
 template <int R> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R)); }
 template <int R> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
-__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// waits for this thread's tensor-memory loads; the loaded values pass through it, so that
+// nothing that uses them can be moved ahead of it
+__device__ __forceinline__ void tc_wait_ld(float (&v)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                   "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])
+                 :: "memory");
+}
+__device__ __forceinline__ void tc_wait_ld(float (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                   "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]),
+                   "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]),
+                   "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]),
+                   "+f"(v[29]), "+f"(v[30]), "+f"(v[31])
+                 :: "memory");
+}
 // K-major operand, 128-byte swizzle: 8-row atoms of 1024 bytes
 __device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t addr) {
     return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
@@ -158,10 +176,10 @@ struct Ring {
 };
 
 // NB: accumulator registers (x rows) per promotion thread; 4 or 8 promotion warps, the second
-// four taking the upper half of the tile's columns.  Tiles of up to 32 rows leave room for
-// two CTAs on an SM.
+// four taking the upper half of the tile's columns (from 33 rows on: one warp per scheduler
+// could not keep up).  Tiles of up to 32 rows leave room for two CTAs on an SM.
 template <typename T, int NB, int PW>
-__global__ void __launch_bounds__(128 + 32 * PW, NB <= 32 ? 2 : 1)
+__global__ void __launch_bounds__(128 + 32 * PW, PW == 4 ? 2 : 1)
 fp8_gemm_kernel(const F8Params p, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap) {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
@@ -211,9 +229,7 @@ fp8_gemm_kernel(const F8Params p, const __grid_constant__ CUtensorMap wmap, cons
         atomicExch(p.err, Q35_ERR_TIMEOUT);
     };
 
-    // registers: 4 x 32 x 56 + 8 x 32 x 224 = 384 x 168
     if (warp < 4) {
-        if (PW == 8) regs_down<56>();
         if (warp == 0) {
             if (lane == 0) {
                 Ring st{};
@@ -272,6 +288,7 @@ fp8_gemm_kernel(const F8Params p, const __grid_constant__ CUtensorMap wmap, cons
         } else if (warp == 1) {
             if (lane == 0) {
                 const uint32_t idesc = idesc_f8(F8_TN, BN);
+                const uint64_t a_desc = smem_desc_sw128(base), b_desc = smem_desc_sw128(base + F8_TN * F8_KB);
                 Ring st{}, ab{};
                 for (int tile = first_tile; tile < tiles && ok; tile += step) {
                     for (int kb = kb0; kb < kb1; ++kb) {
@@ -280,11 +297,11 @@ fp8_gemm_kernel(const F8Params p, const __grid_constant__ CUtensorMap wmap, cons
                             break;
                         }
                         tc_fence_after();
-                        const uint32_t a0 = base + (uint32_t)st.i * stage_bytes, b0 = a0 + F8_TN * F8_KB;
+                        const uint64_t off = (uint64_t)st.i * (stage_bytes >> 4);
                         const uint32_t d = tmem + (uint32_t)ab.i * p.buf_cols;
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
-                            tc_mma_f8(d, smem_desc_sw128(a0 + 32u * j), smem_desc_sw128(b0 + 32u * j), idesc, j > 0 ? 1u : 0u);
+                            tc_mma_f8(d, a_desc + off + 2 * j, b_desc + off + 2 * j, idesc, j > 0 ? 1u : 0u);
                         tc_commit(empty(st.i));
                         tc_commit(acc_full(ab.i));
                         st.next(S);
@@ -301,7 +318,6 @@ fp8_gemm_kernel(const F8Params p, const __grid_constant__ CUtensorMap wmap, cons
             cluster_sync();
         }
     } else {
-        if (PW == 8) regs_up<224>();
         const int q = warp & 3, half = (warp - 4) >> 2;
         const int c0 = half * NB;                       // first column of this thread
         constexpr int W = NB < 32 ? NB : 32, NJ = NB / W;   // columns per load, loads per k-block
@@ -334,7 +350,7 @@ fp8_gemm_kernel(const F8Params p, const __grid_constant__ CUtensorMap wmap, cons
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) {
                     float (&now)[W] = v[j & 1];
-                    tc_wait_ld();
+                    tc_wait_ld(now);
                     if (j + 1 < NJ) {
                         load(j + 1, v[(j + 1) & 1]);
                     } else {
@@ -413,6 +429,7 @@ constexpr int F8P_T = 256;                 // rows of x and of w per tile
 constexpr int F8P_STAGES = 6;
 constexpr uint32_t F8P_STAGE = 2 * 128 * F8_KB;      // one CTA's bytes of a stage: 128 rows of x, 128 of w
 constexpr uint32_t F8P_SC = F8P_STAGES * F8P_STAGE;  // scales: 256 floats a stage
+constexpr int F8P_PITCH = 129;             // floats between columns of the split exchange: no bank conflicts either way
 constexpr uint32_t F8P_BAR = F8P_SC + F8P_STAGES * 1024;
 constexpr size_t F8P_SMEM = 1024 + F8P_BAR + 8 * (3 * F8P_STAGES + 4 + 1) + 16;
 
@@ -427,34 +444,20 @@ __device__ __forceinline__ void tc_mma_f8_pair(uint32_t d, uint64_t a, uint64_t 
                  "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
                  ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
-// arrives on the barrier at this offset in both CTAs
-__device__ __forceinline__ void tc_commit_pair(uint32_t bar) {
+// arrives on the barrier at this offset in the CTAs of `mask`
+__device__ __forceinline__ void tc_commit_pair(uint32_t bar, uint16_t mask) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-                 ::"r"(bar), "h"((uint16_t)3) : "memory");
+                 ::"r"(bar), "h"(mask) : "memory");
 }
+// (no .release.cluster: what it would order, the tensor-memory loads, has completed, and its
+// fence cost more than all of the promotion: 844 against 522 us at 2048 x 28672 x 8192)
 __device__ __forceinline__ void mbar_arrive_at(uint32_t cluster_addr) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
-__device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile("{\n\t.reg .pred P1;\n\t"
-                 "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 P1, [%1], %2;\n\t"
-                 "selp.b32 %0, 1, 0, P1;\n\t}"
-                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-    return ok != 0;
-}
-__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, volatile int *abort_flag) {
-    for (uint32_t i = 0; i < F8_WAIT; ++i) {
-        if (mbar_try_wait_cluster(bar, parity)) return true;
-        if ((i & 255u) == 255u && *abort_flag) return false;
-    }
-    return false;
-}
-
-// Cluster of two: rank 0 leads (it issues the MMAs of both).  The leader's `full` barrier
-// counts both CTAs' copies; commits arrive in both CTAs; both CTAs' promotion warps free an
-// accumulator on the leader's acc_empty.  Registers as above: 384 x 168 at launch.
-template <typename T>
+// Each pair of a cluster: its even rank leads (it issues the MMAs of both).  The leader's `full`
+// barrier counts both CTAs' copies; commits arrive in both CTAs; both CTAs' promotion warps
+// free an accumulator on the leader's acc_empty.  Registers: 4 x 32 x 56 + 8 x 32 x 224 = 384 x 168.
+template <typename T, bool SPLIT>
 __global__ void __launch_bounds__(384, 1)
 fp8_gemm_pair_kernel(const F8Params p, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap) {
     extern __shared__ uint8_t smem_raw[];
@@ -467,13 +470,14 @@ fp8_gemm_pair_kernel(const F8Params p, const __grid_constant__ CUtensorMap wmap,
     auto full = [&](int i) { return bars + 8u * i; };                 // both CTAs' bytes (the leader's)
     auto sc_full = [&](int i) { return bars + 8u * (S + i); };        // scale loader
     auto empty = [&](int i) { return bars + 8u * (2 * S + i); };      // commit + promotion warps
-    auto acc_full = [&](int i) { return bars + 8u * (3 * S + i); };   // commit
-    auto acc_empty = [&](int i) { return bars + 8u * (3 * S + 2 + i); };   // both CTAs' promotion warps (the leader's)
+    auto acc_full = [&](int b) { return bars + 8u * (3 * S + b); };       // commit
+    auto acc_empty = [&](int b) { return bars + 8u * (3 * S + 2 + b); };  // both CTAs' promotion warps (the leader's)
     const uint32_t drain = bars + 8u * (3 * S + 4);
     uint8_t *misc = sbase + F8P_BAR + 8 * (3 * S + 5);
     volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(misc);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(misc + 4);
-    const uint32_t rank = cluster_rank();
+    const uint32_t crank = cluster_rank(), rank = crank & 1, leader = SPLIT ? crank & ~1u : 0u;
+    const uint16_t both = (uint16_t)(3u << leader);
 
     if (tid == 0) {
         for (int i = 0; i < S; ++i) { mbar_init(full(i), 1); mbar_init(sc_full(i), 1); mbar_init(empty(i), 1 + 8); }
@@ -489,13 +493,16 @@ fp8_gemm_pair_kernel(const F8Params p, const __grid_constant__ CUtensorMap wmap,
     }
     tc_fence_before();
     __syncthreads();
-    cluster_sync();                       // both CTAs' barriers stand
+    cluster_sync();                       // every CTA's barriers stand
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     dependency_trigger();
     dependency_wait();
 
-    const int tiles = p.mt * p.nt, step = gridDim.x / 2;
+    const int split = SPLIT ? p.split : 1;
+    const int tiles = p.mt * p.nt, step = gridDim.x / (2 * split), first_tile = blockIdx.x / (2 * split);
+    const int part = SPLIT ? (int)(crank >> 1) : 0;   // this pair's share of k
+    const int kb0 = SPLIT ? (int)((int64_t)p.KB * part / split) : 0, kb1 = SPLIT ? (int)((int64_t)p.KB * (part + 1) / split) : p.KB;
     bool ok = true;
     auto fail = [&]() {
         ok = false;
@@ -507,12 +514,12 @@ fp8_gemm_pair_kernel(const F8Params p, const __grid_constant__ CUtensorMap wmap,
         regs_down<56>();
         if (warp == 0 && lane == 0) {
             Ring st{};
-            for (int tile = blockIdx.x / 2; tile < tiles && ok; tile += step) {
+            for (int tile = first_tile; tile < tiles && ok; tile += step) {
                 const int nt = tile / p.mt, mt = tile - nt * p.mt;
-                for (int kb = 0; kb < p.KB; ++kb) {
+                for (int kb = kb0; kb < kb1; ++kb) {
                     if (!mbar_wait(empty(st.i), st.ph ^ 1u, abort_flag)) { fail(); break; }
                     if (rank == 0) mbar_expect_tx(full(st.i), 2 * F8P_STAGE);
-                    const uint32_t dst = base + (uint32_t)st.i * F8P_STAGE, bar = at_rank(full(st.i), 0);
+                    const uint32_t dst = base + (uint32_t)st.i * F8P_STAGE, bar = at_rank(full(st.i), leader);
                     tma_load_pair(dst, &xmap, kb * F8_KB, mt * F8P_T + 128 * (int)rank, bar);
                     tma_load_pair(dst + 128 * F8_KB, &wmap, kb * F8_KB, nt * F8P_T + 128 * (int)rank, bar);
                     st.next(S);
@@ -524,14 +531,14 @@ fp8_gemm_pair_kernel(const F8Params p, const __grid_constant__ CUtensorMap wmap,
             constexpr int SB = 2;
             const int wb = (p.N + F8_TN - 1) / F8_TN;
             Ring st{};
-            for (int tile = blockIdx.x / 2; tile < tiles && ok; tile += step) {
+            for (int tile = first_tile; tile < tiles && ok; tile += step) {
                 const int nt = tile / p.mt, mt = tile - nt * p.mt;
                 const int n1 = min(2 * nt + 1, wb - 1);
-                for (int kb = 0; kb < p.KB && ok; kb += SB) {
+                for (int kb = kb0; kb < kb1 && ok; kb += SB) {
                     float v[SB][4], w[SB][2];
 #pragma unroll
                     for (int b = 0; b < SB; ++b) {
-                        const bool live = kb + b < p.KB;
+                        const bool live = kb + b < kb1;
                         w[b][0] = live ? p.ws[(int64_t)(2 * nt) * p.KB + kb + b] : 0.0f;
                         w[b][1] = live ? p.ws[(int64_t)n1 * p.KB + kb + b] : 0.0f;
 #pragma unroll
@@ -542,7 +549,7 @@ fp8_gemm_pair_kernel(const F8Params p, const __grid_constant__ CUtensorMap wmap,
                     }
 #pragma unroll
                     for (int b = 0; b < SB; ++b) {
-                        if (kb + b >= p.KB) break;
+                        if (kb + b >= kb1) break;
                         if (!__all_sync(0xffffffffu, mbar_wait(empty(st.i), st.ph ^ 1u, abort_flag))) { fail(); break; }
                         float *sc = reinterpret_cast<float *>(sbase + F8P_SC) + st.i * 256;
 #pragma unroll
@@ -556,37 +563,44 @@ fp8_gemm_pair_kernel(const F8Params p, const __grid_constant__ CUtensorMap wmap,
                     }
                 }
             }
-        } else if (warp == 1 && lane == 0 && rank == 0) {
-            const uint32_t idesc = idesc_f8(F8P_T, F8P_T);
-            Ring st{}, ab{};
-            for (int tile = blockIdx.x / 2; tile < tiles && ok; tile += step) {
-                for (int kb = 0; kb < p.KB; ++kb) {
-                    if (!mbar_wait_cluster(acc_empty(ab.i), ab.ph ^ 1u, abort_flag) ||
-                        !mbar_wait_cluster(full(st.i), st.ph, abort_flag)) { fail(); break; }
-                    tc_fence_after();
-                    const uint32_t a0 = base + (uint32_t)st.i * F8P_STAGE, b0 = a0 + 128 * F8_KB;
-                    const uint32_t d = tmem + (uint32_t)ab.i * 256u;
+        } else if (warp == 1 && lane == 0) {
+            if (rank == 0) {
+                const uint32_t idesc = idesc_f8(F8P_T, F8P_T);
+                const uint64_t a_desc = smem_desc_sw128(base), b_desc = smem_desc_sw128(base + 128 * F8_KB);
+                Ring st{}, ab{};
+                for (int tile = first_tile; tile < tiles && ok; tile += step) {
+                    for (int kb = kb0; kb < kb1; ++kb) {
+                        if (!mbar_wait(full(st.i), st.ph, abort_flag) || !mbar_wait(acc_empty(ab.i), ab.ph ^ 1u, abort_flag)) {
+                            fail();
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint64_t off = (uint64_t)st.i * (F8P_STAGE >> 4);
+                        const uint32_t d = tmem + (uint32_t)ab.i * 256u;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        tc_mma_f8_pair(d, smem_desc_sw128(a0 + 32u * j), smem_desc_sw128(b0 + 32u * j), idesc, j > 0 ? 1u : 0u);
-                    tc_commit_pair(empty(st.i));
-                    tc_commit_pair(acc_full(ab.i));
-                    st.next(S);
-                    ab.next(2);
+                        for (int j = 0; j < 4; ++j)
+                            tc_mma_f8_pair(d, a_desc + off + 2 * j, b_desc + off + 2 * j, idesc, j > 0 ? 1u : 0u);
+                        tc_commit_pair(acc_full(ab.i), both);
+                        tc_commit_pair(empty(st.i), both);
+                        st.next(S);
+                        ab.next(2);
+                    }
                 }
+                tc_commit_pair(drain, both);
             }
+            // every MMA has completed, so every copy it read has landed, in both CTAs
+            if (!mbar_wait(drain, 0, abort_flag)) fail();
         }
-        // every MMA has completed, so every copy it read has landed, in both CTAs
-        if (warp == 1 && lane == 0) {
-            if (rank == 0) tc_commit_pair(drain);
-            if (!mbar_wait_cluster(drain, 0, abort_flag)) fail();
+        if (SPLIT) {
+            cluster_sync();
+            cluster_sync();
         }
     } else {
         regs_up<224>();
         const int q = warp & 3, half = (warp - 4) >> 2;
         float acc[128];
         Ring st{}, ab{};
-        for (int tile = blockIdx.x / 2; tile < tiles && ok; tile += step) {
+        for (int tile = first_tile; tile < tiles && ok; tile += step) {
             const int nt = tile / p.mt, mt = tile - nt * p.mt;
 #pragma unroll
             for (int i = 0; i < 128; ++i) acc[i] = 0.0f;
@@ -602,27 +616,27 @@ fp8_gemm_pair_kernel(const F8Params p, const __grid_constant__ CUtensorMap wmap,
             auto columns = [&](int j) { return tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)ab.i * 256u + (uint32_t)(half * 128 + 32 * j); };
             if (!ready()) break;
             tc_ld32(columns(0), v[0]);
-            for (int kb = 0; kb < p.KB && ok; ++kb) {
+            for (int kb = kb0; kb < kb1 && ok; ++kb) {
                 s = reinterpret_cast<const float *>(sbase + F8P_SC)[st.i * 256 + half * 128 + 32 * q + lane];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    tc_wait_ld();
+                    tc_wait_ld(v[j & 1]);
                     if (j < 3) {
                         tc_ld32(columns(j + 1), v[(j + 1) & 1]);
                     } else {
                         // all of the accumulator has been read
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) { mbar_arrive_at(at_rank(acc_empty(ab.i), 0)); mbar_arrive(empty(st.i)); }
+                        if (lane == 0) { mbar_arrive_at(at_rank(acc_empty(ab.i), leader)); mbar_arrive(empty(st.i)); }
                         st.next(S);
                         ab.next(2);
-                        if (kb + 1 < p.KB && ready()) tc_ld32(columns(0), v[0]);
+                        if (kb + 1 < kb1 && ready()) tc_ld32(columns(0), v[0]);
                     }
 #pragma unroll
                     for (int i = 0; i < 32; ++i) acc[32 * j + i] = fmaf(v[j & 1][i], s, acc[32 * j + i]);
                 }
             }
-            if (!ok) break;
+            if (!ok || SPLIT) break;
             const int m = mt * F8P_T + 128 * (int)rank + 32 * q + lane, n0 = nt * F8P_T + 128 * half;
             if (m < p.M) {
                 T *y = static_cast<T *>(p.y) + (int64_t)m * p.ldy + n0;
@@ -646,11 +660,38 @@ fp8_gemm_pair_kernel(const F8Params p, const __grid_constant__ CUtensorMap wmap,
                 }
             }
         }
+        if (SPLIT) {
+            // column c of the tile belongs to pair c / cols of the cluster; its CTA of this one's
+            // parity receives the sums of every pair in its stage memory (each CTA has drained its
+            // copies and MMAs when it passes the first barrier) and adds them in pair order
+            const int cols = (F8P_T + split - 1) / split;
+            const int nt = first_tile / p.mt, mt = first_tile - nt * p.mt;
+            cluster_sync();
+#pragma unroll
+            for (int j = 0; j < 128; ++j) {
+                const int col = 128 * half + j, to = col / cols;
+                st_cluster(base + 4u * (uint32_t)((part * cols + (col - to * cols)) * F8P_PITCH + 32 * q + lane),
+                           2u * (uint32_t)to + rank, acc[j]);
+            }
+            cluster_sync();
+            const float *sums = reinterpret_cast<const float *>(sbase);
+            const int mine = min(cols, F8P_T - part * cols);
+            for (int r = warp - 4; r < 128; r += 8) {
+                const int m = mt * F8P_T + 128 * (int)rank + r;
+                if (m >= p.M) break;
+                for (int j = lane; j < mine; j += 32) {
+                    float v = 0.0f;
+                    for (int s = 0; s < split; ++s) v += sums[(s * cols + j) * F8P_PITCH + r];
+                    const int n = nt * F8P_T + part * cols + j;
+                    if (n < p.N) static_cast<T *>(p.y)[(int64_t)m * p.ldy + n] = from_f32<T>(v);
+                }
+            }
+        }
     }
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    cluster_sync();                       // neither CTA leaves while the other may arrive on its barriers
+    cluster_sync();                       // no CTA leaves while another may arrive on its barriers
     tc_fence_after();
     if (warp == 1) {
         __syncwarp();
@@ -700,23 +741,25 @@ struct F8Plan {
 F8Plan plan_f8(int32_t M, int32_t N, int32_t KB) {
     constexpr int SMS = 148;
     F8Plan pl{};
-    // a tile for every pair of SMs: two CTAs per tile
-    if (M > 128 && ceil_div(M, F8P_T) * ceil_div(N, F8P_T) >= SMS / 2) {
+    if (M > 128) {
+        // two CTAs per tile; few tiles are split so that every pair of SMs has work, at least
+        // four k-blocks each
         pl.pair = true;
         pl.mt = (int)ceil_div(M, F8P_T);
         pl.nt = (int)ceil_div(N, F8P_T);
-        pl.split = 1;
-        pl.grid = SMS;
+        const int64_t tiles = (int64_t)pl.mt * pl.nt;
+        pl.split = (int)std::max<int64_t>(1, std::min<int64_t>({4, KB / 4, SMS / 2 / tiles}));
+        pl.grid = pl.split > 1 ? (int)tiles * 2 * pl.split : (int)std::min<int64_t>(2 * tiles, SMS);
         pl.BN = 128;
         return pl;
     }
-    pl.mt = (int)ceil_div(M, 256);
-    pl.BN = (int)round_up(ceil_div(M, pl.mt), 16);
+    pl.mt = 1;
+    pl.BN = (int)round_up(M, 16);
     pl.nt = (int)ceil_div(N, F8_TN);
-    pl.NB = pl.BN <= 16 ? 16 : pl.BN <= 32 ? 32 : pl.BN <= 64 ? 64 : 128;
-    pl.PW = pl.BN <= 128 ? 4 : 8;
+    pl.PW = pl.BN <= 32 ? 4 : 8;
+    pl.NB = pl.BN <= 16 ? 16 : pl.BN <= 64 ? 32 : 64;
     const int tiles = pl.mt * pl.nt;
-    const int per_sm = pl.NB <= 32 ? 2 : 1;
+    const int per_sm = pl.PW == 4 ? 2 : 1;
     // as many CTAs per tile as give every slot one, at least four k-blocks each
     pl.split = std::max(1, std::min({8, KB / 4, per_sm * SMS / tiles}));
     pl.grid = pl.split > 1 ? tiles * pl.split : std::min(tiles, per_sm * SMS);
@@ -746,28 +789,25 @@ int launch_f8(const F8Params &p, const F8Plan &pl, const CUtensorMap &wm, const 
     return Q35_OK;
 }
 
-template <typename T>
+template <typename T, bool SPLIT>
 int launch_f8_pair(const F8Params &p, const F8Plan &pl, const CUtensorMap &wm, const CUtensorMap &xm, int dev, cudaStream_t s) {
-    auto kern = fp8_gemm_pair_kernel<T>;
+    auto kern = fp8_gemm_pair_kernel<T, SPLIT>;
     static bool configured[64] = {};
     if (!configured[dev]) {
         Q35_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)F8P_SMEM));
         configured[dev] = true;
     }
-    Q35_CUDA_TRY(launch_dependent(kern, dim3((unsigned)pl.grid), 384, F8P_SMEM, s, 2, p, wm, xm));
+    Q35_CUDA_TRY(launch_dependent(kern, dim3((unsigned)pl.grid), 384, F8P_SMEM, s, 2 * pl.split, p, wm, xm));
     return Q35_OK;
 }
 
 template <typename T>
 int launch_f8(const F8Params &p, const F8Plan &pl, const CUtensorMap &wm, const CUtensorMap &xm, int dev, cudaStream_t s) {
-    if (pl.pair) return launch_f8_pair<T>(p, pl, wm, xm, dev, s);
-    if (pl.PW == 8) return launch_f8<T, 128, 8>(p, pl, wm, xm, dev, s);
-    switch (pl.NB) {
-    case 16: return launch_f8<T, 16, 4>(p, pl, wm, xm, dev, s);
-    case 32: return launch_f8<T, 32, 4>(p, pl, wm, xm, dev, s);
-    case 64: return launch_f8<T, 64, 4>(p, pl, wm, xm, dev, s);
-    default: return launch_f8<T, 128, 4>(p, pl, wm, xm, dev, s);
-    }
+    if (pl.pair)
+        return pl.split > 1 ? launch_f8_pair<T, true>(p, pl, wm, xm, dev, s) : launch_f8_pair<T, false>(p, pl, wm, xm, dev, s);
+    if (pl.NB == 16) return launch_f8<T, 16, 4>(p, pl, wm, xm, dev, s);
+    if (pl.PW == 4) return launch_f8<T, 32, 4>(p, pl, wm, xm, dev, s);
+    return pl.NB == 32 ? launch_f8<T, 32, 8>(p, pl, wm, xm, dev, s) : launch_f8<T, 64, 8>(p, pl, wm, xm, dev, s);
 }
 
 }  // namespace
