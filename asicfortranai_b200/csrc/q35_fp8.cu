@@ -89,6 +89,10 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map
                  " [%0], [%1, {%2, %3}], [%4];"
                  ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar) : "memory");
 }
+__device__ __forceinline__ void l2_prefetch_2d(const CUtensorMap *map, int32_t x, int32_t y) {
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];"
+                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y) : "memory");
+}
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_commit(uint32_t bar) {
@@ -177,7 +181,9 @@ struct Ring {
 
 // NB: accumulator registers (x rows) per promotion thread; 4 or 8 promotion warps, the second
 // four taking the upper half of the tile's columns (from 33 rows on: one warp per scheduler
-// could not keep up).  Tiles of up to 32 rows leave room for two CTAs on an SM.
+// could not keep up).  Tiles of up to 32 rows run two CTAs on an SM (a third of the memory each,
+// with the next launch's CTA set up beside them, was slower: 23.2 against 20.7 us at
+// 1 x 10240 x 8192; so was one: 32).
 template <typename T, int NB, int PW>
 __global__ void __launch_bounds__(128 + 32 * PW, PW == 4 ? 2 : 1)
 fp8_gemm_kernel(const F8Params p, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap) {
@@ -215,13 +221,16 @@ fp8_gemm_kernel(const F8Params p, const __grid_constant__ CUtensorMap wmap, cons
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    dependency_trigger();
-    dependency_wait();
-
     const int rank = p.split > 1 ? (int)cluster_rank() : 0;
     const int first_tile = blockIdx.x / p.split, step = gridDim.x / p.split;
     const int tiles = p.mt * p.nt;
     const int kb0 = (int)((int64_t)p.KB * rank / p.split), kb1 = (int)((int64_t)p.KB * (rank + 1) / p.split);
+    dependency_trigger();
+    // (a fetch into L2 reads nothing: a kernel before this one may still write w)
+    if (PW == 4 && warp == 0 && lane < S && kb0 + lane < kb1)
+        l2_prefetch_2d(&wmap, (kb0 + lane) * F8_KB, first_tile / p.mt * F8_TN);
+    dependency_wait();
+
     bool ok = true;
     auto fail = [&]() {
         ok = false;
@@ -320,7 +329,7 @@ fp8_gemm_kernel(const F8Params p, const __grid_constant__ CUtensorMap wmap, cons
     } else {
         const int q = warp & 3, half = (warp - 4) >> 2;
         const int c0 = half * NB;                       // first column of this thread
-        constexpr int W = NB < 32 ? NB : 32, NJ = NB / W;   // columns per load, loads per k-block
+        constexpr int W = PW == 4 ? 16 : 32, NJ = NB / W;   // columns per load, loads per k-block
         float acc[NB];
         Ring st{}, ab{};
         for (int tile = first_tile; tile < tiles && ok; tile += step) {
