@@ -86,6 +86,15 @@ template <int CODE> __device__ __forceinline__ uint8_t encode8(float v) {
     }
     return (uint8_t)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
 }
+// four of them, the first in the lowest byte
+template <int CODE> __device__ __forceinline__ uint32_t encode8x4(float a, float b, float c, float d) {
+    if (CODE == Q35_CODE_INT8)
+        return encode8<CODE>(a) | ((uint32_t)encode8<CODE>(b) << 8) | ((uint32_t)encode8<CODE>(c) << 16) |
+               ((uint32_t)encode8<CODE>(d) << 24);
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+    return lo | (hi << 16);
+}
 template <int CODE> __device__ __forceinline__ float decode8(uint8_t c) {
     if (CODE == Q35_CODE_INT8) return (float)(int8_t)c;
     const __half_raw h = __nv_cvt_fp8_to_halfraw(c, __NV_E4M3);
