@@ -113,7 +113,8 @@ class Q35Error(RuntimeError):
 
 def dtype_code(dtype) -> int:
     """Q35_DT_* of "f32", "bf16" or "f16" (other values go to the library, which refuses them)."""
-    return DTYPES.get(dtype, dtype if isinstance(dtype, int) else -1)
+    c = DTYPES.get(dtype)
+    return c if c is not None else dtype if isinstance(dtype, int) else -1
 
 
 def code_of(code) -> int:

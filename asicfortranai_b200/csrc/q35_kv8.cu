@@ -65,6 +65,8 @@ constexpr int APPEND_THREADS = 256;
 template <typename T, int CODE, int D, int TB>
 __global__ void __launch_bounds__(APPEND_THREADS) kv8_append_kernel(const AppendParams p) {
     __shared__ float part[APPEND_THREADS / 32];
+    dependency_trigger();
+    dependency_wait();
     const int s = blockIdx.z >> 1, which = blockIdx.z & 1, head = blockIdx.y;
     const SeqRows q = seq_rows(p.row_start, p.past, s, p.rows, p.max_rows, p.max_seq, p.err);
     if (q.n == 0) return;
@@ -106,6 +108,7 @@ __global__ void __launch_bounds__(APPEND_THREADS) kv8_append_kernel(const Append
 constexpr int ATT_WARPS = 8;
 constexpr int ATT_THREADS = 32 * ATT_WARPS;
 constexpr int ATT_M = 16;                 // (row, head) pairs per CTA
+constexpr int ATT_MAX_SPLITS = 64;        // CTAs that share a tile's keys
 
 struct AttnParams {
     const void *q;
@@ -179,6 +182,9 @@ __device__ __forceinline__ void store_out(const AttnParams &p, int64_t row, int 
     else static_cast<T *>(p.out)[row * p.ldo + (int64_t)head * D + d] = from_f32<T>(v);
 }
 
+// CTAs that share a tile of `steps` steps: at most `splits`, each with a step for every warp
+__device__ __forceinline__ int tile_parts(int steps, int splits) { return max(1, min(splits, steps / ATT_WARPS)); }
+
 // grid (split, tile of 16 (row, head) pairs, seq * kv_heads + kv head)
 template <typename T, int CODE, int D>
 __global__ void __launch_bounds__(ATT_THREADS, 1) kv8_attn_kernel(const AttnParams p) {
@@ -191,6 +197,8 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) kv8_attn_kernel(const AttnPara
     uint32_t *qf = reinterpret_cast<uint32_t *>(sm);   // [TERMS][KS][32][4]
     float *mg = reinterpret_cast<float *>(sm);         // [ATT_WARPS][16][RO]
 
+    dependency_trigger();
+    dependency_wait();
     const int split = blockIdx.x, mt = blockIdx.y;
     const int KVH = p.H / p.G;
     const int seq = blockIdx.z / KVH, kvh = blockIdx.z - seq * KVH;
@@ -204,8 +212,10 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) kv8_attn_kernel(const AttnPara
     // keys of this CTA: an equal share of the keys the tile's last row sees
     const int kend_all = sr.past + (f0 + fn - 1) / p.G + 1;
     const int steps = (kend_all + KC - 1) / KC;
-    const int k0 = (int)((int64_t)steps * split / p.splits) * KC;
-    const int k1 = min(kend_all, (int)((int64_t)steps * (split + 1) / p.splits) * KC);
+    const int parts = tile_parts(steps, p.splits);
+    if (split >= parts) return;
+    const int k0 = (int)((int64_t)steps * split / parts) * KC;
+    const int k1 = min(kend_all, (int)((int64_t)steps * (split + 1) / parts) * KC);
 
     // Q rows: a power of two brings each row's largest element to 2^13..2^14
     for (int r = warp; r < ATT_M; r += ATT_WARPS) {
@@ -452,7 +462,7 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) kv8_attn_kernel(const AttnPara
         }
         const int fr = f0 + r;
         const int64_t slot = (tile * p.splits + split) * ATT_M + r;
-        if (p.splits > 1 && lane == 0) p.part_ml[slot] = make_float2(mm, sum);
+        if (parts > 1 && lane == 0) p.part_ml[slot] = make_float2(mm, sum);
         const float inv = 1.0f / sum;
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
@@ -460,50 +470,87 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) kv8_attn_kernel(const AttnPara
             float v = 0.0f;
 #pragma unroll
             for (int w = 0; w < ATT_WARPS; ++w) v = fmaf(mg[(w * ATT_M + r) * RO + d], f[w], v);
-            if (p.splits > 1) p.part_o[slot * D + d] = v;
+            if (parts > 1) p.part_o[slot * D + d] = v;
             else store_out<T, D>(p, sr.r0 + fr / p.G, kvh * p.G + fr % p.G, d, v * inv);
         }
     }
 }
 
-// joins the splits of a tile: grid (16 rows of a tile, tile, seq * kv_heads + kv head), one warp
+// joins the splits of a tile: grid (16 rows of a tile, tile, seq * kv_heads + kv head), four
+// warps that take the splits in turn
+constexpr int COMBINE_THREADS = 128;
 template <typename T, int D>
-__global__ void __launch_bounds__(32) kv8_combine_kernel(const AttnParams p) {
-    const int r = blockIdx.x, mt = blockIdx.y, lane = threadIdx.x;
+__global__ void __launch_bounds__(COMBINE_THREADS) kv8_combine_kernel(const AttnParams p) {
+    constexpr int E = D / 32;                  // outputs per lane
+    __shared__ float acc[4][D];
+    __shared__ float factor[ATT_MAX_SPLITS], norm;
+    dependency_trigger();
+    dependency_wait();
+    const int r = blockIdx.x, mt = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int KVH = p.H / p.G;
     const int seq = blockIdx.z / KVH, kvh = blockIdx.z - seq * KVH;
     const SeqRows sr = seq_rows(p.row_start, p.past, seq, p.rows, p.max_rows, p.max_seq, p.err);
-    const int f = mt * ATT_M + r;
-    if (f >= sr.n * p.G) return;
+    const int f0 = mt * ATT_M, f = f0 + r, fn = min(ATT_M, sr.n * p.G - f0);
+    if (r >= fn) return;
+    constexpr int KC = AttnShape<D>::KC;
+    const int parts = tile_parts((sr.past + (f0 + fn - 1) / p.G + 1 + KC - 1) / KC, p.splits);
+    if (parts == 1) return;                    // (written by the attention itself)
     const int64_t tile = (int64_t)blockIdx.z * gridDim.y + mt;
     const int64_t slot0 = tile * p.splits * ATT_M + r;
-    float mm = -INFINITY;
-    for (int s = 0; s < p.splits; ++s) mm = fmaxf(mm, p.part_ml[slot0 + (int64_t)s * ATT_M].x);
-    float sum = 0.0f, v[D / 32] = {};
-    for (int s = 0; s < p.splits; ++s) {
-        const int64_t slot = slot0 + (int64_t)s * ATT_M;
-        const float2 a = p.part_ml[slot];
-        const float f2 = ex2(a.x - mm);
-        sum = fmaf(a.y, f2, sum);
+    if (warp == 0) {
+        float2 a[ATT_MAX_SPLITS / 32];
+        float m = -INFINITY, l = 0.0f;
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) v[i] = fmaf(p.part_o[slot * D + lane + 32 * i], f2, v[i]);
+        for (int i = 0; i < ATT_MAX_SPLITS / 32; ++i) {
+            const int s = lane + 32 * i;
+            a[i] = s < parts ? p.part_ml[slot0 + (int64_t)s * ATT_M] : make_float2(-INFINITY, 0.0f);
+            m = fmaxf(m, a[i].x);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const float mu = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int i = 0; i < ATT_MAX_SPLITS / 32; ++i) {
+            const float e = ex2(a[i].x - mu);
+            factor[lane + 32 * i] = e;
+            l = fmaf(a[i].y, e, l);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        if (lane == 0) norm = l;
+    }
+    __syncthreads();
+    float v[E] = {};
+#pragma unroll 4
+    for (int s = warp; s < parts; s += 4) {
+        const float *src = p.part_o + (slot0 + (int64_t)s * ATT_M) * D + lane * E;
+        const float e = factor[s];
+#pragma unroll
+        for (int i = 0; i < E; i += 2) {
+            const float2 u = *reinterpret_cast<const float2 *>(src + i);
+            v[i] = fmaf(u.x, e, v[i]);
+            v[i + 1] = fmaf(u.y, e, v[i + 1]);
+        }
     }
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i)
-        store_out<T, D>(p, sr.r0 + f / p.G, kvh * p.G + f % p.G, lane + 32 * i, v[i] / sum);
+    for (int i = 0; i < E; ++i) acc[warp][lane * E + i] = v[i];
+    __syncthreads();
+    for (int d = threadIdx.x; d < D; d += COMBINE_THREADS)
+        store_out<T, D>(p, sr.r0 + f / p.G, kvh * p.G + f % p.G, d, ((acc[0][d] + acc[1][d]) + (acc[2][d] + acc[3][d])) / norm);
 }
-
 
 struct AttnPlan { int mtiles, splits; int64_t tiles; size_t ml_bytes, o_bytes; };
 
-// splits: enough CTAs for every SM, at least one step of every warp each
+// splits: six CTAs for every SM where the tiles alone are fewer, so that sequences of different
+// lengths even out; at least one step of every warp each
 AttnPlan attn_plan(const q35_kv8_cache &c, int32_t heads, int32_t max_rows) {
     AttnPlan pl;
     const int G = heads / c.kv_heads;
     pl.mtiles = (int)ceil_div((int64_t)max_rows * G, ATT_M);
     pl.tiles = (int64_t)pl.mtiles * c.seqs * c.kv_heads;
     const int64_t keys = (int64_t)ATT_WARPS * (4096 / c.head_dim);
-    pl.splits = (int)std::max<int64_t>(1, std::min<int64_t>(148 / std::max<int64_t>(1, pl.tiles), ceil_div(c.max_seq, keys)));
+    pl.splits = (int)std::max<int64_t>(
+        1, std::min<int64_t>({ATT_MAX_SPLITS, 6 * 148 / std::max<int64_t>(1, pl.tiles), c.max_seq / keys}));
     const int64_t slots = pl.splits > 1 ? pl.tiles * pl.splits * ATT_M : 0;
     pl.ml_bytes = (size_t)round_up(slots * (int64_t)sizeof(float2), 256);
     pl.o_bytes = (size_t)slots * c.head_dim * sizeof(float);
@@ -520,11 +567,9 @@ int launch_attn(const AttnParams &p, const AttnPlan &pl, int zs, cudaStream_t s)
         Q35_CUDA_TRY(cudaFuncSetAttribute(kv8_attn_kernel<T, CODE, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         if (dev >= 0 && dev < 64) configured[dev] = true;
     }
-    kv8_attn_kernel<T, CODE, D><<<dim3(pl.splits, pl.mtiles, zs), ATT_THREADS, smem, s>>>(p);
-    Q35_CUDA_TRY(cudaGetLastError());
+    Q35_CUDA_TRY(launch_dependent(kv8_attn_kernel<T, CODE, D>, dim3(pl.splits, pl.mtiles, zs), ATT_THREADS, smem, s, 1, p));
     if (pl.splits > 1) {
-        kv8_combine_kernel<T, D><<<dim3(ATT_M, pl.mtiles, zs), 32, 0, s>>>(p);
-        Q35_CUDA_TRY(cudaGetLastError());
+        Q35_CUDA_TRY(launch_dependent(kv8_combine_kernel<T, D>, dim3(ATT_M, pl.mtiles, zs), COMBINE_THREADS, 0, s, 1, p));
     }
     return Q35_OK;
 }
@@ -542,13 +587,11 @@ int launch_attn(const AttnParams &p, const AttnPlan &pl, int code, int D, int zs
 
 template <typename T, int CODE, int D>
 int launch_append_b(const AppendParams &p, int block, dim3 grid, cudaStream_t s) {
-    switch (block) {
-    case 16: kv8_append_kernel<T, CODE, D, 16><<<grid, APPEND_THREADS, 0, s>>>(p); break;
-    case 32: kv8_append_kernel<T, CODE, D, 32><<<grid, APPEND_THREADS, 0, s>>>(p); break;
-    case 64: kv8_append_kernel<T, CODE, D, 64><<<grid, APPEND_THREADS, 0, s>>>(p); break;
-    default: kv8_append_kernel<T, CODE, D, 128><<<grid, APPEND_THREADS, 0, s>>>(p); break;
-    }
-    Q35_CUDA_TRY(cudaGetLastError());
+    auto kern = block == 16   ? kv8_append_kernel<T, CODE, D, 16>
+                : block == 32 ? kv8_append_kernel<T, CODE, D, 32>
+                : block == 64 ? kv8_append_kernel<T, CODE, D, 64>
+                              : kv8_append_kernel<T, CODE, D, 128>;
+    Q35_CUDA_TRY(launch_dependent(kern, grid, APPEND_THREADS, 0, s, 1, p));
     return Q35_OK;
 }
 template <typename T, int CODE>

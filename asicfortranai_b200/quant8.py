@@ -57,30 +57,35 @@ class KV8Cache:
                  max_seq: int, block: int = 64, code: str = "e4m3", seq_stride: int = 0, scale_seq_stride: int = 0):
         self.ctx = ctx
         self.kv_heads, self.head_dim = kv_heads, head_dim
+        lib = _lib.load()
+        self._append, self._attention = lib.q35_kv8_append_dev, lib.q35_kv8_attention_dev
         self._c = KV8CacheStruct(_lib.code_of(code), seqs, kv_heads, head_dim, max_seq, block, k, v, k_scale, v_scale,
                                  seq_stride, scale_seq_stride)
+        self._ref = C.byref(self._c)
 
     def append(self, k: int, v: int, row_start: int, past: int, rows: int, max_rows: int, dtype: str = "bf16",
                ld: int | None = None) -> None:
         """Rows row_start[s] .. row_start[s+1]-1 of k and v become sequence s's tokens at
         positions past[s] .. (int32 device arrays); rows in all, at most max_rows of one."""
-        _lib.check(_lib.load().q35_kv8_append_dev(self.ctx.h, C.byref(self._c), _lib.dtype_code(dtype), k, v,
-                                                  self.kv_heads * self.head_dim if ld is None else ld, row_start,
-                                                  past, rows, max_rows), "q35_kv8_append_dev")
+        st = self._append(self.ctx.h, self._ref, _lib.dtype_code(dtype), k, v,
+                          self.kv_heads * self.head_dim if ld is None else ld, row_start, past, rows, max_rows)
+        if st:
+            _lib.check(st, "q35_kv8_append_dev")
 
     def attention(self, q: int, out: int, heads: int, row_start: int, past: int, rows: int, max_rows: int,
                   scale: float, dtype: str = "bf16", ldq: int | None = None, ldo: int | None = None,
                   workspace: int | None = None, workspace_bytes: int = 0) -> None:
         """Causal attention of the rows' queries over the cache, their own tokens included."""
         width = heads * self.head_dim
-        _lib.check(_lib.load().q35_kv8_attention_dev(
-            self.ctx.h, C.byref(self._c), _lib.dtype_code(dtype), q, width if ldq is None else ldq, heads, out,
-            width if ldo is None else ldo, row_start, past, rows, max_rows, scale, workspace, workspace_bytes),
-            "q35_kv8_attention_dev")
+        st = self._attention(self.ctx.h, self._ref, _lib.dtype_code(dtype), q, width if ldq is None else ldq, heads, out,
+                             width if ldo is None else ldo, row_start, past, rows, max_rows, scale, workspace,
+                             workspace_bytes)
+        if st:
+            _lib.check(st, "q35_kv8_attention_dev")
 
     def attention_workspace(self, heads: int, rows: int, max_rows: int) -> int:
         """Bytes of device workspace an attention call of this size needs."""
-        n = _lib.load().q35_kv8_attention_workspace(C.byref(self._c), heads, rows, max_rows)
+        n = _lib.load().q35_kv8_attention_workspace(self._ref, heads, rows, max_rows)
         if n < 0:
             raise _lib.Q35Error(f"q35_kv8_attention_workspace: {_lib.last_error()}")
         return int(n)
