@@ -12,11 +12,16 @@
 //
 // Attention.  o = sum_j softmax_j(scale q . k_j) v_j over the row's own position and all
 // before it.  The group's query heads read a kv head's codes once: its (row, head) pairs
-// are the 16 rows of an m16n8k16 tensor-core tile.  Codes become fp16 exactly (both codes
+// are one side of m16n8k16 tensor-core tiles -- the 8 columns (kv8_attn8_kernel, up to 8 pairs
+// in all: single tokens) or the 16 rows (kv8_attn_kernel).  Codes become fp16 exactly (both codes
 // fit its 11 bits), the scale multiplies the fp32 scores of its block, and v's scale the
 // probabilities, relative to the largest v scale seen so far (at most 1), so no range is
 // lost.  A query row is scaled by a power of two to use fp16's range; fp32 queries and their
 // probabilities take two fp16 terms each (22 bits).  Maximum, sum and outputs are fp32.
+//
+// Single tokens are bound by HBM in the end and by instructions on the way (two conversions a
+// pair of codes); their form takes K and V^T as the 16-row operand, so that half the MMAs and half
+// the accumulators do, and turns the weights around with movmatrix.
 //
 // No shared-memory staging of codes: a lane's 16 consecutive bytes of a key serve four
 // k-steps of Q K^T (the order of the d indices is free as long as Q uses the same), and its
@@ -119,7 +124,7 @@ struct AttnParams {
     int64_t ldq, ldo, seq_stride, scale_seq_stride;
     const int32_t *row_start, *past;
     int32_t rows, max_rows, H, G, max_seq, nblk;   // G: heads per kv head
-    int32_t splits, tiles;
+    int32_t splits, tile_rows, step_keys;          // rows of a tile, keys of a warp's step
     int32_t block_shift;                           // log2 of the tokens per scale
     float scale;
     float *part_o;                                 // [tile][split][16][D] unnormalised outputs
@@ -136,6 +141,11 @@ __device__ __forceinline__ uint4 ldg16(const uint8_t *p) {
     uint4 v;
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
                  : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ float ldg(const float *p) {
+    float v;
+    asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
     return v;
 }
 __device__ __forceinline__ uint2 ldg8(const uint8_t *p) {
@@ -164,7 +174,10 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint4 &a, uint32_t
 }
 
 template <int D> struct AttnShape {
-    static constexpr int KC = 4096 / D;        // keys per warp and step: 64, 32, 16
+    // keys per warp and step: 32, 16, 16 (twice as many for D = 64 and 128 left room for one CTA an
+    // SM, whose two warps a scheduler waited for memory: 104 against 91 us for three long sequences)
+    static constexpr int KC = D == 64 ? 32 : 16;
+    static constexpr int CTAS = D == 256 ? 1 : 2;   // per SM
     static constexpr int KS = D / 16;          // k-steps of Q K^T
     static constexpr int ROWS_O = D + 4;       // padded row of the merge buffer, floats
 };
@@ -187,7 +200,7 @@ __device__ __forceinline__ int tile_parts(int steps, int splits) { return max(1,
 
 // grid (split, tile of 16 (row, head) pairs, seq * kv_heads + kv head)
 template <typename T, int CODE, int D>
-__global__ void __launch_bounds__(ATT_THREADS, 1) kv8_attn_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(ATT_THREADS, AttnShape<D>::CTAS) kv8_attn_kernel(const AttnParams p) {
     constexpr int TERMS = std::is_same<T, float>::value ? 2 : 1;
     constexpr int KC = AttnShape<D>::KC, KS = AttnShape<D>::KS, NT = KC / 8, VT = D / 8;
     constexpr int RO = AttnShape<D>::ROWS_O;
@@ -257,6 +270,7 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) kv8_attn_kernel(const AttnPara
         lim[h] = r < fn ? sr.past + (f0 + r) / p.G + 1 : 0;
         qs[h] = qscale[r];
     }
+    const int all_see = min(k1, sr.past + f0 / p.G + 1);     // keys below this: every row sees them
     const int64_t hb = seq * p.seq_stride + (int64_t)kvh * p.max_seq * D;
     const uint8_t *kb = p.k + hb, *vb = p.v + hb;
     const int64_t sb = seq * p.scale_seq_stride + (int64_t)kvh * p.nblk;
@@ -278,7 +292,7 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) kv8_attn_kernel(const AttnPara
     auto load_k = [&](int kk) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            const uint8_t *a = kb + (int64_t)min(kk + 8 * t + g, k1 - 1) * D + 16 * c;
+            const uint8_t *a = kb + (int64_t)(kk + KC > k1 ? min(kk + 8 * t + g, k1 - 1) : kk + 8 * t + g) * D + 16 * c;
 #pragma unroll
             for (int j = 0; j < KL; ++j) kr[t][j] = ldg16(a + 64 * j);
         }
@@ -289,7 +303,7 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) kv8_attn_kernel(const AttnPara
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int key = kk + 16 * s + 2 * c + (i & 1) + 8 * (i >> 1);
-                const uint8_t *a = vb + (int64_t)min(key, k1 - 1) * D;
+                const uint8_t *a = vb + (int64_t)(kk + KC > k1 ? min(key, k1 - 1) : key) * D;
                 if constexpr (D == 64) {
                     const uint2 u = ldg8(a + 8 * g);
                     vr[s][i][0][0] = u.x; vr[s][i][0][1] = u.y;
@@ -300,17 +314,40 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) kv8_attn_kernel(const AttnPara
                         vr[s][i][j][0] = u.x; vr[s][i][j][1] = u.y; vr[s][i][j][2] = u.z; vr[s][i][j][3] = u.w;
                     }
                 }
-                if (key >= k1) {                // past the last key: whatever is stored there must not count
+            }
+    };
+    // past the last key: whatever is stored there must not count (where the codes are used: a
+    // selection behind the load would wait for it)
+    auto clear_v = [&](int kk) {
+#pragma unroll
+        for (int s = 0; s < NT / 2; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (kk + 16 * s + 2 * c + (i & 1) + 8 * (i >> 1) >= k1) {
 #pragma unroll
                     for (int j = 0; j < VL; ++j)
 #pragma unroll
                         for (int w = 0; w < VW; ++w) vr[s][i][j][w] = 0u;
                 }
+    };
+
+    // scales of the next step's 16-key pieces (blocks hold 16 tokens or more); as the codes, they
+    // are on their way a step ahead
+    float nks[NT / 2], nvs[NT / 2];
+    auto load_scales = [&](int kk) {
+#pragma unroll
+        for (int u = 0; u < NT / 2; ++u) {
+            const int key = kk + 16 * u;
+            nks[u] = nvs[u] = 0.0f;
+            if (key < k1) {
+                nks[u] = ldg(ksb + (key >> p.block_shift));
+                nvs[u] = ldg(vsb + (key >> p.block_shift));
             }
+        }
     };
 
     int kk = k0 + warp * KC;
-    if (kk < k1) { load_k(kk); load_v(kk); }
+    if (kk < k1) { load_k(kk); load_scales(kk); load_v(kk); }
     for (; kk < k1; kk += ATT_WARPS * KC) {
         const int nk = kk + ATT_WARPS * KC;
         float s[NT][4];
@@ -334,25 +371,32 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) kv8_attn_kernel(const AttnPara
                     if (TERMS == 2) mma16816(s[t], ql, b0, b1);
                 }
             }
-        // scales of the step's 16-key pieces (blocks hold 16 tokens or more)
         float ksc[NT / 2], vsc[NT / 2], vtop = vref;
 #pragma unroll
         for (int u = 0; u < NT / 2; ++u) {
-            const int key = kk + 16 * u;
-            ksc[u] = key < k1 ? ksb[key >> p.block_shift] : 0.0f;
-            vsc[u] = key < k1 ? vsb[key >> p.block_shift] : 0.0f;
+            ksc[u] = nks[u];
+            vsc[u] = nvs[u];
             vtop = fmaxf(vtop, vsc[u]);
         }
-        if (nk < k1) load_k(nk);
+        if (nk < k1) { load_k(nk); load_scales(nk); }
         float mx[2] = {m[0], m[1]};
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int key = kk + 8 * t + 2 * c + (i & 1), h = i >> 1;
-                s[t][i] = key < lim[h] && key < k1 ? s[t][i] * (qs[h] * ksc[t / 2]) : -INFINITY;
-                mx[h] = fmaxf(mx[h], s[t][i]);
-            }
+            for (int i = 0; i < 4; ++i) s[t][i] *= qs[i >> 1] * ksc[t / 2];
+        if (kk + KC > all_see) {                 // some row does not see some key of the step
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int key = kk + 8 * t + 2 * c + (i & 1);
+                    if (key >= lim[i >> 1] || key >= k1) s[t][i] = -INFINITY;
+                }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mx[i >> 1] = fmaxf(mx[i >> 1], s[t][i]);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
@@ -371,10 +415,12 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) kv8_attn_kernel(const AttnPara
             down[h] *= vdown;
             m[h] = mx[h];
         }
+        if (__any_sync(0xffffffffu, down[0] != 1.0f || down[1] != 1.0f)) {
 #pragma unroll
-        for (int t = 0; t < VT; ++t)
+            for (int t = 0; t < VT; ++t)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[t][i] *= down[i >> 1];
+                for (int i = 0; i < 4; ++i) o[t][i] *= down[i >> 1];
+        }
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -384,6 +430,7 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) kv8_attn_kernel(const AttnPara
                 s[t][i] = e;
             }
         // outputs
+        if (kk + KC > k1) clear_v(kk);
 #pragma unroll
         for (int u = 0; u < NT / 2; ++u) {
             const float w = vsc[u] == vref ? 1.0f : vsc[u] * vinv;
@@ -476,7 +523,326 @@ __global__ void __launch_bounds__(ATT_THREADS, 1) kv8_attn_kernel(const AttnPara
     }
 }
 
-// joins the splits of a tile: grid (16 rows of a tile, tile, seq * kv_heads + kv head), four
+// ---- up to 8 (row, head) pairs --------------------------------------------------------
+
+template <int D> struct Attn8Shape {
+    static constexpr int U = D == 64 ? 4 : D == 128 ? 2 : 1;   // 16-key pieces per warp and step
+    static constexpr int KC = 16 * U;
+    static constexpr int KS = D / 16;
+    static constexpr int ROWS_O = D + 4;
+};
+template <int D> constexpr size_t attn8_smem(int terms) {
+    const size_t qf = (size_t)terms * Attn8Shape<D>::KS * 32 * 8;
+    const size_t mg = (size_t)ATT_WARPS * 8 * Attn8Shape<D>::ROWS_O * 4;
+    return qf > mg ? qf : mg;
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
+// grid (split, tile of 8 (row, head) pairs, seq * kv_heads + kv head)
+template <typename T, int CODE, int D>
+__global__ void __launch_bounds__(ATT_THREADS, D == 256 ? 1 : 2) kv8_attn8_kernel(const AttnParams p) {
+    constexpr int TERMS = std::is_same<T, float>::value ? 2 : 1;
+    constexpr int U = Attn8Shape<D>::U, KC = Attn8Shape<D>::KC, KS = Attn8Shape<D>::KS, OT = D / 16;
+    constexpr int RO = Attn8Shape<D>::ROWS_O, TM = 8;
+    extern __shared__ __align__(16) uint8_t sm[];
+    __shared__ float qscale[TM];
+    __shared__ float2 ml[ATT_WARPS][TM];
+    uint32_t *qf = reinterpret_cast<uint32_t *>(sm);   // [KS][32][TERMS][2]
+    float *mg = reinterpret_cast<float *>(sm);         // [ATT_WARPS][8][RO]
+
+    dependency_trigger();
+    dependency_wait();
+    const int split = blockIdx.x, mt = blockIdx.y;
+    const int KVH = p.H / p.G;
+    const int seq = blockIdx.z / KVH, kvh = blockIdx.z - seq * KVH;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const SeqRows sr = seq_rows(p.row_start, p.past, seq, p.rows, p.max_rows, p.max_seq, p.err);
+    const int f0 = mt * TM;
+    const int fn = min(TM, sr.n * p.G - f0);
+    if (fn <= 0) return;
+    const int64_t tile = (int64_t)blockIdx.z * gridDim.y + mt;
+    const int kend_all = sr.past + (f0 + fn - 1) / p.G + 1;
+    const int steps = (kend_all + KC - 1) / KC;
+    const int parts = tile_parts(steps, p.splits);
+    if (split >= parts) return;
+    const int k0 = (int)((int64_t)steps * split / parts) * KC;
+    const int k1 = min(kend_all, (int)((int64_t)steps * (split + 1) / parts) * KC);
+    const int all_see = min(k1, sr.past + f0 / p.G + 1);     // keys below this: every row sees them
+    const int64_t hb = seq * p.seq_stride + (int64_t)kvh * p.max_seq * D;
+    const uint8_t *kb = p.k + hb + 16 * c, *vb = p.v + hb + (D == 64 ? 8 : 16) * g;
+    const int64_t sb = seq * p.scale_seq_stride + (int64_t)kvh * p.nblk;
+    const float *ksb = p.ks + sb, *vsb = p.vs + sb;
+
+    constexpr int KL = D / 64;                  // 16-byte loads per key and lane
+    constexpr int VW = D == 64 ? 2 : 4;         // words per V load
+    constexpr int VL = D == 256 ? 2 : 1;
+    uint4 kr[U][2][KL];                         // keys 16 u + g, + 8: bytes 64 j + 16 c ..
+    uint32_t vr[U][4][VL][VW];                  // keys 16 u + 2c, +1, +8, +9
+    float nks[U], nvs[U];
+    auto load_k = [&](int kk) {
+        const bool tail = kk + KC > k1;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                int key = kk + 16 * u + 8 * h + g;
+                if (tail) key = min(key, k1 - 1);
+#pragma unroll
+                for (int j = 0; j < KL; ++j) kr[u][h][j] = ldg16(kb + (int64_t)key * D + 64 * j);
+            }
+            const int key = min(kk + 16 * u, k1 - 1);
+            nks[u] = ldg(ksb + (key >> p.block_shift));
+            nvs[u] = ldg(vsb + (key >> p.block_shift));
+        }
+    };
+    auto load_v = [&](int kk) {
+        const bool tail = kk + KC > k1;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                int key = kk + 16 * u + 2 * c + (i & 1) + 8 * (i >> 1);
+                if (tail) key = min(key, k1 - 1);
+                const uint8_t *a = vb + (int64_t)key * D;
+                if constexpr (D == 64) {
+                    const uint2 w = ldg8(a);
+                    vr[u][i][0][0] = w.x; vr[u][i][0][1] = w.y;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < VL; ++j) {
+                        const uint4 w = ldg16(a + 128 * j);
+                        vr[u][i][j][0] = w.x; vr[u][i][j][1] = w.y; vr[u][i][j][2] = w.z; vr[u][i][j][3] = w.w;
+                    }
+                }
+            }
+    };
+    int kk = k0 + warp * KC;
+    if (kk < k1) { load_k(kk); load_v(kk); }
+
+    // Q rows, scaled as in kv8_attn_kernel: warp r prepares row r
+    {
+        const int r = warp, f = f0 + r;
+        const bool live = r < fn;
+        const T *src = static_cast<const T *>(p.q) + (live ? (int64_t)(sr.r0 + f / p.G) * p.ldq +
+                                                                 (int64_t)(kvh * p.G + f % p.G) * D : 0);
+        float x[D / 32], a = 0.0f;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+            x[i] = live ? to_f32<T>(src[lane + 32 * i]) : 0.0f;
+            a = fmaxf(a, fabsf(x[i]));
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+        const int e = min(126, 13 - ((int)(__float_as_uint(a) >> 23) - 127));
+        const float up = a > 0.0f ? __uint_as_float((uint32_t)(e + 127) << 23) : 1.0f;
+        if (lane == 0) qscale[r] = p.scale * 1.4426950408889634f * (a > 0.0f ? __uint_as_float((uint32_t)(127 - e) << 23) : 1.0f);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+            const int d = lane + 32 * i;
+            const int ks = (d / 64) * 4 + (d % 16) / 4, ln = r * 4 + (d % 64) / 16, reg = (d >> 1) & 1, half = d & 1;
+            const float y = x[i] * up;
+            const __half hi = __float2half_rn(y);
+            __half *dst = reinterpret_cast<__half *>(qf + (ks * 32 + ln) * 2 * TERMS + reg) + half;
+            *dst = hi;
+            if (TERMS == 2) dst[4] = __float2half_rn(y - __half2float(hi));
+        }
+    }
+    __syncthreads();
+
+    // pairs 2c and 2c + 1: limits, scales, running maximum (the same in every lane of a column)
+    // and this lane's share of the sum
+    int lim[2];
+    float qs[2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int r = 2 * c + h;
+        lim[h] = r < fn ? sr.past + (f0 + r) / p.G + 1 : 0;
+        qs[h] = qscale[r];
+    }
+    float o[OT][4];
+#pragma unroll
+    for (int t = 0; t < OT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[t][i] = 0.0f;
+    float vref = 0.0f, vinv = 0.0f;             // largest v scale so far and its reciprocal
+
+    for (; kk < k1; kk += ATT_WARPS * KC) {
+        const int nk = kk + ATT_WARPS * KC;
+        float s[U][4];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[u][i] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < KL; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t q0, q1, q2, q3;
+                if (TERMS == 2) {
+                    const uint4 v = *reinterpret_cast<const uint4 *>(qf + ((j * 4 + i) * 32 + lane) * 4);
+                    q0 = v.x; q1 = v.y; q2 = v.z; q3 = v.w;
+                } else {
+                    const uint2 v = *reinterpret_cast<const uint2 *>(qf + ((j * 4 + i) * 32 + lane) * 2);
+                    q0 = v.x; q1 = v.y; q2 = q3 = 0u;
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    uint4 a;
+                    const uint4 &x = kr[u][0][j], &y = kr[u][1][j];
+                    codes_f16<CODE>(i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w, a.x, a.z);
+                    codes_f16<CODE>(i == 0 ? y.x : i == 1 ? y.y : i == 2 ? y.z : y.w, a.y, a.w);
+                    mma16816(s[u], a, q0, q1);
+                    if (TERMS == 2) mma16816(s[u], a, q2, q3);
+                }
+            }
+        float ksc[U], vsc[U], vtop = vref;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            ksc[u] = nks[u];
+            vsc[u] = nvs[u];
+            if (kk + 16 * u < k1) vtop = fmaxf(vtop, vsc[u]);
+        }
+        if (nk < k1) load_k(nk);
+        float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[u][i] *= qs[i & 1] * ksc[u];
+        if (kk + KC > all_see) {                 // some row does not see some key of the step
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int key = kk + 16 * u + g + 8 * (i >> 1);
+                    if (key >= lim[i & 1] || key >= k1) s[u][i] = -INFINITY;
+                }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mx[i & 1] = fmaxf(mx[i & 1], s[u][i]);
+        // a larger score or v scale than before: the outputs so far move to the new references
+        if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1] || vtop > vref)) {
+            if (vtop > vref) vinv = 1.0f / vtop;
+            const float vdown = vtop > vref ? vref * vinv : 1.0f;
+            vref = vtop;
+            float down[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float x = fmaxf(mx[h], m[h]);
+#pragma unroll
+                for (int b = 4; b < 32; b <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, b));
+                down[h] = x == -INFINITY ? 1.0f : ex2(m[h] - x);
+                m[h] = x;
+                l[h] *= down[h];
+                down[h] *= vdown;
+            }
+#pragma unroll
+            for (int t = 0; t < OT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[t][i] *= down[i & 1];
+        }
+        if (kk + KC > k1) {
+            // past the last key: whatever is stored there must not count (cleared where the codes
+            // are used: a selection behind the load would wait for it)
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (kk + 16 * u + 2 * c + (i & 1) + 8 * (i >> 1) >= k1) {
+#pragma unroll
+                        for (int j = 0; j < VL; ++j)
+#pragma unroll
+                            for (int w = 0; w < VW; ++w) vr[u][i][j][w] = 0u;
+                    }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float w = kk + 16 * u >= k1 ? 0.0f : vsc[u] == vref ? 1.0f : vsc[u] * vinv;
+            float x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float mu = m[i & 1] == -INFINITY ? 0.0f : m[i & 1];     // a row that has seen no key yet
+                const float e = ex2(s[u][i] - mu);
+                l[i & 1] += e;
+                x[i] = e * w;
+            }
+            const uint32_t h0 = pack2<__half>(x[0], x[1]), h1 = pack2<__half>(x[2], x[3]);
+            const uint32_t b0 = transpose8x8(h0), b1 = transpose8x8(h1);
+            uint32_t c0 = 0u, c1 = 0u;
+            if (TERMS == 2) {
+                const float2 f0 = __half22float2(*reinterpret_cast<const __half2 *>(&h0));
+                const float2 f1 = __half22float2(*reinterpret_cast<const __half2 *>(&h1));
+                c0 = transpose8x8(pack2<__half>(x[0] - f0.x, x[1] - f0.y));
+                c1 = transpose8x8(pack2<__half>(x[2] - f1.x, x[3] - f1.y));
+            }
+#pragma unroll
+            for (int j = 0; j < VL; ++j)
+#pragma unroll
+                for (int w4 = 0; w4 < VW; ++w4)
+#pragma unroll
+                    for (int hh = 0; hh < 2; ++hh) {
+                        // keys 2c, 2c+1 interleaved byte by byte, and keys 2c+8, 2c+9: two d of each
+                        uint4 a;
+                        codes_f16<CODE>(__byte_perm(vr[u][0][j][w4], vr[u][1][j][w4], hh ? 0x7362 : 0x5140), a.x, a.y);
+                        codes_f16<CODE>(__byte_perm(vr[u][2][j][w4], vr[u][3][j][w4], hh ? 0x7362 : 0x5140), a.z, a.w);
+                        const int t = (j * VW + w4) * 2 + hh;
+                        mma16816(o[t], a, b0, b1);
+                        if (TERMS == 2) mma16816(o[t], a, c0, c1);
+                    }
+        }
+        if (nk < k1) load_v(nk);
+    }
+
+    // merge the warps: every warp's rows relative to its own maximum
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int b = 4; b < 32; b <<= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], b);
+        if (g == 0) ml[warp][2 * c + h] = make_float2(m[h], l[h]);
+    }
+    __syncthreads();       // Q fragments are read no more
+#pragma unroll
+    for (int t = 0; t < OT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int d = (D == 64 ? 8 * g : (t / 8) * 128 + 16 * g) + 2 * (t % 8) + (i >> 1);
+            mg[(warp * TM + 2 * c + (i & 1)) * RO + d] = o[t][i] * vref;
+        }
+    __syncthreads();
+    if (warp < fn) {
+        const int r = warp;
+        float mm = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < ATT_WARPS; ++w) mm = fmaxf(mm, ml[w][r].x);
+        const float mu = mm == -INFINITY ? 0.0f : mm;
+        float sum = 0.0f, f[ATT_WARPS];
+#pragma unroll
+        for (int w = 0; w < ATT_WARPS; ++w) {
+            f[w] = ex2(ml[w][r].x - mu);
+            sum = fmaf(ml[w][r].y, f[w], sum);
+        }
+        const int fr = f0 + r;
+        const int64_t slot = (tile * p.splits + split) * TM + r;
+        if (parts > 1 && lane == 0) p.part_ml[slot] = make_float2(mm, sum);
+        const float inv = 1.0f / sum;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+            const int d = lane + 32 * i;
+            float v = 0.0f;
+#pragma unroll
+            for (int w = 0; w < ATT_WARPS; ++w) v = fmaf(mg[(w * TM + r) * RO + d], f[w], v);
+            if (parts > 1) p.part_o[slot * D + d] = v;
+            else store_out<T, D>(p, sr.r0 + fr / p.G, kvh * p.G + fr % p.G, d, v * inv);
+        }
+    }
+}
+
+// joins the splits of a tile: grid (rows of a tile, tile, seq * kv_heads + kv head), four
 // warps that take the splits in turn
 constexpr int COMBINE_THREADS = 128;
 template <typename T, int D>
@@ -490,20 +856,19 @@ __global__ void __launch_bounds__(COMBINE_THREADS) kv8_combine_kernel(const Attn
     const int KVH = p.H / p.G;
     const int seq = blockIdx.z / KVH, kvh = blockIdx.z - seq * KVH;
     const SeqRows sr = seq_rows(p.row_start, p.past, seq, p.rows, p.max_rows, p.max_seq, p.err);
-    const int f0 = mt * ATT_M, f = f0 + r, fn = min(ATT_M, sr.n * p.G - f0);
+    const int f0 = mt * p.tile_rows, f = f0 + r, fn = min(p.tile_rows, sr.n * p.G - f0);
     if (r >= fn) return;
-    constexpr int KC = AttnShape<D>::KC;
-    const int parts = tile_parts((sr.past + (f0 + fn - 1) / p.G + 1 + KC - 1) / KC, p.splits);
+    const int parts = tile_parts((sr.past + (f0 + fn - 1) / p.G + p.step_keys) / p.step_keys, p.splits);
     if (parts == 1) return;                    // (written by the attention itself)
     const int64_t tile = (int64_t)blockIdx.z * gridDim.y + mt;
-    const int64_t slot0 = tile * p.splits * ATT_M + r;
+    const int64_t slot0 = tile * p.splits * p.tile_rows + r;
     if (warp == 0) {
         float2 a[ATT_MAX_SPLITS / 32];
         float m = -INFINITY, l = 0.0f;
 #pragma unroll
         for (int i = 0; i < ATT_MAX_SPLITS / 32; ++i) {
             const int s = lane + 32 * i;
-            a[i] = s < parts ? p.part_ml[slot0 + (int64_t)s * ATT_M] : make_float2(-INFINITY, 0.0f);
+            a[i] = s < parts ? p.part_ml[slot0 + (int64_t)s * p.tile_rows] : make_float2(-INFINITY, 0.0f);
             m = fmaxf(m, a[i].x);
         }
 #pragma unroll
@@ -523,7 +888,7 @@ __global__ void __launch_bounds__(COMBINE_THREADS) kv8_combine_kernel(const Attn
     float v[E] = {};
 #pragma unroll 4
     for (int s = warp; s < parts; s += 4) {
-        const float *src = p.part_o + (slot0 + (int64_t)s * ATT_M) * D + lane * E;
+        const float *src = p.part_o + (slot0 + (int64_t)s * p.tile_rows) * D + lane * E;
         const float e = factor[s];
 #pragma unroll
         for (int i = 0; i < E; i += 2) {
@@ -539,19 +904,22 @@ __global__ void __launch_bounds__(COMBINE_THREADS) kv8_combine_kernel(const Attn
         store_out<T, D>(p, sr.r0 + f / p.G, kvh * p.G + f % p.G, d, ((acc[0][d] + acc[1][d]) + (acc[2][d] + acc[3][d])) / norm);
 }
 
-struct AttnPlan { int mtiles, splits; int64_t tiles; size_t ml_bytes, o_bytes; };
+struct AttnPlan { int tile_rows, step_keys, mtiles, splits; int64_t tiles; size_t ml_bytes, o_bytes; };
 
-// splits: six CTAs for every SM where the tiles alone are fewer, so that sequences of different
-// lengths even out; at least one step of every warp each
+// tiles of 8 (row, head) pairs where a sequence has no more, else of 16.  splits: six CTAs for
+// every SM where the tiles alone are fewer, so that sequences of different lengths even out; at
+// least one step of every warp each
 AttnPlan attn_plan(const q35_kv8_cache &c, int32_t heads, int32_t max_rows) {
     AttnPlan pl;
-    const int G = heads / c.kv_heads;
-    pl.mtiles = (int)ceil_div((int64_t)max_rows * G, ATT_M);
+    const int G = heads / c.kv_heads, D = c.head_dim;
+    pl.tile_rows = (int64_t)max_rows * G <= 8 ? 8 : ATT_M;
+    pl.step_keys = pl.tile_rows == 8 ? (D == 64 ? 64 : D == 128 ? 32 : 16) : (D == 64 ? 32 : 16);
+    pl.mtiles = (int)ceil_div((int64_t)max_rows * G, pl.tile_rows);
     pl.tiles = (int64_t)pl.mtiles * c.seqs * c.kv_heads;
-    const int64_t keys = (int64_t)ATT_WARPS * (4096 / c.head_dim);
+    const int64_t keys = (int64_t)ATT_WARPS * pl.step_keys;
     pl.splits = (int)std::max<int64_t>(
         1, std::min<int64_t>({ATT_MAX_SPLITS, 6 * 148 / std::max<int64_t>(1, pl.tiles), c.max_seq / keys}));
-    const int64_t slots = pl.splits > 1 ? pl.tiles * pl.splits * ATT_M : 0;
+    const int64_t slots = pl.splits > 1 ? pl.tiles * pl.splits * pl.tile_rows : 0;
     pl.ml_bytes = (size_t)round_up(slots * (int64_t)sizeof(float2), 256);
     pl.o_bytes = (size_t)slots * c.head_dim * sizeof(float);
     return pl;
@@ -559,18 +927,21 @@ AttnPlan attn_plan(const q35_kv8_cache &c, int32_t heads, int32_t max_rows) {
 
 template <typename T, int CODE, int D>
 int launch_attn(const AttnParams &p, const AttnPlan &pl, int zs, cudaStream_t s) {
-    const size_t smem = attn_smem<D>(std::is_same<T, float>::value ? 2 : 1);
-    static bool configured[64] = {};
+    constexpr int terms = std::is_same<T, float>::value ? 2 : 1;
+    static_assert(AttnShape<D>::KC == (D == 64 ? 32 : 16) && Attn8Shape<D>::KC == (D == 64 ? 64 : D == 128 ? 32 : 16), "attn_plan's steps");
+    const bool small = pl.tile_rows == 8;
+    auto kern = small ? kv8_attn8_kernel<T, CODE, D> : kv8_attn_kernel<T, CODE, D>;
+    const size_t smem = small ? attn8_smem<D>(terms) : attn_smem<D>(terms);
+    static bool configured[64][2] = {};
     int dev = 0;
     Q35_CUDA_TRY(cudaGetDevice(&dev));
-    if (dev < 0 || dev >= 64 || !configured[dev]) {
-        Q35_CUDA_TRY(cudaFuncSetAttribute(kv8_attn_kernel<T, CODE, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        if (dev >= 0 && dev < 64) configured[dev] = true;
+    if (dev < 0 || dev >= 64 || !configured[dev][small]) {
+        Q35_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        if (dev >= 0 && dev < 64) configured[dev][small] = true;
     }
-    Q35_CUDA_TRY(launch_dependent(kv8_attn_kernel<T, CODE, D>, dim3(pl.splits, pl.mtiles, zs), ATT_THREADS, smem, s, 1, p));
-    if (pl.splits > 1) {
-        Q35_CUDA_TRY(launch_dependent(kv8_combine_kernel<T, D>, dim3(ATT_M, pl.mtiles, zs), COMBINE_THREADS, 0, s, 1, p));
-    }
+    Q35_CUDA_TRY(launch_dependent(kern, dim3(pl.splits, pl.mtiles, zs), ATT_THREADS, smem, s, 1, p));
+    if (pl.splits > 1)
+        Q35_CUDA_TRY(launch_dependent(kv8_combine_kernel<T, D>, dim3(pl.tile_rows, pl.mtiles, zs), COMBINE_THREADS, 0, s, 1, p));
     return Q35_OK;
 }
 
@@ -691,7 +1062,7 @@ int launch_kv8_attention(const q35_kv8_cache &c, int dtype, const void *q, int64
     p.row_start = r.row_start; p.past = r.past;
     p.rows = r.rows; p.max_rows = r.max_rows;
     p.H = heads; p.G = heads / c.kv_heads; p.max_seq = c.max_seq; p.nblk = nblk(c);
-    p.splits = pl.splits; p.tiles = (int32_t)pl.tiles;
+    p.splits = pl.splits; p.tile_rows = pl.tile_rows; p.step_keys = pl.step_keys;
     p.block_shift = c.block == 16 ? 4 : c.block == 32 ? 5 : c.block == 64 ? 6 : 7;
     p.scale = scale;
     p.part_ml = static_cast<float2 *>(workspace);
