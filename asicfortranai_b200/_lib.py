@@ -85,6 +85,7 @@ SIGNATURES = {
                                         C.c_float, _vp, _sz]),
     "q35_kv8_attention_workspace": (C.c_int64, [_vp, _i32, _i32, _i32]),
     "q35_model_set_sampling": (C.c_int, [_vp, _vp]),
+    "q35_model_set_kv_format": (C.c_int, [_vp, C.c_int, _i32]),
     "q35_model_create": (C.c_int, [_vp, _vp, C.POINTER(_vp)]),
     "q35_model_create_tp": (C.c_int, [_vp, _vp, _vp, C.POINTER(_vp)]),
     "q35_model_destroy": (C.c_int, [_vp]),

@@ -57,6 +57,7 @@ struct Options {
     uint64_t seed = 0;
     std::string tokenizer;
     std::string tokens_in, tokens_out;
+    int kv_format = Q35_KV_FP32;
     int device = 0;
 };
 
@@ -76,6 +77,8 @@ void usage(FILE *f) {
                  "  --layers/--hidden/--heads/--kv-heads/--head-dim/--ffn/--vocab/--max-seq N\n"
                  "                         override the preset's shape\n"
                  "  --format 3p5|int4      weight format (default: 3p5, int4 with --layer-dir)\n"
+                 "  --kv-cache F           fp32 | int8 | e4m3: how the KV cache is held (default fp32; 8-bit\n"
+                 "                         caches have a scale for each block of 64 tokens and head)\n"
                  "  --rope-mode 0|1        0: the reference's position-in-call angles, 1: absolute\n"
                  "  --weights FILE         3.5-bit safetensors checkpoint (repeat for shards)\n"
                  "  --layer-dir DIR        INT4 stream-binary files DIR/weights_layer{l}.bin\n"
@@ -141,6 +144,14 @@ bool parse(int argc, char **argv, Options &o) {
         else if (a == "--vocab") { if (!(v = need(i))) return false; o.vocab = std::atoi(v); }
         else if (a == "--max-seq") { if (!(v = need(i))) return false; o.max_seq = std::atoi(v); }
         else if (a == "--rope-mode") { if (!(v = need(i))) return false; o.rope_mode = std::atoi(v); }
+        else if (a == "--kv-cache") {
+            if (!(v = need(i))) return false;
+            const std::string f = v;
+            if (f == "fp32") o.kv_format = Q35_KV_FP32;
+            else if (f == "int8") o.kv_format = Q35_KV_INT8;
+            else if (f == "e4m3") o.kv_format = Q35_KV_E4M3;
+            else { std::fprintf(stderr, "llama_generate: unknown KV cache format %s\n", v); return false; }
+        }
         else if (a == "--format") {
             if (!(v = need(i))) return false;
             const std::string f = v;
@@ -332,6 +343,10 @@ int main(int argc, char **argv) {
     smp.seed = o.seed;
     st = q35_model_set_sampling(m, &smp);
     if (st) return fail("sampling", st);
+    if (o.kv_format != Q35_KV_FP32) {
+        st = q35_model_set_kv_format(m, o.kv_format, 64);
+        if (st) return fail("KV cache", st);
+    }
     const int plen = (int)ids.size();
     const int steps = std::max(0, std::min(o.max_tokens, c.max_seq - plen));
     std::vector<int32_t> out((size_t)std::max(1, steps));

@@ -526,7 +526,7 @@ __global__ void __launch_bounds__(ATT_THREADS, AttnShape<D>::CTAS) kv8_attn_kern
 // ---- up to 8 (row, head) pairs --------------------------------------------------------
 
 template <int D> struct Attn8Shape {
-    static constexpr int U = D == 64 ? 4 : D == 128 ? 2 : 1;   // 16-key pieces per warp and step
+    static constexpr int U = D == 64 ? 2 : 1;                // 16-key pieces per warp and step (twice as many spilled)
     static constexpr int KC = 16 * U;
     static constexpr int KS = D / 16;
     static constexpr int ROWS_O = D + 4;
@@ -913,7 +913,7 @@ AttnPlan attn_plan(const q35_kv8_cache &c, int32_t heads, int32_t max_rows) {
     AttnPlan pl;
     const int G = heads / c.kv_heads, D = c.head_dim;
     pl.tile_rows = (int64_t)max_rows * G <= 8 ? 8 : ATT_M;
-    pl.step_keys = pl.tile_rows == 8 ? (D == 64 ? 64 : D == 128 ? 32 : 16) : (D == 64 ? 32 : 16);
+    pl.step_keys = D == 64 ? 32 : 16;
     pl.mtiles = (int)ceil_div((int64_t)max_rows * G, pl.tile_rows);
     pl.tiles = (int64_t)pl.mtiles * c.seqs * c.kv_heads;
     const int64_t keys = (int64_t)ATT_WARPS * pl.step_keys;
@@ -928,7 +928,7 @@ AttnPlan attn_plan(const q35_kv8_cache &c, int32_t heads, int32_t max_rows) {
 template <typename T, int CODE, int D>
 int launch_attn(const AttnParams &p, const AttnPlan &pl, int zs, cudaStream_t s) {
     constexpr int terms = std::is_same<T, float>::value ? 2 : 1;
-    static_assert(AttnShape<D>::KC == (D == 64 ? 32 : 16) && Attn8Shape<D>::KC == (D == 64 ? 64 : D == 128 ? 32 : 16), "attn_plan's steps");
+    static_assert(AttnShape<D>::KC == (D == 64 ? 32 : 16) && Attn8Shape<D>::KC == AttnShape<D>::KC, "attn_plan's steps");
     const bool small = pl.tile_rows == 8;
     auto kern = small ? kv8_attn8_kernel<T, CODE, D> : kv8_attn_kernel<T, CODE, D>;
     const size_t smem = small ? attn8_smem<D>(terms) : attn_smem<D>(terms);
@@ -1045,6 +1045,12 @@ size_t kv8_attention_workspace(const q35_kv8_cache &c, int32_t heads, int32_t ro
     if (rows <= 0) return 0;
     const AttnPlan pl = attn_plan(c, heads, max_rows);
     return pl.ml_bytes + pl.o_bytes;
+}
+
+size_t kv8_workspace_bound(const q35_kv8_cache &c, int32_t heads) {
+    // tiles * splits is at most 6 * 148 wherever a tile is split at all (attn_plan)
+    (void)heads;
+    return (size_t)6 * 148 * ATT_M * (sizeof(float2) + sizeof(float) * (size_t)c.head_dim) + 256;
 }
 
 int launch_kv8_attention(const q35_kv8_cache &c, int dtype, const void *q, int64_t ldq, int32_t heads, void *out,

@@ -13,6 +13,8 @@ struct Kv8Rows {
 int kv8_check(const q35_kv8_cache *c);
 int launch_kv8_append(const q35_kv8_cache &c, int dtype, const void *k, const void *v, int64_t ld, const Kv8Rows &r,
                       int *err, cudaStream_t s);
+// bytes that cover every call on the cache with at most max_rows rows a sequence
+size_t kv8_workspace_bound(const q35_kv8_cache &c, int32_t heads);
 size_t kv8_attention_workspace(const q35_kv8_cache &c, int32_t heads, int32_t rows, int32_t max_rows);
 // out (q's type, row stride ldo) or, when out_q is set, trunc(127 o) as the next int8 matmul takes it
 // (rows heads * head_dim apart)

@@ -241,6 +241,31 @@ __global__ void rope_kv_kernel(const float *__restrict__ yqkv, float *__restrict
     }
 }
 
+// The same rotation without the cache: q rows, and k in place in the q|k|v rows.
+__global__ void rope_rows_kernel(float *__restrict__ yqkv, float *__restrict__ q, const int32_t *__restrict__ row_seq,
+                                 const int32_t *__restrict__ row_i, const int32_t *__restrict__ cache_pos,
+                                 const float2 *__restrict__ cs, int32_t H, int32_t KVH, int32_t D, int32_t max_seq,
+                                 int32_t rope_mode, int *err) {
+    pdl_trigger();
+    pdl_wait();
+    const int r = blockIdx.x, hh = blockIdx.y;
+    const int i = row_i[r], pos = cache_pos[row_seq[r]] + i;
+    if (pos < 0 || pos >= max_seq) {
+        if (threadIdx.x == 0 && hh == 0) atomicExch(err, Q35_ERR_INVALID);
+        return;
+    }
+    const int rp = rope_mode ? pos : i, half = D / 2;
+    float *y = yqkv + (size_t)r * (H + 2 * KVH) * D + hh * D;     // heads 0..H-1 the queries, then the keys
+    float *to = hh < H ? q + ((size_t)r * H + hh) * D : y;
+    for (int d = threadIdx.x; d < half; d += blockDim.x) {
+        const float2 c = cs[(size_t)rp * half + d];
+        const float2 ab = *reinterpret_cast<const float2 *>(y + 2 * d);
+        const float ra = __fsub_rn(__fmul_rn(ab.x, c.x), __fmul_rn(ab.y, c.y));
+        const float rb = __fadd_rn(__fmul_rn(ab.x, c.y), __fmul_rn(ab.y, c.x));
+        *reinterpret_cast<float2 *>(to + 2 * d) = make_float2(ra, rb);
+    }
+}
+
 // Every fp32 reduction below runs in a fixed order (per-thread fused chains, 32-lane xor
 // butterflies, chunk merges in chunk order) and every exponential is q35_expf, so the
 // results are reproducible bit for bit by a CPU restatement of the same order.
@@ -1083,6 +1108,13 @@ int launch_rope_kv(const float *yqkv, float *q, float *kc, float *vc, const int3
                    cudaStream_t s) {
     return launch_pdl(rope_kv_kernel, dim3(R, H + KVH), dim3(64), 0, s, yqkv, q, kc, vc, row_seq, row_i,
                       cache_pos, cs, layer, n_layers, H, KVH, D, max_seq, rope_mode, err);
+}
+
+int launch_rope_rows(float *yqkv, float *q, const int32_t *row_seq, const int32_t *row_i, const int32_t *cache_pos,
+                     const float2 *cs, int R, int H, int KVH, int D, int max_seq, int rope_mode, int *err,
+                     cudaStream_t s) {
+    return launch_pdl(rope_rows_kernel, dim3(R, H + KVH), dim3(64), 0, s, yqkv, q, row_seq, row_i, cache_pos, cs, H, KVH, D,
+                      max_seq, rope_mode, err);
 }
 
 int attn_part_floats(int R, int H, int D, int max_seq) {

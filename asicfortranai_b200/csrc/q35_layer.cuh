@@ -12,6 +12,9 @@ int launch_rope_kv(const float *yqkv, float *q, float *kc, float *vc, const int3
                    const int32_t *row_i, const int32_t *cache_pos, const float2 *cs, int layer,
                    int n_layers, int R, int H, int KVH, int D, int max_seq, int rope_mode, int *err,
                    cudaStream_t s);
+// RoPE alone: q and, in place in yqkv, k (the rows of an 8-bit cache's append)
+int launch_rope_rows(float *yqkv, float *q, const int32_t *row_seq, const int32_t *row_i, const int32_t *cache_pos,
+                     const float2 *cs, int R, int H, int KVH, int D, int max_seq, int rope_mode, int *err, cudaStream_t s);
 // floats of the chunk-partial buffer the multi-row attention path needs for R rows
 int attn_part_floats(int R, int H, int D, int max_seq);
 // one row: 8-CTA clusters merging through distributed shared memory; several rows:

@@ -22,6 +22,7 @@
 #include <string>
 #include <vector>
 
+#include "q35_kv8.cuh"
 #include "q35_layer.cuh"
 
 using namespace q35;
@@ -47,6 +48,15 @@ struct q35_model_s {
     float *embed = nullptr, *final_norm = nullptr, *lm_head = nullptr;
     float2 *rope = nullptr;
     float *kc = nullptr, *vc = nullptr;
+    // cache in 8 bits (q35_model_set_kv_format): codes and scales in the order of kc and vc, which
+    // are not held then; row tables of its calls
+    int kv_format = Q35_KV_FP32, kv_block = 0;
+    uint8_t *k8 = nullptr, *v8 = nullptr;
+    float *k8_scale = nullptr, *v8_scale = nullptr;
+    void *kv8_ws = nullptr;
+    int32_t *step_start = nullptr;       // [B + 1] 0, 1, ..: the rows of a decode step
+    int32_t *call_start = nullptr;       // [2] 0, R: the rows of one sequence's call
+    int kv_seq = -1;                     // sequence of the current call (-1: a decode step, row r = sequence r)
     int32_t *cache_pos = nullptr;        // [B] device
     std::vector<int32_t> host_pos;       // mirror of cache_pos
     // activations [maxR][...]
@@ -162,6 +172,57 @@ int generate_matrix(q35_model m, q35_weights *slot, int fmt, int N, int K, uint6
     return q35_weights_generate(m->ctx, fmt, N, K, seed, tid, sigma, slot);
 }
 
+int kv_blocks(q35_model m) { return (m->cfg.max_seq + m->kv_block - 1) / m->kv_block; }
+
+// the 8-bit cache of layer l: all sequences, or sequence `seq` alone
+q35_kv8_cache kv8_view(q35_model m, int l, int seq) {
+    const int64_t per_seq = (int64_t)m->L * m->KVH * m->cfg.max_seq * m->D;
+    const int64_t sc_seq = (int64_t)m->L * m->KVH * kv_blocks(m);
+    const int s0 = seq < 0 ? 0 : seq;
+    const int64_t o = s0 * per_seq + per_seq / m->L * l, so = s0 * sc_seq + sc_seq / m->L * l;
+    q35_kv8_cache c;
+    c.code = m->kv_format == Q35_KV_INT8 ? Q35_CODE_INT8 : Q35_CODE_E4M3;
+    c.seqs = seq < 0 ? m->B : 1;
+    c.kv_heads = m->KVH;
+    c.head_dim = m->D;
+    c.max_seq = m->cfg.max_seq;
+    c.block = m->kv_block;
+    c.k = m->k8 + o; c.v = m->v8 + o;
+    c.k_scale = m->k8_scale + so; c.v_scale = m->v8_scale + so;
+    c.seq_stride = per_seq;
+    c.scale_seq_stride = sc_seq;
+    return c;
+}
+
+// RoPE, append and attention of R rows over the 8-bit cache, from the q|k|v rows; the output as
+// the o projection takes it
+int kv8_rows(q35_model m, int l, int R) {
+    cudaStream_t s = m->ctx->stream;
+    int *err = m->ctx->ws.err;
+    const int ld = m->QN + 2 * m->KN;
+    int st = launch_rope_rows(m->yqkv, m->q, m->row_seq, m->row_i, m->cache_pos, m->rope, R, m->H, m->KVH, m->D,
+                              m->cfg.max_seq, m->cfg.rope_mode, err, s);
+    const q35_kv8_cache c = kv8_view(m, l, m->kv_seq);
+    Kv8Rows r;
+    r.row_start = m->kv_seq < 0 ? m->step_start : m->call_start;
+    r.past = m->cache_pos + (m->kv_seq < 0 ? 0 : m->kv_seq);
+    r.rows = R;
+    r.max_rows = m->kv_seq < 0 ? 1 : R;
+    if (!st) st = launch_kv8_append(c, Q35_DT_F32, m->yqkv + m->QN, m->yqkv + m->QN + m->KN, ld, r, err, s);
+    if (!st)
+        st = launch_kv8_attention(c, Q35_DT_F32, m->q, m->QN, m->H, nullptr, 0, m->xi8, r, 1.0f / sqrtf((float)m->D),
+                                  m->kv8_ws, err, s);
+    return st;
+}
+
+// frees one of the model's allocations ahead of its end
+void drop(q35_model m, void *p) {
+    if (!p) return;
+    auto it = std::find(m->allocs.begin(), m->allocs.end(), p);
+    if (it != m->allocs.end()) m->allocs.erase(it);
+    cudaFree(p);
+}
+
 // attention of R rows in chunks of 64 rows (the partial buffer holds 64 rows)
 int attention_rows(q35_model m, int l, int R) {
     int st = Q35_OK;
@@ -200,13 +261,18 @@ int layer_rows(q35_model m, int l, int R, bool pre_normed = false, const float *
     rope.row_seq = m->row_seq; rope.row_i = m->row_i; rope.cache_pos = m->cache_pos; rope.cs = m->rope;
     rope.layer = l; rope.n_layers = m->L; rope.H = m->H; rope.KVH = m->KVH; rope.D = m->D;
     rope.max_seq = c.max_seq; rope.rope_mode = c.rope_mode;
-    bool roped = false;
-    if (!st) st = gemm_rows_rope(ctx, w.qkv, m->xi8, R, m->yqkv, rope, &roped);
-    if (!st && !roped) st = gemm_rows(ctx, w.qkv, m->xi8, R, nullptr, m->yqkv, nullptr);
-    if (!st && !roped)
-        st = launch_rope_kv(m->yqkv, m->q, m->kc, m->vc, m->row_seq, m->row_i, m->cache_pos, m->rope, l, m->L, R,
-                            m->H, m->KVH, m->D, c.max_seq, c.rope_mode, err, s);
-    if (!st) st = attention_rows(m, l, R);
+    if (m->kv_format == Q35_KV_FP32) {
+        bool roped = false;
+        if (!st) st = gemm_rows_rope(ctx, w.qkv, m->xi8, R, m->yqkv, rope, &roped);
+        if (!st && !roped) st = gemm_rows(ctx, w.qkv, m->xi8, R, nullptr, m->yqkv, nullptr);
+        if (!st && !roped)
+            st = launch_rope_kv(m->yqkv, m->q, m->kc, m->vc, m->row_seq, m->row_i, m->cache_pos, m->rope, l, m->L, R,
+                                m->H, m->KVH, m->D, c.max_seq, c.rope_mode, err, s);
+        if (!st) st = attention_rows(m, l, R);
+    } else {
+        if (!st) st = gemm_rows(ctx, w.qkv, m->xi8, R, nullptr, m->yqkv, nullptr);
+        if (!st) st = kv8_rows(m, l, R);
+    }
     bool ffn_normed = false;
     if (m->world == 1) {
         if (!st) st = gemm_rows(ctx, w.o, m->xi8, R, nullptr, m->x, m->x);
@@ -740,13 +806,81 @@ int q35_model_set_sampling(q35_model m, const q35_sampling *cfg) {
     return Q35_OK;
 }
 
+// the new arrays are allocated before the old ones go, so a failure leaves the model as it was
+int q35_model_set_kv_format(q35_model m, int format, int32_t block) {
+    if (!m) return set_error(Q35_ERR_INVALID, "model is NULL");
+    if (format != Q35_KV_FP32 && format != Q35_KV_INT8 && format != Q35_KV_E4M3)
+        return set_error(Q35_ERR_INVALID, "set_kv_format: unknown format");
+    if (format != Q35_KV_FP32 && block != 16 && block != 32 && block != 64 && block != 128)
+        return set_error(Q35_ERR_INVALID, "set_kv_format: block must be 16, 32, 64 or 128 tokens");
+    if (format == Q35_KV_FP32) block = 0;
+    if (format != Q35_KV_FP32 && (int64_t)m->B * m->KVH > 32767)
+        return set_error(Q35_ERR_INVALID, "set_kv_format: more than 32767 sequences x kv heads");
+    DeviceGuard g(m->ctx->device);
+    {
+        std::lock_guard<std::mutex> lk(m->ctx->mu);
+        Q35_CUDA_TRY(cudaStreamSynchronize(m->ctx->stream));
+        if (format != m->kv_format || block != m->kv_block) {
+            const size_t kv = (size_t)m->B * m->L * m->KVH * m->cfg.max_seq * m->D;
+            float *kc = nullptr, *vc = nullptr, *ks = nullptr, *vs = nullptr;
+            uint8_t *k8 = nullptr, *v8 = nullptr, *ws = nullptr;
+            int st = Q35_OK;
+            if (format == Q35_KV_FP32) {
+                st = dalloc(m, &kc, kv);
+                if (!st) st = dalloc(m, &vc, kv);
+            } else {
+                const size_t sc = (size_t)m->B * m->L * m->KVH * ((m->cfg.max_seq + block - 1) / block);
+                q35_kv8_cache probe{};
+                probe.head_dim = m->D;
+                st = dalloc(m, &k8, kv);
+                if (!st) st = dalloc(m, &v8, kv);
+                if (!st) st = dalloc(m, &ks, sc);
+                if (!st) st = dalloc(m, &vs, sc);
+                if (!st) st = dalloc(m, &ws, kv8_workspace_bound(probe, m->H));
+                if (!st && !m->step_start) {
+                    std::vector<int32_t> t(m->B + 1);
+                    for (int b = 0; b <= m->B; ++b) t[b] = b;
+                    int32_t *a = nullptr, *c = nullptr;
+                    st = dalloc(m, &a, t.size());
+                    if (!st) st = dalloc(m, &c, 2);
+                    if (!st && cudaMemcpy(a, t.data(), t.size() * sizeof(int32_t), cudaMemcpyHostToDevice) != cudaSuccess)
+                        st = set_error(Q35_ERR_CUDA, "set_kv_format: row table");
+                    if (st) { drop(m, a); drop(m, c); }
+                    else { m->step_start = a; m->call_start = c; }
+                }
+            }
+            if (st) {
+                for (void *p : {(void *)kc, (void *)vc, (void *)k8, (void *)v8, (void *)ks, (void *)vs, (void *)ws}) drop(m, p);
+                return st;
+            }
+            if (m->gexec) { cudaGraphExecDestroy(m->gexec); m->gexec = nullptr; }
+            if (m->g) { cudaGraphDestroy(m->g); m->g = nullptr; }
+            for (void *p : {(void *)m->kc, (void *)m->vc, (void *)m->k8, (void *)m->v8, (void *)m->k8_scale,
+                            (void *)m->v8_scale, m->kv8_ws})
+                drop(m, p);
+            m->kc = kc; m->vc = vc; m->k8 = k8; m->v8 = v8; m->k8_scale = ks; m->v8_scale = vs; m->kv8_ws = ws;
+            m->kv_format = format;
+            m->kv_block = block;
+        }
+    }
+    return q35_model_reset(m);
+}
+
 int q35_model_reset(q35_model m) {
     if (!m) return set_error(Q35_ERR_INVALID, "model is NULL");
     DeviceGuard g(m->ctx->device);
     cudaStream_t s = m->ctx->stream;
     const size_t kv = (size_t)m->B * m->L * m->KVH * m->cfg.max_seq * m->D;
-    Q35_CUDA_TRY(cudaMemsetAsync(m->kc, 0, kv * sizeof(float), s));
-    Q35_CUDA_TRY(cudaMemsetAsync(m->vc, 0, kv * sizeof(float), s));
+    if (m->kv_format == Q35_KV_FP32) {
+        Q35_CUDA_TRY(cudaMemsetAsync(m->kc, 0, kv * sizeof(float), s));
+        Q35_CUDA_TRY(cudaMemsetAsync(m->vc, 0, kv * sizeof(float), s));
+    } else {
+        const size_t sc = (size_t)m->B * m->L * m->KVH * kv_blocks(m) * sizeof(float);
+        Q35_CUDA_TRY(cudaMemsetAsync(m->k8, 0, kv, s));
+        Q35_CUDA_TRY(cudaMemsetAsync(m->v8, 0, kv, s));
+        Q35_CUDA_TRY(cudaMemsetAsync(m->k8_scale, 0, sc, s));
+        Q35_CUDA_TRY(cudaMemsetAsync(m->v8_scale, 0, sc, s));
+    }
     Q35_CUDA_TRY(cudaMemsetAsync(m->cache_pos, 0, sizeof(int32_t) * m->B, s));
     Q35_CUDA_TRY(cudaMemsetAsync(m->step_ctr, 0, sizeof(int32_t), s));
     Q35_CUDA_TRY(cudaMemsetAsync(m->draws, 0, sizeof(int32_t) * m->B, s));
@@ -770,6 +904,9 @@ int q35_model_forward(q35_model m, int32_t seq, const int32_t *ids, int32_t S, f
     Q35_CUDA_TRY(cudaMemcpyAsync(m->row_seq, rs.data(), sizeof(int32_t) * S, cudaMemcpyHostToDevice, s));
     Q35_CUDA_TRY(cudaMemcpyAsync(m->row_i, ri.data(), sizeof(int32_t) * S, cudaMemcpyHostToDevice, s));
     Q35_CUDA_TRY(cudaMemcpyAsync(m->seqs, &seq, sizeof(int32_t), cudaMemcpyHostToDevice, s));
+    const int32_t start[2] = {0, S};
+    if (m->call_start) Q35_CUDA_TRY(cudaMemcpyAsync(m->call_start, start, sizeof(start), cudaMemcpyHostToDevice, s));
+    m->kv_seq = seq;
     const int lm0 = logits ? 0 : S - 1, lmn = logits ? S : 1;
     st = forward_rows(m, S, lm0, lmn, m->tok_tmp, 1, S, logits != nullptr, lmn - 1);
     if (st) return st;
@@ -795,6 +932,7 @@ int q35_model_last_tokens(q35_model m, int32_t *tokens) {
 // decode step over all B sequences; ids (host, [B]) overrides the device tokens when set
 static int decode_enqueue(q35_model m) {
     // rows r -> sequence r at position 0 of the call
+    m->kv_seq = -1;
     return forward_rows(m, m->B, 0, m->B, m->tok, m->B, 1, m->gather_logits, 0);
 }
 
@@ -919,6 +1057,9 @@ int q35_model_layer_forward(q35_model m, int32_t layer, int32_t seq, const float
     Q35_CUDA_TRY(cudaMemcpyAsync(m->row_i, ri.data(), sizeof(int32_t) * S, cudaMemcpyHostToDevice, s));
     Q35_CUDA_TRY(cudaMemcpyAsync(m->seqs, &seq, sizeof(int32_t), cudaMemcpyHostToDevice, s));
     m->rows_one_seq = true;
+    const int32_t start[2] = {0, S};
+    if (m->call_start) Q35_CUDA_TRY(cudaMemcpyAsync(m->call_start, start, sizeof(start), cudaMemcpyHostToDevice, s));
+    m->kv_seq = seq;
     st = layer_rows(m, layer, S);
     if (!st && advance) st = launch_advance(m->cache_pos, m->seqs, 1, S, s);
     if (st) return st;
@@ -942,6 +1083,15 @@ int q35_model_debug_buffer(q35_model m, const char *name, void *host, size_t byt
     else if (n == "ygu") { src = m->ygu; cap = R * 2 * (size_t)m->F * 4; }
     else if (n == "xi8") { src = m->xi8; cap = R * (size_t)std::max({m->hidden, m->QN, m->F}); }
     else if (n == "hq") { src = m->hq; cap = R * (size_t)m->F; }
+    else if (m->kv_format != Q35_KV_FP32 && (n == "kc" || n == "vc"))
+        return set_error(Q35_ERR_STATE, "debug_buffer: the cache is held in 8 bits");
+    else if (m->kv_format != Q35_KV_FP32 && (n == "k8" || n == "v8")) {
+        src = n == "k8" ? m->k8 : m->v8;
+        cap = (size_t)m->B * m->L * m->KVH * m->cfg.max_seq * m->D;
+    } else if (m->kv_format != Q35_KV_FP32 && (n == "k8_scale" || n == "v8_scale")) {
+        src = n == "k8_scale" ? m->k8_scale : m->v8_scale;
+        cap = (size_t)m->B * m->L * m->KVH * kv_blocks(m) * sizeof(float);
+    }
     else if (n == "kc") { src = m->kc; cap = (size_t)m->B * m->L * m->KVH * m->cfg.max_seq * m->D * 4; }
     else if (n == "vc") { src = m->vc; cap = (size_t)m->B * m->L * m->KVH * m->cfg.max_seq * m->D * 4; }
     else return set_error(Q35_ERR_INVALID, "debug_buffer: unknown buffer " + n);

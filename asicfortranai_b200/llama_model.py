@@ -8,6 +8,7 @@
     logits = model.forward_llama(ids, S)     # (S, vocab), Fortran order
     out = model.apply_transformer_layer(l, x, S)
     model.set_sampling("top_p", top_p=0.95, seed=1)   # llama_generate.f90:94-98 (default greedy)
+    model.set_kv_cache("int8", block=64)     # the KV cache in 8 bits (default fp32)
     toks = model.generate(prompts, n_steps)  # all sequences of the batch
     model.cleanup_llama_model()
 """
@@ -55,6 +56,7 @@ class Sampling(C.Structure):
                 ("top_p", C.c_float), ("seed", C.c_uint64)]
 
 
+KV_FORMATS = {"fp32": 0, "int8": 1, "e4m3": 2}
 SAMPLE_MODES = {"greedy": 0, "temperature": 1, "top_k": 2, "top_p": 3}
 
 
@@ -171,8 +173,16 @@ class LLaMAModel:
         smp = Sampling(m, temperature, top_k, top_p, seed)
         _lib.check(_lib.load().q35_model_set_sampling(self.h, C.byref(smp)), "set_sampling")
 
+    def set_kv_cache(self, fmt="fp32", block: int = 64):
+        """How the KV cache is held: "fp32" (default), "int8" or "e4m3" with a scale for each
+        block of 16, 32, 64 or 128 tokens and head.  Empties every sequence.  Under tensor
+        parallelism every rank calls it with the same arguments."""
+        f = KV_FORMATS[fmt] if isinstance(fmt, str) else int(fmt)
+        _lib.check(_lib.load().q35_model_set_kv_format(self.h, f, block), "set_kv_cache")
+
     def debug_buffer(self, name: str, shape, dtype=np.float32):
-        """Copy of an internal buffer (row-major): x, yqkv, q, ygu, xi8, kc, vc."""
+        """Copy of an internal buffer (row-major): x, yqkv, q, ygu, xi8, kc, vc (k8, v8,
+        k8_scale, v8_scale of an 8-bit cache)."""
         out = np.zeros(shape, dtype)
         _lib.check(_lib.load().q35_model_debug_buffer(self.h, name.encode(), out.ctypes.data, out.nbytes),
                    "debug_buffer")

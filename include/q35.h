@@ -405,6 +405,13 @@ typedef struct {
     uint64_t seed;
 } q35_sampling;
 int q35_model_set_sampling(q35_model m, const q35_sampling *cfg);
+/* how the model keeps its KV cache (no counterpart in the reference; default Q35_KV_FP32): in
+ * 8 bits with a scale for each block of `block` tokens (16, 32, 64 or 128; ignored for fp32) and
+ * head, by q35_kv8_append_dev's and q35_kv8_attention_dev's rules.  A quarter of the memory, and
+ * a rounding of every key and value to 8 bits.  Empties every sequence (as q35_model_reset);
+ * under tensor parallelism every rank makes the same call. */
+enum { Q35_KV_FP32 = 0, Q35_KV_INT8 = 1, Q35_KV_E4M3 = 2 };
+int q35_model_set_kv_format(q35_model m, int format, int32_t block);
 /* apply_transformer_layer (transformer_layer.f90:527-565) of one layer on host x(S,hidden)
  * column-major for sequence seq; advance != 0 moves the sequence's position by S */
 int q35_model_layer_forward(q35_model m, int32_t layer, int32_t seq, const float *x, int32_t S,
@@ -413,7 +420,9 @@ size_t q35_model_weight_bytes(q35_model m);
 /* copy the first `bytes` of an internal activation buffer to the host, for layer-level
  * checks: "x", "yqkv", "q", "ygu" (fp32, row-major [rows][width]; gate|up columns
  * interleaved), "xi8", "hq" (int8: matmul inputs; hq the down projection's), "kc",
- * "vc" (KV caches [seq][layer][kv_head][max_seq][head_dim]) */
+ * "vc" (KV caches [seq][layer][kv_head][max_seq][head_dim]); with a cache in 8 bits "k8", "v8"
+ * (its codes, the same order) and "k8_scale", "v8_scale" (fp32
+ * [seq][layer][kv_head][ceil(max_seq/block)]) instead of "kc" and "vc" */
 int q35_model_debug_buffer(q35_model m, const char *name, void *host, size_t bytes);
 
 /* ---- drop-in entry points with the reference's own signatures (host pointers) ----
