@@ -19,6 +19,8 @@
 // lost.  A query row is scaled by a power of two to use fp16's range; fp32 queries and their
 // probabilities take two fp16 terms each (22 bits).  Maximum, sum and outputs are fp32.
 //
+// Prompts of 16-bit queries take 128-row tiles on tcgen05 instead (q35_kv8_prompt.cu).
+//
 // Single tokens are bound by HBM in the end and by instructions on the way (two conversions a
 // pair of codes); their form takes K and V^T as the 16-row operand, so that half the MMAs and half
 // the accumulators do, and turns the weights around with movmatrix.
@@ -45,25 +47,6 @@ struct AppendParams {
     int32_t rows, max_rows, G, max_seq, nblk;
     int *err;
 };
-
-// the rows of sequence s: first row, count (0 with the error word set when the tables are
-// inconsistent or the cache would overflow) and the tokens before them
-struct SeqRows { int r0, n, past; };
-__device__ __forceinline__ SeqRows seq_rows(const int32_t *row_start, const int32_t *past, int s, int rows,
-                                            int max_rows, int max_seq, int *err) {
-    SeqRows q;
-    q.r0 = row_start[s];
-    const int r1 = row_start[s + 1];
-    q.n = r1 - q.r0;
-    q.past = past[s];
-    const bool ok = q.r0 >= 0 && r1 >= q.r0 && r1 <= rows && q.n <= max_rows && q.past >= 0 &&
-                    (int64_t)q.past + q.n <= max_seq;
-    if (!ok) {
-        if (threadIdx.x == 0) atomicExch(err, Q35_ERR_INVALID);
-        q.n = 0;
-    }
-    return q;
-}
 
 constexpr int APPEND_THREADS = 256;
 
@@ -115,56 +98,10 @@ constexpr int ATT_THREADS = 32 * ATT_WARPS;
 constexpr int ATT_M = 16;                 // (row, head) pairs per CTA
 constexpr int ATT_MAX_SPLITS = 64;        // CTAs that share a tile's keys
 
-struct AttnParams {
-    const void *q;
-    void *out;
-    int8_t *out_q;
-    const uint8_t *k, *v;
-    const float *ks, *vs;
-    int64_t ldq, ldo, seq_stride, scale_seq_stride;
-    const int32_t *row_start, *past;
-    int32_t rows, max_rows, H, G, max_seq, nblk;   // G: heads per kv head
-    int32_t splits, tile_rows, step_keys;          // rows of a tile, keys of a warp's step
-    int32_t block_shift;                           // log2 of the tokens per scale
-    float scale;
-    float *part_o;                                 // [tile][split][16][D] unnormalised outputs
-    float2 *part_ml;                               // [tile][split][16] maximum (log2 units) and sum
-    int *err;
-};
-
-__device__ __forceinline__ float ex2(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-__device__ __forceinline__ uint4 ldg16(const uint8_t *p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
-}
-__device__ __forceinline__ float ldg(const float *p) {
-    float v;
-    asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
-    return v;
-}
 __device__ __forceinline__ uint2 ldg8(const uint8_t *p) {
     uint2 v;
     asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
     return v;
-}
-// four codes to two fp16 pairs (bytes 0,1 and 2,3)
-template <int CODE> __device__ __forceinline__ void codes_f16(uint32_t w, uint32_t &lo, uint32_t &hi) {
-    if (CODE == Q35_CODE_INT8) {
-        // 0x64xx is the fp16 number 1024 + xx: biased bytes, minus 1024 + 128, exactly
-        const uint32_t u = w ^ 0x80808080u;
-        const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
-        asm("sub.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(a), "r"(0x64806480u));
-        asm("sub.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(b), "r"(0x64806480u));
-    } else {
-        asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
-            : "=r"(lo), "=r"(hi) : "r"(w));
-    }
 }
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9},"
@@ -1057,6 +994,7 @@ int launch_kv8_attention(const q35_kv8_cache &c, int dtype, const void *q, int64
                          int64_t ldo, int8_t *out_q, const Kv8Rows &r, float scale, void *workspace, int *err,
                          cudaStream_t s) {
     if (r.rows == 0) return Q35_OK;
+    const bool prompt = !out_q && kv8_prompt_takes(c, dtype, heads, r.max_rows);
     const AttnPlan pl = attn_plan(c, heads, r.max_rows);
     if (pl.mtiles > 65535) return set_error(Q35_ERR_INVALID, "kv8: too many rows in one call");
     AttnParams p;
@@ -1075,6 +1013,7 @@ int launch_kv8_attention(const q35_kv8_cache &c, int dtype, const void *q, int64
     p.part_o = reinterpret_cast<float *>(static_cast<char *>(workspace) + pl.ml_bytes);
     p.err = err;
     const int zs = c.seqs * c.kv_heads;
+    if (prompt) return launch_kv8_prompt(p, dtype, c.code, c.head_dim, zs, s);
     switch (dtype) {
     case Q35_DT_F32: return launch_attn<float>(p, pl, c.code, c.head_dim, zs, s);
     case Q35_DT_BF16: return launch_attn<__nv_bfloat16>(p, pl, c.code, c.head_dim, zs, s);

@@ -1,0 +1,441 @@
+// q35_kv8_prompt.cu -- causal attention of many rows over the 8-bit KV cache on the 5th-generation
+// tensor cores (16-bit queries, head_dim 64 or 128); q35_kv8.cu has the definition, the cache and
+// the other forms.
+//
+// One CTA per tile of 128 (row, head) pairs of a sequence and kv head, two CTAs per SM (one's
+// softmax under the other's MMAs).  Per 64 keys:
+//   * converters: warps 4, 5 turn K's codes into fp16 (exact) in shared memory, keys as rows; warps
+//     6, 7 V's, transposed on the way (a thread's 8 keys x 16 d become 16 rows of 8 keys), so both
+//     MMA operands are K-major with the 128-byte swizzle;
+//   * MMA issuer (warp 8, one thread): S = Q K^T into one of two tensor-memory buffers, then
+//     O += P V with P from tensor memory;
+//   * softmax (warps 0..3, a row per thread): S from tensor memory, times the row's and the
+//     block's scale, masked; weights relative to a reference that follows the running maximum
+//     only when that has grown by 2^8 (weights stay below 2^8, fp16 holds them with 11 bits), so
+//     O is rarely moved; weights times the block's v scale over the largest one so far go back
+//     as fp16 into S's buffer.
+// Sums and O are fp32.  The exponentials (16 a clock and SM: 512 clocks for a tile's 64 keys, as
+// long as the MMAs) and the softmax's other 6 instructions a score bound it.
+//
+// Waits are bounded as in q35_fp8.cu.
+#include <type_traits>
+
+#include "q35_kv8.cuh"
+#include "q35_tc.cuh"
+
+namespace q35 {
+namespace {
+
+constexpr int PT_ROWS = 128;               // (row, head) pairs per CTA
+constexpr int PT_KEYS = 64;                // keys per step
+constexpr int PT_THREADS = 288;
+constexpr float PT_SLACK = 8.0f;           // log2 by which a row's maximum may pass its reference
+
+template <int D> struct Prompt {
+    static constexpr uint32_t Q = PT_ROWS * D * 2, K = PT_KEYS * D * 2, V = D * PT_KEYS * 2;
+    static constexpr uint32_t off_k = Q, off_v = Q + 2 * K, off_bar = Q + 2 * K + 2 * V;
+    static constexpr size_t smem = 1024 + off_bar + 8 * 14 + 16;
+};
+
+__device__ __forceinline__ void tc_mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// A from tensor memory
+__device__ __forceinline__ void tc_mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0],"
+                 " {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16,"
+                 " %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+                 ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+                   "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
+                   "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]),
+                   "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+                 : "memory");
+}
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// D fp32, A and B fp16, both K-major
+__host__ __device__ constexpr uint32_t idesc_f16(int m, int n) {
+    return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ void st_shared16(uint32_t addr, uint4 v) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+// makes this thread's shared-memory writes visible to the tensor cores' reads
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// byte offset of 16-byte chunk `chunk` (0..7) of row `row` in a block of 128-byte rows, 128-byte swizzle
+__device__ __forceinline__ uint32_t swz(int row, int chunk) { return (uint32_t)(row * 128 + ((chunk ^ (row & 7)) << 4)); }
+
+template <typename T, int CODE, int D>
+__global__ void __launch_bounds__(PT_THREADS, 2) kv8_prompt_kernel(const AttnParams p) {
+    using L = Prompt<D>;
+    constexpr int DB = D / 64;                 // 64-element blocks of a row of Q and K
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+    uint8_t *sbase = smem_raw + (base - raw);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t bars = base + L::off_bar;
+    auto k_full = [&](int i) { return bars + 8u * i; };            // 2 converter warps
+    auto k_empty = [&](int i) { return bars + 8u * (2 + i); };     // commit of Q K^T
+    auto v_full = [&](int i) { return bars + 8u * (4 + i); };      // 2 converter warps
+    auto pv_done = [&](int i) { return bars + 8u * (6 + i); };     // commit of P V (frees V's stage and S's buffer)
+    auto s_full = [&](int i) { return bars + 8u * (8 + i); };      // commit of Q K^T
+    auto p_full = [&](int i) { return bars + 8u * (10 + i); };     // 4 softmax warps
+    const uint32_t q_full = bars + 8u * 12, drain = bars + 8u * 13;
+    uint8_t *misc = sbase + L::off_bar + 8 * 14;
+    volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(misc);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(misc + 4);
+
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(k_full(i), 2); mbar_init(k_empty(i), 1); mbar_init(v_full(i), 2);
+            mbar_init(pv_done(i), 1); mbar_init(s_full(i), 1); mbar_init(p_full(i), 4);
+        }
+        mbar_init(q_full, 4);
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_u32((const void *)tmem_slot)), "r"(256u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;          // S buffers at 0 and 64, O at 128
+    dependency_trigger();
+    dependency_wait();
+
+    // the tiles with most keys first
+    const int mt = gridDim.x - 1 - blockIdx.x;
+    const int KVH = p.H / p.G;
+    const int seq = blockIdx.y / KVH, kvh = blockIdx.y - seq * KVH;
+    const SeqRows sr = seq_rows(p.row_start, p.past, seq, p.rows, p.max_rows, p.max_seq, p.err);
+    const int f0 = mt * PT_ROWS;
+    const int fn = min(PT_ROWS, sr.n * p.G - f0);
+    const int kend = fn > 0 ? sr.past + (f0 + fn - 1) / p.G + 1 : 0;   // keys the tile's last row sees
+    const int steps = (kend + PT_KEYS - 1) / PT_KEYS;                  // (0: nothing to do)
+    const int64_t hb = seq * p.seq_stride + (int64_t)kvh * p.max_seq * D;
+    const int64_t sb = seq * p.scale_seq_stride + (int64_t)kvh * p.nblk;
+    bool ok = true;
+    auto fail = [&]() {
+        ok = false;
+        *abort_flag = 1;
+        atomicExch(p.err, Q35_ERR_TIMEOUT);
+    };
+
+    if (warp < 4) {
+        // ---------------- Q, softmax, output: row `tid` of the tile ----------------
+        const int r = tid, f = f0 + r;
+        const bool live = r < fn;
+        const int lim = live ? sr.past + f / p.G + 1 : 0;
+        const int64_t row = sr.r0 + (live ? f / p.G : 0);
+        const int head = kvh * p.G + (live ? f % p.G : 0);
+        float qs = 0.0f;
+        if (steps > 0) {
+            const T *src = static_cast<const T *>(p.q) + row * p.ldq + (int64_t)head * D;
+            float a = 0.0f;
+            if (live) {
+                const bool vec = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
+#pragma unroll 4
+                for (int d = 0; d < D; d += 8) {
+                    __align__(16) T x[8];
+                    if (vec) *reinterpret_cast<uint4 *>(x) = *reinterpret_cast<const uint4 *>(src + d);
+                    else
+                        for (int i = 0; i < 8; ++i) x[i] = src[d + i];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) a = fmaxf(a, fabsf(to_f32<T>(x[i])));
+                }
+            }
+            // a power of two brings the row's largest element to 2^13..2^14
+            const int e = min(126, 13 - ((int)(__float_as_uint(a) >> 23) - 127));
+            const float up = a > 0.0f ? __uint_as_float((uint32_t)(e + 127) << 23) : 1.0f;
+            qs = p.scale * 1.4426950408889634f * (a > 0.0f ? __uint_as_float((uint32_t)(127 - e) << 23) : 1.0f);
+#pragma unroll 4
+            for (int d = 0; d < D; d += 8) {
+                uint32_t w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    w[i] = live ? pack2<__half>(to_f32<T>(src[d + 2 * i]) * up, to_f32<T>(src[d + 2 * i + 1]) * up) : 0u;
+                st_shared16(base + (uint32_t)(d / 64) * (PT_ROWS * 128) + swz(r, (d % 64) / 8), make_uint4(w[0], w[1], w[2], w[3]));
+            }
+            fence_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);
+        }
+
+        const float *ksb = p.ks + sb, *vsb = p.vs + sb;
+        const int all_see = fn > 0 ? sr.past + f0 / p.G + 1 : 0;       // keys below this: every row sees them
+        const uint32_t lanes = (uint32_t)(32 * warp) << 16;
+        float m = -INFINITY, l = 0.0f;            // reference of the weights, their sum
+        float vref = 0.0f, vinv = 0.0f;           // largest v scale so far and its reciprocal
+        float nk[4], nv[4];                       // scales of the next step's 16-key pieces
+        auto load_scales = [&](int kk) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int key = min(kk + 16 * u, kend - 1);
+                nk[u] = ldg(ksb + (key >> p.block_shift));
+                nv[u] = ldg(vsb + (key >> p.block_shift));
+            }
+        };
+        if (steps > 0) load_scales(0);
+        for (int j = 0; j < steps && ok; ++j) {
+            const int b = j & 1, kk = j * PT_KEYS;
+            const uint32_t ph = (uint32_t)((j >> 1) & 1);
+            float ks[4], vs[4], vtop = vref;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                ks[u] = nk[u] * qs;
+                vs[u] = kk + 16 * u < kend ? nv[u] : 0.0f;
+                vtop = fmaxf(vtop, vs[u]);
+            }
+            if (j + 1 < steps) load_scales(kk + PT_KEYS);
+            if (!__all_sync(0xffffffffu, mbar_wait(s_full(b), ph, abort_flag))) { fail(); break; }
+            tc_fence_after();
+            float s[2][32];
+            tc_ld32(tmem + lanes + (uint32_t)(64 * b), s[0]);
+            tc_ld32(tmem + lanes + (uint32_t)(64 * b + 32), s[1]);
+            tc_wait_ld(s[0]);
+            tc_wait_ld(s[1]);
+            float mx = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 64; ++i) s[i / 32][i % 32] *= ks[i / 16];
+            if (kk + PT_KEYS > all_see) {
+#pragma unroll
+                for (int i = 0; i < 64; ++i)
+                    if (kk + i >= lim) s[i / 32][i % 32] = -INFINITY;
+            }
+#pragma unroll
+            for (int i = 0; i < 64; ++i) mx = fmaxf(mx, s[i / 32][i % 32]);
+            // O moves to new references only where a row's maximum has passed its own by 2^8, or for
+            // a larger v scale (the same in every thread)
+            if (__any_sync(0xffffffffu, mx > m + PT_SLACK || vtop > vref)) {
+                if (vtop > vref) vinv = 1.0f / vtop;
+                const float vdown = vtop > vref ? vref * vinv : 1.0f;
+                vref = vtop;
+                const float to = mx > m + PT_SLACK ? mx : m;
+                float down = to == -INFINITY ? 1.0f : ex2(m - to);
+                m = to;
+                l *= down;
+                down *= vdown;
+                if (j > 0) {
+                    if (!__all_sync(0xffffffffu, mbar_wait(pv_done(b ^ 1), (uint32_t)(((j - 1) >> 1) & 1), abort_flag))) { fail(); break; }
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int d = 0; d < D; d += 32) {
+                        float o[32];
+                        uint32_t w[32];
+                        tc_ld32(tmem + lanes + 128u + (uint32_t)d, o);
+                        tc_wait_ld(o);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(o[i] * down);
+                        tc_st32(tmem + lanes + 128u + (uint32_t)d, w);
+                    }
+                    tc_wait_st();
+                }
+            }
+            const float mu = m == -INFINITY ? 0.0f : m;                // a row that has seen no key yet
+            uint32_t pk[32];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const float w = vs[u] == vref ? 1.0f : vs[u] * vinv;
+#pragma unroll
+                for (int i = 16 * u; i < 16 * u + 16; i += 2) {
+                    const float e0 = ex2(s[i / 32][i % 32] - mu), e1 = ex2(s[i / 32][i % 32 + 1] - mu);
+                    l += e0 + e1;
+                    pk[i / 2] = pack2<__half>(e0 * w, e1 * w);
+                }
+            }
+            tc_st32(tmem + lanes + (uint32_t)(64 * b), pk);
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full(b));
+        }
+        if (steps > 0 && ok) {
+            const int b = (steps - 1) & 1;
+            if (!__all_sync(0xffffffffu, mbar_wait(pv_done(b), (uint32_t)(((steps - 1) >> 1) & 1), abort_flag))) fail();
+            tc_fence_after();
+            const float inv = vref / l;
+            T *dst = static_cast<T *>(p.out) + row * p.ldo + (int64_t)head * D;
+            const bool vec = (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
+#pragma unroll 1
+            for (int d = 0; d < D && ok; d += 32) {
+                float o[32];
+                tc_ld32(tmem + lanes + 128u + (uint32_t)d, o);
+                tc_wait_ld(o);
+                if (!live) continue;
+                if (vec) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8)
+                        *reinterpret_cast<uint4 *>(dst + d + i) =
+                            make_uint4(pack2<T>(o[i] * inv, o[i + 1] * inv), pack2<T>(o[i + 2] * inv, o[i + 3] * inv),
+                                       pack2<T>(o[i + 4] * inv, o[i + 5] * inv), pack2<T>(o[i + 6] * inv, o[i + 7] * inv));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) dst[d + i] = from_f32<T>(o[i] * inv);
+                }
+            }
+        }
+    } else if (warp < 6) {
+        // ---------------- K: fp16 rows ----------------
+        const int t = tid - 128;                                     // 0..63: key t of the step
+        const uint8_t *kb = p.k + hb;
+        uint4 c[D / 16];
+        auto load = [&](int j) {
+            const uint8_t *a = kb + (int64_t)min(j * PT_KEYS + t, kend - 1) * D;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) c[i] = ldg16(a + 16 * i);
+        };
+        if (steps > 0) load(0);
+        for (int j = 0; j < steps && ok; ++j) {
+            const int b = j & 1;
+            if (!__all_sync(0xffffffffu, mbar_wait(k_empty(b), (uint32_t)((j >> 1) & 1) ^ 1u, abort_flag))) { fail(); break; }
+            const uint32_t dst = base + L::off_k + (uint32_t)b * L::K;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                uint4 x, y;
+                codes_f16<CODE>(c[i].x, x.x, x.y);
+                codes_f16<CODE>(c[i].y, x.z, x.w);
+                codes_f16<CODE>(c[i].z, y.x, y.y);
+                codes_f16<CODE>(c[i].w, y.z, y.w);
+                const uint32_t blk = dst + (uint32_t)(i / 4) * (PT_KEYS * 128);
+                st_shared16(blk + swz(t, 2 * (i % 4)), x);
+                st_shared16(blk + swz(t, 2 * (i % 4) + 1), y);
+            }
+            if (j + 1 < steps) load(j + 1);
+            fence_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(k_full(b));
+        }
+    } else if (warp < 8) {
+        // ---------------- V: fp16, transposed ----------------
+        const int t = tid - 192, kg = t & 7, dg = t >> 3;            // keys 8 kg .., d 16 dg .. (8 groups at D = 128)
+        const uint8_t *vb = p.v + hb + 16 * dg;
+        uint4 c[8];
+        const bool live = dg < D / 16;
+        auto load = [&](int j) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) c[i] = ldg16(vb + (int64_t)min(j * PT_KEYS + 8 * kg + i, kend - 1) * D);
+        };
+        if (steps > 0 && live) load(0);
+        for (int j = 0; j < steps && ok; ++j) {
+            const int b = j & 1;
+            if (!__all_sync(0xffffffffu, mbar_wait(pv_done(b), (uint32_t)((j >> 1) & 1) ^ 1u, abort_flag))) { fail(); break; }
+            if (live) {
+                // past the last key: whatever is stored there must not count
+                if ((j + 1) * PT_KEYS > kend) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (j * PT_KEYS + 8 * kg + i >= kend) c[i] = make_uint4(0u, 0u, 0u, 0u);
+                }
+                const uint32_t dst = base + L::off_v + (uint32_t)b * L::V;
+                auto word = [&](const uint4 &u, int w) { return w == 0 ? u.x : w == 1 ? u.y : w == 2 ? u.z : u.w; };
+#pragma unroll
+                for (int w = 0; w < 4; ++w)
+#pragma unroll
+                    for (int hh = 0; hh < 2; ++hh) {
+                        uint4 x, y;                                   // d = 16 dg + 4 w + 2 hh, and the next
+                        const uint32_t sel = hh ? 0x7362 : 0x5140;
+                        codes_f16<CODE>(__byte_perm(word(c[0], w), word(c[1], w), sel), x.x, y.x);
+                        codes_f16<CODE>(__byte_perm(word(c[2], w), word(c[3], w), sel), x.y, y.y);
+                        codes_f16<CODE>(__byte_perm(word(c[4], w), word(c[5], w), sel), x.z, y.z);
+                        codes_f16<CODE>(__byte_perm(word(c[6], w), word(c[7], w), sel), x.w, y.w);
+                        const int d = 16 * dg + 4 * w + 2 * hh;
+                        st_shared16(dst + swz(d, kg), x);
+                        st_shared16(dst + swz(d + 1, kg), y);
+                    }
+                if (j + 1 < steps) load(j + 1);
+            }
+            fence_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(v_full(b));
+        }
+    } else if (lane == 0 && steps > 0) {
+        // ---------------- MMA issuer ----------------
+        const uint32_t is = idesc_f16(PT_ROWS, PT_KEYS), io = idesc_f16(PT_ROWS, D);
+        const uint64_t qd = smem_desc_sw128(base);
+        if (!mbar_wait(q_full, 0, abort_flag)) fail();
+        auto scores = [&](int j) {
+            const int b = j & 1;
+            const uint32_t ph = (uint32_t)((j >> 1) & 1);
+            // the buffer's weights have been read: P V of step j - 2
+            if (!mbar_wait(k_full(b), ph, abort_flag) || (j >= 2 && !mbar_wait(pv_done(b), ph ^ 1u, abort_flag))) { fail(); return; }
+            tc_fence_after();
+            const uint64_t kd = smem_desc_sw128(base + L::off_k + (uint32_t)b * L::K);
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i)
+                tc_mma_f16(tmem + (uint32_t)(64 * b), qd + (uint64_t)((i / 4) * (PT_ROWS * 128 >> 4) + 2 * (i % 4)),
+                           kd + (uint64_t)((i / 4) * (PT_KEYS * 128 >> 4) + 2 * (i % 4)), is, i > 0 ? 1u : 0u);
+            tc_commit(k_empty(b));
+            tc_commit(s_full(b));
+        };
+        if (ok) scores(0);
+        for (int j = 0; j < steps && ok; ++j) {
+            const int b = j & 1;
+            const uint32_t ph = (uint32_t)((j >> 1) & 1);
+            if (j + 1 < steps) scores(j + 1);
+            if (!ok) break;
+            if (!mbar_wait(p_full(b), ph, abort_flag) || !mbar_wait(v_full(b), ph, abort_flag)) { fail(); break; }
+            tc_fence_after();
+            const uint64_t vd = smem_desc_sw128(base + L::off_v + (uint32_t)b * L::V);
+#pragma unroll
+            for (int i = 0; i < PT_KEYS / 16; ++i)
+                tc_mma_f16_ts(tmem + 128u, tmem + (uint32_t)(64 * b + 8 * i), vd + (uint64_t)(2 * i), io, j > 0 || i > 0 ? 1u : 0u);
+            tc_commit(pv_done(b));
+        }
+        tc_commit(drain);
+        if (!mbar_wait(drain, 0, abort_flag)) fail();
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 8) {
+        __syncwarp();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256u) : "memory");
+    }
+}
+
+template <typename T, int CODE, int D> int launch_prompt(const AttnParams &p, int zs, cudaStream_t s) {
+    auto kern = kv8_prompt_kernel<T, CODE, D>;
+    static bool configured[64] = {};
+    int dev = 0;
+    Q35_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !configured[dev]) {
+        Q35_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Prompt<D>::smem));
+        if (dev >= 0 && dev < 64) configured[dev] = true;
+    }
+    const dim3 grid((unsigned)ceil_div((int64_t)p.max_rows * p.G, PT_ROWS), (unsigned)zs);
+    Q35_CUDA_TRY(launch_dependent(kern, grid, PT_THREADS, Prompt<D>::smem, s, 1, p));
+    return Q35_OK;
+}
+template <typename T> int launch_prompt(const AttnParams &p, int code, int D, int zs, cudaStream_t s) {
+    if (code == Q35_CODE_INT8)
+        return D == 64 ? launch_prompt<T, Q35_CODE_INT8, 64>(p, zs, s) : launch_prompt<T, Q35_CODE_INT8, 128>(p, zs, s);
+    return D == 64 ? launch_prompt<T, Q35_CODE_E4M3, 64>(p, zs, s) : launch_prompt<T, Q35_CODE_E4M3, 128>(p, zs, s);
+}
+
+}  // namespace
+
+// 16-bit queries with head_dim 64 or 128, half a tile of (row, head) pairs at least: below that the
+// 16-row form has more CTAs and no idle rows
+bool kv8_prompt_takes(const q35_kv8_cache &c, int dtype, int32_t heads, int32_t max_rows) {
+    return dtype != Q35_DT_F32 && c.head_dim <= 128 && (int64_t)max_rows * (heads / c.kv_heads) >= PROMPT_PAIRS;
+}
+
+int launch_kv8_prompt(const AttnParams &p, int dtype, int code, int D, int zs, cudaStream_t s) {
+    return dtype == Q35_DT_BF16 ? launch_prompt<__nv_bfloat16>(p, code, D, zs, s) : launch_prompt<__half>(p, code, D, zs, s);
+}
+
+}  // namespace q35
