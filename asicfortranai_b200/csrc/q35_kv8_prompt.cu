@@ -34,7 +34,7 @@ constexpr float PT_SLACK = 8.0f;           // log2 by which a row's maximum may 
 template <int D> struct Prompt {
     static constexpr uint32_t Q = PT_ROWS * D * 2, K = PT_KEYS * D * 2, V = D * PT_KEYS * 2;
     static constexpr uint32_t off_k = Q, off_v = Q + 2 * K, off_bar = Q + 2 * K + 2 * V;
-    static constexpr size_t smem = 1024 + off_bar + 8 * 14 + 16;
+    static constexpr size_t smem = 1024 + off_bar + 8 * 18 + 16 + 4 * 32;
 };
 
 __device__ __forceinline__ void tc_mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -58,6 +58,13 @@ __device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t (&v)[32])
                    "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
                    "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]),
                    "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+                 : "memory");
+}
+__device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0],"
+                 " {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                 ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+                   "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
                  : "memory");
 }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -90,15 +97,18 @@ __global__ void __launch_bounds__(PT_THREADS, 2) kv8_prompt_kernel(const AttnPar
     auto s_full = [&](int i) { return bars + 8u * (8 + i); };      // commit of Q K^T
     auto p_full = [&](int i) { return bars + 8u * (10 + i); };     // 4 softmax warps
     const uint32_t q_full = bars + 8u * 12, drain = bars + 8u * 13;
-    uint8_t *misc = sbase + L::off_bar + 8 * 14;
+    auto sc_full = [&](int i) { return bars + 8u * (14 + i); };    // a step's scales stand in slot i of 4
+    uint8_t *misc = sbase + L::off_bar + 8 * 18;
     volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(misc);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(misc + 4);
+    float *scales = reinterpret_cast<float *>(misc + 16);          // [4][4 of k, 4 of v]: by 16 keys
 
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(k_full(i), 2); mbar_init(k_empty(i), 1); mbar_init(v_full(i), 2);
             mbar_init(pv_done(i), 1); mbar_init(s_full(i), 1); mbar_init(p_full(i), 4);
         }
+        for (int i = 0; i < 4; ++i) mbar_init(sc_full(i), 1);
         mbar_init(q_full, 4);
         mbar_init(drain, 1);
         *abort_flag = 0;
@@ -157,10 +167,11 @@ __global__ void __launch_bounds__(PT_THREADS, 2) kv8_prompt_kernel(const AttnPar
                     for (int i = 0; i < 8; ++i) a = fmaxf(a, fabsf(to_f32<T>(x[i])));
                 }
             }
-            // a power of two brings the row's largest element to 2^13..2^14
+            // a power of two brings the row's largest element to 2^13..2^14 (the scale's sign with it, so
+            // that the largest product is the largest score)
             const int e = min(126, 13 - ((int)(__float_as_uint(a) >> 23) - 127));
-            const float up = a > 0.0f ? __uint_as_float((uint32_t)(e + 127) << 23) : 1.0f;
-            qs = p.scale * 1.4426950408889634f * (a > 0.0f ? __uint_as_float((uint32_t)(127 - e) << 23) : 1.0f);
+            const float up = copysignf(a > 0.0f ? __uint_as_float((uint32_t)(e + 127) << 23) : 1.0f, p.scale);
+            qs = fabsf(p.scale) * 1.4426950408889634f * (a > 0.0f ? __uint_as_float((uint32_t)(127 - e) << 23) : 1.0f);
 #pragma unroll 4
             for (int d = 0; d < D; d += 8) {
                 uint32_t w[4];
@@ -174,49 +185,46 @@ __global__ void __launch_bounds__(PT_THREADS, 2) kv8_prompt_kernel(const AttnPar
             if (lane == 0) mbar_arrive(q_full);
         }
 
-        const float *ksb = p.ks + sb, *vsb = p.vs + sb;
         const int all_see = fn > 0 ? sr.past + f0 / p.G + 1 : 0;       // keys below this: every row sees them
         const uint32_t lanes = (uint32_t)(32 * warp) << 16;
         float m = -INFINITY, l = 0.0f;            // reference of the weights, their sum
         float vref = 0.0f, vinv = 0.0f;           // largest v scale so far and its reciprocal
-        float nk[4], nv[4];                       // scales of the next step's 16-key pieces
-        auto load_scales = [&](int kk) {
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int key = min(kk + 16 * u, kend - 1);
-                nk[u] = ldg(ksb + (key >> p.block_shift));
-                nv[u] = ldg(vsb + (key >> p.block_shift));
-            }
-        };
-        if (steps > 0) load_scales(0);
         for (int j = 0; j < steps && ok; ++j) {
             const int b = j & 1, kk = j * PT_KEYS;
             const uint32_t ph = (uint32_t)((j >> 1) & 1);
-            float ks[4], vs[4], vtop = vref;
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                ks[u] = nk[u] * qs;
-                vs[u] = kk + 16 * u < kend ? nv[u] : 0.0f;
-                vtop = fmaxf(vtop, vs[u]);
-            }
-            if (j + 1 < steps) load_scales(kk + PT_KEYS);
-            if (!__all_sync(0xffffffffu, mbar_wait(s_full(b), ph, abort_flag))) { fail(); break; }
+            // (a slot is written again for step j + 4, which the K converters reach only after P V of step
+            // j, so its phase is still the one to wait for)
+            if (!__all_sync(0xffffffffu, mbar_wait(sc_full(j & 3), (uint32_t)((j >> 2) & 1), abort_flag) &&
+                                             mbar_wait(s_full(b), ph, abort_flag))) { fail(); break; }
+            const float4 k4 = *reinterpret_cast<const float4 *>(scales + 8 * (j & 3));
+            const float4 v4 = *reinterpret_cast<const float4 *>(scales + 8 * (j & 3) + 4);
+            // (never 0: a masked score times 0 would be NaN)
+            const float ks[4] = {fmaxf(k4.x * qs, 1e-37f), fmaxf(k4.y * qs, 1e-37f), fmaxf(k4.z * qs, 1e-37f), fmaxf(k4.w * qs, 1e-37f)};
+            const float vs[4] = {v4.x, v4.y, v4.z, v4.w};
+            const float vtop = fmaxf(fmaxf(vref, fmaxf(vs[0], vs[1])), fmaxf(vs[2], vs[3]));
             tc_fence_after();
-            float s[2][32];
-            tc_ld32(tmem + lanes + (uint32_t)(64 * b), s[0]);
-            tc_ld32(tmem + lanes + (uint32_t)(64 * b + 32), s[1]);
-            tc_wait_ld(s[0]);
-            tc_wait_ld(s[1]);
+            // the scores are read twice, 32 at a time: for the maximum, then for the weights (all 64 with
+            // their weights would not fit the registers of two CTAs an SM)
+            const bool edge = kk + PT_KEYS > all_see;                  // some row does not see some key
             float mx = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 64; ++i) s[i / 32][i % 32] *= ks[i / 16];
-            if (kk + PT_KEYS > all_see) {
+            for (int hh = 0; hh < 2; ++hh) {
+                float s[32];
+                tc_ld32(tmem + lanes + (uint32_t)(64 * b + 32 * hh), s);
+                tc_wait_ld(s);
+                if (edge) {
 #pragma unroll
-                for (int i = 0; i < 64; ++i)
-                    if (kk + i >= lim) s[i / 32][i % 32] = -INFINITY;
+                    for (int i = 0; i < 32; ++i)
+                        if (kk + 32 * hh + i >= lim) s[i] = -INFINITY;
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    float x = s[16 * u];
+#pragma unroll
+                    for (int i = 1; i < 16; ++i) x = fmaxf(x, s[16 * u + i]);
+                    mx = fmaxf(mx, x * ks[2 * hh + u]);
+                }
             }
-#pragma unroll
-            for (int i = 0; i < 64; ++i) mx = fmaxf(mx, s[i / 32][i % 32]);
             // O moves to new references only where a row's maximum has passed its own by 2^8, or for
             // a larger v scale (the same in every thread)
             if (__any_sync(0xffffffffu, mx > m + PT_SLACK || vtop > vref)) {
@@ -245,18 +253,31 @@ __global__ void __launch_bounds__(PT_THREADS, 2) kv8_prompt_kernel(const AttnPar
                 }
             }
             const float mu = m == -INFINITY ? 0.0f : m;                // a row that has seen no key yet
-            uint32_t pk[32];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const float w = vs[u] == vref ? 1.0f : vs[u] * vinv;
+            for (int hh = 0; hh < 2; ++hh) {
+                // (the weights of the first half take the place of its own scores, the second's too)
+                float s[32];
+                uint32_t pk[16];
+                tc_ld32(tmem + lanes + (uint32_t)(64 * b + 32 * hh), s);
+                tc_wait_ld(s);
+                if (edge) {
 #pragma unroll
-                for (int i = 16 * u; i < 16 * u + 16; i += 2) {
-                    const float e0 = ex2(s[i / 32][i % 32] - mu), e1 = ex2(s[i / 32][i % 32 + 1] - mu);
-                    l += e0 + e1;
-                    pk[i / 2] = pack2<__half>(e0 * w, e1 * w);
+                    for (int i = 0; i < 32; ++i)
+                        if (kk + 32 * hh + i >= lim) s[i] = -INFINITY;
                 }
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const float c = ks[2 * hh + u], v = vs[2 * hh + u];
+                    const float w = v == vref ? 1.0f : v * vinv;
+#pragma unroll
+                    for (int i = 16 * u; i < 16 * u + 16; i += 2) {
+                        const float e0 = ex2(fmaf(s[i], c, -mu)), e1 = ex2(fmaf(s[i + 1], c, -mu));
+                        l += e0 + e1;
+                        pk[i / 2] = pack2<__half>(e0 * w, e1 * w);
+                    }
+                }
+                tc_st16(tmem + lanes + (uint32_t)(64 * b + 16 * hh), pk);
             }
-            tc_st32(tmem + lanes + (uint32_t)(64 * b), pk);
             tc_wait_st();
             tc_fence_before();
             __syncwarp();
@@ -297,7 +318,15 @@ __global__ void __launch_bounds__(PT_THREADS, 2) kv8_prompt_kernel(const AttnPar
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) c[i] = ldg16(a + 16 * i);
         };
-        if (steps > 0) load(0);
+        // lanes 0..3 of warp 4 the step's k scales, 4..7 its v scales
+        const float *sp = (t < 4 ? p.ks : p.vs) + sb;
+        float sc = 0.0f;
+        auto load_scale = [&](int j) {
+            const int key = j * PT_KEYS + 16 * (t & 3);
+            sc = 0.0f;
+            if (t < 8 && key < kend) sc = ldg(sp + (key >> p.block_shift));
+        };
+        if (steps > 0) { load(0); load_scale(0); }
         for (int j = 0; j < steps && ok; ++j) {
             const int b = j & 1;
             if (!__all_sync(0xffffffffu, mbar_wait(k_empty(b), (uint32_t)((j >> 1) & 1) ^ 1u, abort_flag))) { fail(); break; }
@@ -313,10 +342,14 @@ __global__ void __launch_bounds__(PT_THREADS, 2) kv8_prompt_kernel(const AttnPar
                 st_shared16(blk + swz(t, 2 * (i % 4)), x);
                 st_shared16(blk + swz(t, 2 * (i % 4) + 1), y);
             }
-            if (j + 1 < steps) load(j + 1);
+            if (t < 8) scales[8 * (j & 3) + t] = sc;
+            if (j + 1 < steps) { load(j + 1); load_scale(j + 1); }
             fence_async();
             __syncwarp();
-            if (lane == 0) mbar_arrive(k_full(b));
+            if (lane == 0) {
+                mbar_arrive(k_full(b));
+                if (warp == 4) mbar_arrive(sc_full(j & 3));
+            }
         }
     } else if (warp < 8) {
         // ---------------- V: fp16, transposed ----------------
