@@ -30,6 +30,7 @@
 // 16 bytes of each of four keys serve 16 column tiles of P V (the order of the output
 // columns is free), so every load is a 16-byte register load and there is no transpose.
 #include <algorithm>
+#include <cstring>
 #include <type_traits>
 
 #include "q35_kv8.cuh"
@@ -45,6 +46,7 @@ struct AppendParams {
     int64_t seq_stride, scale_seq_stride;
     const int32_t *row_start, *past;
     int32_t rows, max_rows, G, max_seq, nblk;
+    bool vec;                  // rows of x start on 16-byte boundaries
     int *err;
 };
 
@@ -67,10 +69,42 @@ __global__ void __launch_bounds__(APPEND_THREADS) kv8_append_kernel(const Append
     float *scale = p.scales[which] + s * p.scale_seq_stride + (int64_t)head * p.nblk + blk;
     const int held = first - t0, fresh = last - first;
 
-    float amax = 0.0f;
-    for (int e = threadIdx.x; e < fresh * D; e += APPEND_THREADS) {
-        const float a = fabsf(to_f32<T>(x[(int64_t)(e / D) * p.ld + e % D]));
-        if (a <= 3.402823466e38f) amax = fmaxf(amax, a);
+    // four elements a thread and round, all of the block's rounds in flight (a whole block of 128
+    // tokens by 256 is 32 rounds: those take two passes over the input)
+    constexpr int R = TB * D / (4 * APPEND_THREADS) < 8 ? (TB * D / (4 * APPEND_THREADS) < 1 ? 1 : TB * D / (4 * APPEND_THREADS)) : 8;
+    const bool vec = p.vec;
+    auto load4 = [&](int e, float (&v)[4]) {
+        const T *s = x + (int64_t)(e / D) * p.ld + e % D;
+        if (vec) {
+            if constexpr (sizeof(T) == 4) {
+                const float4 u = *reinterpret_cast<const float4 *>(s);
+                v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+            } else {
+                const uint2 u = *reinterpret_cast<const uint2 *>(s);
+                T w[4];
+                memcpy(w, &u, 8);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = to_f32<T>(w[i]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = to_f32<T>(s[i]);
+        }
+    };
+    float amax = 0.0f, v[R][4];
+    const int total = fresh * D;
+    for (int e0 = 4 * threadIdx.x; e0 < total; e0 += 4 * APPEND_THREADS * R) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (e0 + 4 * APPEND_THREADS * r < total) load4(e0 + 4 * APPEND_THREADS * r, v[r]);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (e0 + 4 * APPEND_THREADS * r < total)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float a = fabsf(v[r][i]);
+                    if (a <= 3.402823466e38f) amax = fmaxf(amax, a);
+                }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
@@ -82,12 +116,30 @@ __global__ void __launch_bounds__(APPEND_THREADS) kv8_append_kernel(const Append
     const float now = fmaxf(old, __fdiv_rn(amax, code_max<CODE>()));
     if (threadIdx.x == 0) *scale = now;
     if (held && now != old)
-        for (int e = threadIdx.x; e < held * D; e += APPEND_THREADS)
-            codes[e] = encode8<CODE>(__fdiv_rn(__fmul_rn(decode8<CODE>(codes[e]), old), now));
+        for (int e = 4 * threadIdx.x; e < held * D; e += 4 * APPEND_THREADS) {
+            const uint32_t c = *reinterpret_cast<const uint32_t *>(codes + e);
+            float u[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) u[i] = __fdiv_rn(__fmul_rn(decode8<CODE>((uint8_t)(c >> (8 * i))), old), now);
+            *reinterpret_cast<uint32_t *>(codes + e) = encode8x4<CODE>(u[0], u[1], u[2], u[3]);
+        }
     codes += held * D;
-    for (int e = threadIdx.x; e < fresh * D; e += APPEND_THREADS) {
-        const float v = to_f32<T>(x[(int64_t)(e / D) * p.ld + e % D]);
-        codes[e] = now == 0.0f || v != v ? 0 : encode8<CODE>(__fdiv_rn(v, now));
+    const bool once = total <= 4 * APPEND_THREADS * R;       // the values are still here
+    for (int e0 = 4 * threadIdx.x; e0 < total; e0 += 4 * APPEND_THREADS * R) {
+        if (!once) {
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+                if (e0 + 4 * APPEND_THREADS * r < total) load4(e0 + 4 * APPEND_THREADS * r, v[r]);
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int e = e0 + 4 * APPEND_THREADS * r;
+            if (e >= total) continue;
+            float u[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) u[i] = now == 0.0f || v[r][i] != v[r][i] ? 0.0f : __fdiv_rn(v[r][i], now);
+            *reinterpret_cast<uint32_t *>(codes + e) = encode8x4<CODE>(u[0], u[1], u[2], u[3]);
+        }
     }
 }
 
@@ -967,6 +1019,7 @@ int launch_kv8_append(const q35_kv8_cache &c, int dtype, const void *k, const vo
     p.row_start = r.row_start; p.past = r.past;
     p.rows = r.rows; p.max_rows = r.max_rows;
     p.G = c.kv_heads; p.max_seq = c.max_seq; p.nblk = nblk(c);
+    p.vec = aligned_to(k, 16) && aligned_to(v, 16) && ld * (int64_t)dtype_size(dtype) % 16 == 0;
     p.err = err;
     // blocks a run of max_rows tokens can touch, wherever it starts
     const int bx = (int)((r.max_rows + (int64_t)c.block - 2) / c.block + 1);

@@ -310,13 +310,14 @@ __global__ void __launch_bounds__(PT_THREADS, 2) kv8_prompt_kernel(const AttnPar
         }
     } else if (warp < 6) {
         // ---------------- K: fp16 rows ----------------
-        const int t = tid - 128;                                     // 0..63: key t of the step
-        const uint8_t *kb = p.k + hb;
-        uint4 c[D / 16];
+        // D / 16 neighbouring lanes take a key's row (whole lines); a thread has D / 16 pieces of 16 codes
+        constexpr int LK = D / 16, KR = 64 / LK;                     // lanes per key, keys per round of 64 threads
+        const int t = tid - 128, ch = t % LK, key0 = t / LK;
+        const uint8_t *kb = p.k + hb + 16 * ch;
+        uint4 c[LK];
         auto load = [&](int j) {
-            const uint8_t *a = kb + (int64_t)min(j * PT_KEYS + t, kend - 1) * D;
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i) c[i] = ldg16(a + 16 * i);
+            for (int i = 0; i < LK; ++i) c[i] = ldg16(kb + (int64_t)min(j * PT_KEYS + KR * i + key0, kend - 1) * D);
         };
         // lanes 0..3 of warp 4 the step's k scales, 4..7 its v scales
         const float *sp = (t < 4 ? p.ks : p.vs) + sb;
@@ -331,16 +332,18 @@ __global__ void __launch_bounds__(PT_THREADS, 2) kv8_prompt_kernel(const AttnPar
             const int b = j & 1;
             if (!__all_sync(0xffffffffu, mbar_wait(k_empty(b), (uint32_t)((j >> 1) & 1) ^ 1u, abort_flag))) { fail(); break; }
             const uint32_t dst = base + L::off_k + (uint32_t)b * L::K;
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i) {
+            const uint32_t blk = dst + (uint32_t)(ch / 4) * (PT_KEYS * 128);
+            const int odd = ch / 4;                                  // (the two 64-d blocks' lanes write the
+#pragma unroll                                                       // halves in opposite order: no bank conflicts)
+            for (int i = 0; i < LK; ++i) {
                 uint4 x, y;
                 codes_f16<CODE>(c[i].x, x.x, x.y);
                 codes_f16<CODE>(c[i].y, x.z, x.w);
                 codes_f16<CODE>(c[i].z, y.x, y.y);
                 codes_f16<CODE>(c[i].w, y.z, y.w);
-                const uint32_t blk = dst + (uint32_t)(i / 4) * (PT_KEYS * 128);
-                st_shared16(blk + swz(t, 2 * (i % 4)), x);
-                st_shared16(blk + swz(t, 2 * (i % 4) + 1), y);
+                const int key = KR * i + key0;
+                st_shared16(blk + swz(key, 2 * (ch % 4) + odd), odd ? y : x);
+                st_shared16(blk + swz(key, 2 * (ch % 4) + 1 - odd), odd ? x : y);
             }
             if (t < 8) scales[8 * (j & 3) + t] = sc;
             if (j + 1 < steps) { load(j + 1); load_scale(j + 1); }
