@@ -52,6 +52,39 @@ struct AppendParams {
 
 constexpr int APPEND_THREADS = 256;
 
+// Four codes of x / s.  A code is the fp32 quotient, rounded; x * r with r = 1/s rounded is within
+// 2^-22 of it, so where no rounding boundary lies that near the product rounds to the same code and
+// the division is left out (it costs ten instructions or so a value, the product with its check
+// five).  `fast` is off where r could overflow.
+template <int CODE> __device__ __forceinline__ uint32_t encode_quotients(const float (&x)[4], float s, float r, bool fast) {
+    float t[4];
+    bool near = !fast;
+    uint32_t word = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t[i] = (x[i] != x[i] ? 0.0f : x[i]) * r;
+    if (CODE == Q35_CODE_INT8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float c = fminf(fmaxf(t[i], -127.0f), 127.0f);
+            const float k = __fadd_rn(c, 12582912.0f);        // 3 2^22: the sum's last bits are the whole number
+            near |= fabsf(c - __fadd_rn(k, -12582912.0f)) > 0.4999f;
+            word |= (__float_as_uint(k) & 0xffu) << (8 * i);
+        }
+    } else {
+        // boundaries lie half way between numbers of 3 fraction bits (from 2^-6 on)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            near |= fabsf(t[i]) < 0.015626f || ((__float_as_uint(t[i]) - 0x7fff8u) & 0xfffffu) < 16u;
+        word = encode8x4<CODE>(t[0], t[1], t[2], t[3]);
+    }
+    if (near) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t[i] = s == 0.0f || x[i] != x[i] ? 0.0f : __fdiv_rn(x[i], s);
+        word = encode8x4<CODE>(t[0], t[1], t[2], t[3]);
+    }
+    return word;
+}
+
 template <typename T, int CODE, int D, int TB>
 __global__ void __launch_bounds__(APPEND_THREADS) kv8_append_kernel(const AppendParams p) {
     __shared__ float part[APPEND_THREADS / 32];
@@ -64,9 +97,9 @@ __global__ void __launch_bounds__(APPEND_THREADS) kv8_append_kernel(const Append
     const int t0 = blk * TB;                              // first token of the block
     const int first = max(t0, q.past), last = min(t0 + TB, q.past + q.n);   // new tokens [first, last)
     if (first >= last) return;
-    const T *x = static_cast<const T *>(p.x[which]) + (int64_t)(q.r0 + first - q.past) * p.ld + (int64_t)head * D;
-    uint8_t *codes = p.codes[which] + s * p.seq_stride + ((int64_t)head * p.max_seq + t0) * D;
-    float *scale = p.scales[which] + s * p.scale_seq_stride + (int64_t)head * p.nblk + blk;
+    const T *x = static_cast<const T *>(which ? p.x[1] : p.x[0]) + (int64_t)(q.r0 + first - q.past) * p.ld + (int64_t)head * D;
+    uint8_t *codes = (which ? p.codes[1] : p.codes[0]) + s * p.seq_stride + ((int64_t)head * p.max_seq + t0) * D;
+    float *scale = (which ? p.scales[1] : p.scales[0]) + s * p.scale_seq_stride + (int64_t)head * p.nblk + blk;
     const int held = first - t0, fresh = last - first;
 
     // four elements a thread and round, all of the block's rounds in flight (a whole block of 128
@@ -124,6 +157,7 @@ __global__ void __launch_bounds__(APPEND_THREADS) kv8_append_kernel(const Append
             *reinterpret_cast<uint32_t *>(codes + e) = encode8x4<CODE>(u[0], u[1], u[2], u[3]);
         }
     codes += held * D;
+    const float recip = __fdiv_rn(1.0f, now);
     const bool once = total <= 4 * APPEND_THREADS * R;       // the values are still here
     for (int e0 = 4 * threadIdx.x; e0 < total; e0 += 4 * APPEND_THREADS * R) {
         if (!once) {
@@ -135,10 +169,7 @@ __global__ void __launch_bounds__(APPEND_THREADS) kv8_append_kernel(const Append
         for (int r = 0; r < R; ++r) {
             const int e = e0 + 4 * APPEND_THREADS * r;
             if (e >= total) continue;
-            float u[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) u[i] = now == 0.0f || v[r][i] != v[r][i] ? 0.0f : __fdiv_rn(v[r][i], now);
-            *reinterpret_cast<uint32_t *>(codes + e) = encode8x4<CODE>(u[0], u[1], u[2], u[3]);
+            *reinterpret_cast<uint32_t *>(codes + e) = encode_quotients<CODE>(v[r], now, recip, now >= 1e-30f);
         }
     }
 }
