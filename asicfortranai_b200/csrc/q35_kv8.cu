@@ -30,6 +30,7 @@
 // 16 bytes of each of four keys serve 16 column tiles of P V (the order of the output
 // columns is free), so every load is a 16-byte register load and there is no transpose.
 #include <algorithm>
+#include <cfloat>
 #include <cstring>
 #include <type_traits>
 
@@ -301,7 +302,9 @@ __global__ void __launch_bounds__(ATT_THREADS, AttnShape<D>::CTAS) kv8_attn_kern
     for (int t = 0; t < VT; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[t][i] = 0.0f;
-    float vref = 0.0f, vinv = 0.0f;             // largest v scale so far and its reciprocal
+    // largest v scale that each of the two rows has seen and its reciprocal (a later row's would cost
+    // an earlier one bits of its weights); the smallest normal number stands for less
+    float vref[2] = {FLT_MIN, FLT_MIN}, vinv[2] = {1.0f / FLT_MIN, 1.0f / FLT_MIN};
 
     constexpr int KL = D / 64;                  // 16-byte loads per key and lane: 1, 2, 4
     uint4 kr[NT][KL];                           // K codes of a step: key 8t + g, bytes 64 j + 16 c ..
@@ -391,12 +394,15 @@ __global__ void __launch_bounds__(ATT_THREADS, AttnShape<D>::CTAS) kv8_attn_kern
                     if (TERMS == 2) mma16816(s[t], ql, b0, b1);
                 }
             }
-        float ksc[NT / 2], vsc[NT / 2], vtop = vref;
+        float ksc[NT / 2], vsc[NT / 2][2], vtop[2] = {vref[0], vref[1]};
 #pragma unroll
         for (int u = 0; u < NT / 2; ++u) {
             ksc[u] = nks[u];
-            vsc[u] = nvs[u];
-            vtop = fmaxf(vtop, vsc[u]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                vsc[u][h] = kk + 16 * u < min(lim[h], k1) ? nvs[u] : 0.0f;
+                vtop[h] = fmaxf(vtop[h], vsc[u][h]);
+            }
         }
         if (nk < k1) { load_k(nk); load_scales(nk); }
         float mx[2] = {m[0], m[1]};
@@ -423,12 +429,15 @@ __global__ void __launch_bounds__(ATT_THREADS, AttnShape<D>::CTAS) kv8_attn_kern
             mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
         }
         // the outputs so far move to the new maximum and the new reference v scale
-        if (vtop > vref) vinv = 1.0f / vtop;
-        const float vdown = vtop > vref ? vref * vinv : 1.0f;
-        vref = vtop;
         float mu[2], down[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+            float vdown = 1.0f;
+            if (vtop[h] > vref[h]) {
+                vinv[h] = 1.0f / vtop[h];
+                vdown = vref[h] * vinv[h];
+                vref[h] = vtop[h];
+            }
             mu[h] = mx[h] == -INFINITY ? 0.0f : mx[h];     // a row that has seen no key yet
             down[h] = ex2(m[h] - mu[h]);
             l[h] *= down[h];
@@ -453,11 +462,11 @@ __global__ void __launch_bounds__(ATT_THREADS, AttnShape<D>::CTAS) kv8_attn_kern
         if (kk + KC > k1) clear_v(kk);
 #pragma unroll
         for (int u = 0; u < NT / 2; ++u) {
-            const float w = vsc[u] == vref ? 1.0f : vsc[u] * vinv;
+            const float w[2] = {vsc[u][0] == vref[0] ? 1.0f : vsc[u][0] * vinv[0], vsc[u][1] == vref[1] ? 1.0f : vsc[u][1] * vinv[1]};
             uint4 pa, pl;
             float x[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) { x[i] = s[2 * u][i] * w; x[4 + i] = s[2 * u + 1][i] * w; }
+            for (int i = 0; i < 4; ++i) { x[i] = s[2 * u][i] * w[i >> 1]; x[4 + i] = s[2 * u + 1][i] * w[i >> 1]; }
             pa = make_uint4(pack2<__half>(x[0], x[1]), pack2<__half>(x[2], x[3]), pack2<__half>(x[4], x[5]),
                             pack2<__half>(x[6], x[7]));
             if (TERMS == 2) {
@@ -513,7 +522,7 @@ __global__ void __launch_bounds__(ATT_THREADS, AttnShape<D>::CTAS) kv8_attn_kern
         for (int i = 0; i < 4; ++i) {
             const int n = 2 * c + (i & 1);      // column tile t, column n: see load_v
             const int d = D == 64 ? n * 8 + t : (t / 16) * 128 + n * 16 + t % 16;
-            mg[(warp * ATT_M + g + 8 * (i >> 1)) * RO + d] = o[t][i] * vref;
+            mg[(warp * ATT_M + g + 8 * (i >> 1)) * RO + d] = o[t][i] * vref[i >> 1];
         }
     __syncthreads();
     for (int r = warp; r < fn; r += ATT_WARPS) {
@@ -688,7 +697,9 @@ __global__ void __launch_bounds__(ATT_THREADS, D == 256 ? 1 : 2) kv8_attn8_kerne
     for (int t = 0; t < OT; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[t][i] = 0.0f;
-    float vref = 0.0f, vinv = 0.0f;             // largest v scale so far and its reciprocal
+    // largest v scale that each of the two rows has seen and its reciprocal (a later row's would cost
+    // an earlier one bits of its weights); the smallest normal number stands for less
+    float vref[2] = {FLT_MIN, FLT_MIN}, vinv[2] = {1.0f / FLT_MIN, 1.0f / FLT_MIN};
 
     for (; kk < k1; kk += ATT_WARPS * KC) {
         const int nk = kk + ATT_WARPS * KC;
@@ -719,12 +730,15 @@ __global__ void __launch_bounds__(ATT_THREADS, D == 256 ? 1 : 2) kv8_attn8_kerne
                     if (TERMS == 2) mma16816(s[u], a, q2, q3);
                 }
             }
-        float ksc[U], vsc[U], vtop = vref;
+        float ksc[U], vsc[U][2], vtop[2] = {vref[0], vref[1]};
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             ksc[u] = nks[u];
-            vsc[u] = nvs[u];
-            if (kk + 16 * u < k1) vtop = fmaxf(vtop, vsc[u]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                vsc[u][h] = kk + 16 * u < min(lim[h], k1) ? nvs[u] : 0.0f;
+                vtop[h] = fmaxf(vtop[h], vsc[u][h]);
+            }
         }
         if (nk < k1) load_k(nk);
         float mx[2] = {-INFINITY, -INFINITY};
@@ -746,13 +760,16 @@ __global__ void __launch_bounds__(ATT_THREADS, D == 256 ? 1 : 2) kv8_attn8_kerne
 #pragma unroll
             for (int i = 0; i < 4; ++i) mx[i & 1] = fmaxf(mx[i & 1], s[u][i]);
         // a larger score or v scale than before: the outputs so far move to the new references
-        if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1] || vtop > vref)) {
-            if (vtop > vref) vinv = 1.0f / vtop;
-            const float vdown = vtop > vref ? vref * vinv : 1.0f;
-            vref = vtop;
+        if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1] || vtop[0] > vref[0] || vtop[1] > vref[1])) {
             float down[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
+                float vdown = 1.0f;
+                if (vtop[h] > vref[h]) {
+                    vinv[h] = 1.0f / vtop[h];
+                    vdown = vref[h] * vinv[h];
+                    vref[h] = vtop[h];
+                }
                 float x = fmaxf(mx[h], m[h]);
 #pragma unroll
                 for (int b = 4; b < 32; b <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, b));
@@ -782,14 +799,14 @@ __global__ void __launch_bounds__(ATT_THREADS, D == 256 ? 1 : 2) kv8_attn8_kerne
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const float w = kk + 16 * u >= k1 ? 0.0f : vsc[u] == vref ? 1.0f : vsc[u] * vinv;
+            const float w[2] = {vsc[u][0] == vref[0] ? 1.0f : vsc[u][0] * vinv[0], vsc[u][1] == vref[1] ? 1.0f : vsc[u][1] * vinv[1]};
             float x[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float mu = m[i & 1] == -INFINITY ? 0.0f : m[i & 1];     // a row that has seen no key yet
                 const float e = ex2(s[u][i] - mu);
                 l[i & 1] += e;
-                x[i] = e * w;
+                x[i] = e * w[i & 1];
             }
             const uint32_t h0 = pack2<__half>(x[0], x[1]), h1 = pack2<__half>(x[2], x[3]);
             const uint32_t b0 = transpose8x8(h0), b1 = transpose8x8(h1);
@@ -831,7 +848,7 @@ __global__ void __launch_bounds__(ATT_THREADS, D == 256 ? 1 : 2) kv8_attn8_kerne
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int d = (D == 64 ? 8 * g : (t / 8) * 128 + 16 * g) + 2 * (t % 8) + (i >> 1);
-            mg[(warp * TM + 2 * c + (i & 1)) * RO + d] = o[t][i] * vref;
+            mg[(warp * TM + 2 * c + (i & 1)) * RO + d] = o[t][i] * vref[i & 1];
         }
     __syncthreads();
     if (warp < fn) {

@@ -18,6 +18,7 @@
 // long as the MMAs) and the softmax's other 6 instructions a score bound it.
 //
 // Waits are bounded as in q35_fp8.cu.
+#include <cfloat>
 #include <type_traits>
 
 #include "q35_kv8.cuh"
@@ -188,7 +189,9 @@ __global__ void __launch_bounds__(PT_THREADS, 2) kv8_prompt_kernel(const AttnPar
         const int all_see = fn > 0 ? sr.past + f0 / p.G + 1 : 0;       // keys below this: every row sees them
         const uint32_t lanes = (uint32_t)(32 * warp) << 16;
         float m = -INFINITY, l = 0.0f;            // reference of the weights, their sum
-        float vref = 0.0f, vinv = 0.0f;           // largest v scale so far and its reciprocal
+        // largest v scale that the row has seen and its reciprocal (a later row's would cost an earlier
+        // one bits of its weights); the smallest normal number stands for less
+        float vref = FLT_MIN, vinv = 1.0f / FLT_MIN;
         for (int j = 0; j < steps && ok; ++j) {
             const int b = j & 1, kk = j * PT_KEYS;
             const uint32_t ph = (uint32_t)((j >> 1) & 1);
@@ -200,12 +203,17 @@ __global__ void __launch_bounds__(PT_THREADS, 2) kv8_prompt_kernel(const AttnPar
             const float4 v4 = *reinterpret_cast<const float4 *>(scales + 8 * (j & 3) + 4);
             // (never 0: a masked score times 0 would be NaN)
             const float ks[4] = {fmaxf(k4.x * qs, 1e-37f), fmaxf(k4.y * qs, 1e-37f), fmaxf(k4.z * qs, 1e-37f), fmaxf(k4.w * qs, 1e-37f)};
-            const float vs[4] = {v4.x, v4.y, v4.z, v4.w};
+            const bool edge = kk + PT_KEYS > all_see;                  // some row does not see some key
+            float vs[4] = {v4.x, v4.y, v4.z, v4.w};
+            if (edge) {
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (kk + 16 * u >= lim) vs[u] = 0.0f;
+            }
             const float vtop = fmaxf(fmaxf(vref, fmaxf(vs[0], vs[1])), fmaxf(vs[2], vs[3]));
             tc_fence_after();
             // the scores are read twice, 32 at a time: for the maximum, then for the weights (all 64 with
             // their weights would not fit the registers of two CTAs an SM)
-            const bool edge = kk + PT_KEYS > all_see;                  // some row does not see some key
             float mx = -INFINITY;
 #pragma unroll
             for (int hh = 0; hh < 2; ++hh) {
@@ -226,7 +234,7 @@ __global__ void __launch_bounds__(PT_THREADS, 2) kv8_prompt_kernel(const AttnPar
                 }
             }
             // O moves to new references only where a row's maximum has passed its own by 2^8, or for
-            // a larger v scale (the same in every thread)
+            // a larger v scale
             if (__any_sync(0xffffffffu, mx > m + PT_SLACK || vtop > vref)) {
                 if (vtop > vref) vinv = 1.0f / vtop;
                 const float vdown = vtop > vref ? vref * vinv : 1.0f;
@@ -287,24 +295,27 @@ __global__ void __launch_bounds__(PT_THREADS, 2) kv8_prompt_kernel(const AttnPar
             const int b = (steps - 1) & 1;
             if (!__all_sync(0xffffffffu, mbar_wait(pv_done(b), (uint32_t)(((steps - 1) >> 1) & 1), abort_flag))) fail();
             tc_fence_after();
-            const float inv = vref / l;
+            const float inv = 1.0f / l;
             T *dst = static_cast<T *>(p.out) + row * p.ldo + (int64_t)head * D;
             const bool vec = (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
 #pragma unroll 1
             for (int d = 0; d < D && ok; d += 32) {
                 float o[32];
+                __syncwarp();
                 tc_ld32(tmem + lanes + 128u + (uint32_t)d, o);
                 tc_wait_ld(o);
                 if (!live) continue;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = o[i] * inv * vref;
                 if (vec) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 8)
                         *reinterpret_cast<uint4 *>(dst + d + i) =
-                            make_uint4(pack2<T>(o[i] * inv, o[i + 1] * inv), pack2<T>(o[i + 2] * inv, o[i + 3] * inv),
-                                       pack2<T>(o[i + 4] * inv, o[i + 5] * inv), pack2<T>(o[i + 6] * inv, o[i + 7] * inv));
+                            make_uint4(pack2<T>(o[i], o[i + 1]), pack2<T>(o[i + 2], o[i + 3]), pack2<T>(o[i + 4], o[i + 5]),
+                                       pack2<T>(o[i + 6], o[i + 7]));
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) dst[d + i] = from_f32<T>(o[i] * inv);
+                    for (int i = 0; i < 32; ++i) dst[d + i] = from_f32<T>(o[i]);
                 }
             }
         }
