@@ -5,8 +5,8 @@
 //   scales k_scale, v_scale [seq][kv_head][ceil(max_seq / block)], block of 16..128 tokens
 //
 // Append.  Tokens that join a block can be larger than the ones it holds, so the block's
-// scale is s' = max(s, max |new| / Q) (s = 0 for a block without older tokens); where it
-// grew, the older codes become the codes nearest to (code * s) / s'.  One CTA per (block,
+// scale is s' = max(s, max |new| (1/Q)) (s = 0 for a block without older tokens, 1/Q and the
+// product rounded to binary32); where it grew, the older codes become the codes nearest to (code * s) / s'.  One CTA per (block,
 // head, k or v): it alone reads and writes the block, so nothing races.  Non-finite input
 // does not enter the maximum; infinities are stored as +-Q, NaN as 0.
 //
@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(APPEND_THREADS) kv8_append_kernel(const Append
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < APPEND_THREADS / 32; ++w) amax = fmaxf(amax, part[w]);
-    const float now = fmaxf(old, __fdiv_rn(amax, code_max<CODE>()));
+    const float now = fmaxf(old, __fmul_rn(amax, 1.0f / code_max<CODE>()));
     if (threadIdx.x == 0) *scale = now;
     if (held && now != old)
         for (int e = 4 * threadIdx.x; e < held * D; e += 4 * APPEND_THREADS) {

@@ -289,10 +289,10 @@ typedef struct {
  * left out and recorded (Q35_ERR_INVALID from q35_ctx_device_error).
  *
  * Appends k and v (dtype, [rows] of kv_heads * head_dim elements, ld apart).  A block's scale
- * becomes max(scale, max |new| / (127 or 448)), counting from 0 for a block without older
- * tokens; where it grew the block's older codes are rounded again.  Infinities are stored as
- * the largest code, NaN as 0.  q35_kv8_append_dev neither reads nor writes anything behind a
- * sequence's last token but the scale of its last block. */
+ * becomes max(scale, max |new| * (1/127 or 1/448)) in binary32, counting from 0 for a block
+ * without older tokens; where it grew the block's older codes are rounded again.  Infinities
+ * are stored as the largest code, NaN as 0.  q35_kv8_append_dev neither reads nor writes
+ * anything behind a sequence's last token but the scale of its last block. */
 int q35_kv8_append_dev(q35_ctx ctx, const q35_kv8_cache *cache, int dtype, const void *k, const void *v,
                        int64_t ld, const int32_t *row_start, const int32_t *past, int32_t rows,
                        int32_t max_rows);

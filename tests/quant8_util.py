@@ -43,7 +43,7 @@ def append_ref(codes, scale, new, past, block, code):
         fin = np.abs(x[np.isfinite(x)])
         amax = fin.max() if fin.size else F(0)
         old = scale[b] if first > t0 else F(0)
-        now = max(old, F(amax / QMAX[code]))
+        now = max(old, F(amax * F(1 / QMAX[code])))
         if first > t0 and now != old:
             v = (decode(codes[t0:first], code).astype(F) * old).astype(F)
             with np.errstate(over="ignore", invalid="ignore"):
