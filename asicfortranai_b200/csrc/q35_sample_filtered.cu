@@ -28,7 +28,9 @@
 // the cut are loaded from the other CTAs, by one warp.
 //
 // Bound by the exponentials (15 binary64 operations and about as many integer ones an entry)
-// where nothing cuts the vocabulary first, and by barrier latency for one row.
+// where nothing cuts the vocabulary first, and by barrier latency for one row.  Measured: 64 rows
+// of 100,277 62 us (26 MB, 4 us of HBM; of a top-p row's 97 k clocks 23 k are exponentials, 22 k
+// the histogram of masses, 9 k each loading and dropping), one row of 32,000 14 us.
 #include <cfloat>
 
 #include "q35_q8.cuh"
