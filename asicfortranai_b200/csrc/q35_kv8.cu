@@ -24,7 +24,7 @@
 // MB, 4.1 TB/s); one token after 2000 12 to 18 us, three launches.  The append of 2048 tokens of
 // 40 heads 36 us (64 MB): its issue slots are 62 % busy.
 //
-// Prompts of 16-bit queries take 128-row tiles on tcgen05 instead (q35_kv8_prompt.cu).
+// Prompts take 128-row tiles on tcgen05 instead (q35_kv8_prompt.cu).
 //
 // Single tokens are bound by HBM in the end and by instructions on the way (two conversions a
 // pair of codes); their form takes K and V^T as the 16-row operand, so that half the MMAs and half
@@ -1100,7 +1100,7 @@ int launch_kv8_attention(const q35_kv8_cache &c, int dtype, const void *q, int64
                          int64_t ldo, int8_t *out_q, const Kv8Rows &r, float scale, void *workspace, int *err,
                          cudaStream_t s) {
     if (r.rows == 0) return Q35_OK;
-    const bool prompt = !out_q && kv8_prompt_takes(c, dtype, heads, r.max_rows);
+    const bool prompt = kv8_prompt_takes(c, heads, r.max_rows);
     const AttnPlan pl = attn_plan(c, heads, r.max_rows);
     if (pl.mtiles > 65535) return set_error(Q35_ERR_INVALID, "kv8: too many rows in one call");
     AttnParams p;

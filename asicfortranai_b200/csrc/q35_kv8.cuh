@@ -41,9 +41,8 @@ struct AttnParams {
     int *err;
 };
 
-// (row, head) pairs from which on a sequence's rows take the prompt kernel
-constexpr int PROMPT_PAIRS = 64;
-bool kv8_prompt_takes(const q35_kv8_cache &c, int dtype, int32_t heads, int32_t max_rows);
+// whether rows of this number take the prompt kernel
+bool kv8_prompt_takes(const q35_kv8_cache &c, int32_t heads, int32_t max_rows);
 int launch_kv8_prompt(const AttnParams &p, int dtype, int code, int D, int zs, cudaStream_t s);
 
 #ifdef __CUDACC__

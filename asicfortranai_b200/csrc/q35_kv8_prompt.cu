@@ -1,9 +1,8 @@
 // q35_kv8_prompt.cu -- causal attention of many rows over the 8-bit KV cache on the 5th-generation
-// tensor cores (16-bit queries, head_dim 64 or 128); q35_kv8.cu has the definition, the cache and
-// the other forms.
+// tensor cores; q35_kv8.cu has the definition, the cache and the other forms.
 //
-// One CTA per tile of 128 (row, head) pairs of a sequence and kv head, two CTAs per SM (one's
-// softmax under the other's MMAs).  Per 64 keys:
+// One CTA per tile of 128 (row, head) pairs of a sequence and kv head, two CTAs per SM where the
+// memory takes them (one's softmax under the other's MMAs).  Per 64 keys:
 //   * converters: warps 4, 5 turn K's codes into fp16 (exact) in shared memory, keys as rows; warps
 //     6, 7 V's, transposed on the way (a thread's 8 keys x 16 d become 16 rows of 8 keys), so both
 //     MMA operands are K-major with the 128-byte swizzle;
@@ -14,8 +13,12 @@
 //     only when that has grown by 2^8 (weights stay below 2^8, fp16 holds them with 11 bits), so
 //     O is rarely moved; weights times the block's v scale over the largest one so far go back
 //     as fp16 into S's buffer.
-// Sums and O are fp32.  The exponentials (16 a clock and SM: 512 clocks for a tile's 64 keys, as
-// long as the MMAs) and the softmax's other 6 instructions a score bound it.
+// fp32 queries and their weights take two fp16 terms each (22 bits), with two MMAs for one.
+//
+// Sums and O are fp32.  Measured, 2048 rows of 40 heads of 128 over 2001 older tokens, bf16: 276 us
+// (of 75 for the operations at the fp16 rate), f32 about 400.  A CTA's step of 64 keys takes 3300
+// clocks, of which a softmax warp works 2000 (1500 of them on the weights: 16 exponentials a clock
+// and SM alone are 512 for each of the SM's two CTAs) and the tensor pipe is busy for 640.
 //
 // Waits are bounded as in q35_fp8.cu.
 #include <cfloat>
@@ -32,9 +35,15 @@ constexpr int PT_KEYS = 64;                // keys per step
 constexpr int PT_THREADS = 288;
 constexpr float PT_SLACK = 8.0f;           // log2 by which a row's maximum may pass its reference
 
-template <int D> struct Prompt {
-    static constexpr uint32_t Q = PT_ROWS * D * 2, K = PT_KEYS * D * 2, V = D * PT_KEYS * 2;
-    static constexpr uint32_t off_k = Q, off_v = Q + 2 * K, off_bar = Q + 2 * K + 2 * V;
+constexpr float PT_BOOST = 128.0f;         // factor of the weights in fp16: 2^8 2^7 is in its range, and 2^-31 not 0
+
+// TERMS: fp16 terms of a query element and of a weight (2 for fp32 queries: 22 bits)
+template <int TERMS, int D> struct Prompt {
+    static constexpr uint32_t Q = PT_ROWS * D * 2, K = PT_KEYS * D * 2, V = D * PT_KEYS * 2;   // Q: one term
+    static constexpr int stages = TERMS * D > 256 ? 1 : 2;             // of K and V: what the memory takes
+    static constexpr int ctas = TERMS * D > 128 ? 1 : 2;               // per SM
+    static constexpr uint32_t tmem = D > 128 ? 512 : 256;              // columns: S 2 x 64, O
+    static constexpr uint32_t off_k = TERMS * Q, off_v = off_k + stages * K, off_bar = off_v + stages * V;
     static constexpr size_t smem = 1024 + off_bar + 8 * 18 + 16 + 4 * 32;
 };
 
@@ -83,9 +92,11 @@ __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.
 __device__ __forceinline__ uint32_t swz(int row, int chunk) { return (uint32_t)(row * 128 + ((chunk ^ (row & 7)) << 4)); }
 
 template <typename T, int CODE, int D>
-__global__ void __launch_bounds__(PT_THREADS, 2) kv8_prompt_kernel(const AttnParams p) {
-    using L = Prompt<D>;
-    constexpr int DB = D / 64;                 // 64-element blocks of a row of Q and K
+__global__ void __launch_bounds__(PT_THREADS, (Prompt<std::is_same<T, float>::value ? 2 : 1, D>::ctas))
+kv8_prompt_kernel(const AttnParams p) {
+    constexpr int TERMS = std::is_same<T, float>::value ? 2 : 1;
+    using L = Prompt<TERMS, D>;
+    constexpr int ST = L::stages;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     uint8_t *sbase = smem_raw + (base - raw);
@@ -117,7 +128,7 @@ __global__ void __launch_bounds__(PT_THREADS, 2) kv8_prompt_kernel(const AttnPar
     }
     if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-                     ::"r"(smem_u32((const void *)tmem_slot)), "r"(256u) : "memory");
+                     ::"r"(smem_u32((const void *)tmem_slot)), "r"(L::tmem) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     tc_fence_before();
@@ -155,15 +166,23 @@ __global__ void __launch_bounds__(PT_THREADS, 2) kv8_prompt_kernel(const AttnPar
         float qs = 0.0f;
         if (steps > 0) {
             const T *src = static_cast<const T *>(p.q) + row * p.ldq + (int64_t)head * D;
+            const bool vec = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
+            auto load8 = [&](int d, T (&x)[8]) {
+                if (vec) {
+#pragma unroll
+                    for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+                        reinterpret_cast<uint4 *>(x)[i] = reinterpret_cast<const uint4 *>(src + d)[i];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[i] = src[d + i];
+                }
+            };
             float a = 0.0f;
             if (live) {
-                const bool vec = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
 #pragma unroll 4
                 for (int d = 0; d < D; d += 8) {
                     __align__(16) T x[8];
-                    if (vec) *reinterpret_cast<uint4 *>(x) = *reinterpret_cast<const uint4 *>(src + d);
-                    else
-                        for (int i = 0; i < 8; ++i) x[i] = src[d + i];
+                    load8(d, x);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) a = fmaxf(a, fabsf(to_f32<T>(x[i])));
                 }
@@ -173,13 +192,23 @@ __global__ void __launch_bounds__(PT_THREADS, 2) kv8_prompt_kernel(const AttnPar
             const int e = min(126, 13 - ((int)(__float_as_uint(a) >> 23) - 127));
             const float up = copysignf(a > 0.0f ? __uint_as_float((uint32_t)(e + 127) << 23) : 1.0f, p.scale);
             qs = fabsf(p.scale) * 1.4426950408889634f * (a > 0.0f ? __uint_as_float((uint32_t)(127 - e) << 23) : 1.0f);
-#pragma unroll 4
+#pragma unroll 2
             for (int d = 0; d < D; d += 8) {
-                uint32_t w[4];
+                __align__(16) T x[8];
+                uint32_t w[4], lo[4] = {0u, 0u, 0u, 0u};
+                if (live) load8(d, x);
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    w[i] = live ? pack2<__half>(to_f32<T>(src[d + 2 * i]) * up, to_f32<T>(src[d + 2 * i + 1]) * up) : 0u;
-                st_shared16(base + (uint32_t)(d / 64) * (PT_ROWS * 128) + swz(r, (d % 64) / 8), make_uint4(w[0], w[1], w[2], w[3]));
+                for (int i = 0; i < 4; ++i) {
+                    const float y0 = to_f32<T>(x[2 * i]) * up, y1 = to_f32<T>(x[2 * i + 1]) * up;
+                    w[i] = live ? pack2<__half>(y0, y1) : 0u;
+                    if (TERMS == 2 && live) {
+                        const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+                        lo[i] = pack2<__half>(y0 - h.x, y1 - h.y);
+                    }
+                }
+                const uint32_t at = base + (uint32_t)(d / 64) * (PT_ROWS * 128) + swz(r, (d % 64) / 8);
+                st_shared16(at, make_uint4(w[0], w[1], w[2], w[3]));
+                if (TERMS == 2) st_shared16(at + L::Q, make_uint4(lo[0], lo[1], lo[2], lo[3]));
             }
             fence_async();
             __syncwarp();
@@ -190,8 +219,8 @@ __global__ void __launch_bounds__(PT_THREADS, 2) kv8_prompt_kernel(const AttnPar
         const uint32_t lanes = (uint32_t)(32 * warp) << 16;
         float m = -INFINITY, l = 0.0f;            // reference of the weights, their sum
         // largest v scale that the row has seen and its reciprocal (a later row's would cost an earlier
-        // one bits of its weights); the smallest normal number stands for less
-        float vref = FLT_MIN, vinv = 1.0f / FLT_MIN;
+        // one bits of its weights); 2^-119 stands for less
+        float vref = PT_BOOST * FLT_MIN, vinv = 1.0f / FLT_MIN;        // (the reciprocal times PT_BOOST)
         for (int j = 0; j < steps && ok; ++j) {
             const int b = j & 1, kk = j * PT_KEYS;
             const uint32_t ph = (uint32_t)((j >> 1) & 1);
@@ -236,8 +265,8 @@ __global__ void __launch_bounds__(PT_THREADS, 2) kv8_prompt_kernel(const AttnPar
             // O moves to new references only where a row's maximum has passed its own by 2^8, or for
             // a larger v scale
             if (__any_sync(0xffffffffu, mx > m + PT_SLACK || vtop > vref)) {
-                if (vtop > vref) vinv = 1.0f / vtop;
-                const float vdown = vtop > vref ? vref * vinv : 1.0f;
+                if (vtop > vref) vinv = PT_BOOST / vtop;
+                const float vdown = vtop > vref ? vref * vinv * (1.0f / PT_BOOST) : 1.0f;
                 vref = vtop;
                 const float to = mx > m + PT_SLACK ? mx : m;
                 float down = to == -INFINITY ? 1.0f : ex2(m - to);
@@ -263,9 +292,10 @@ __global__ void __launch_bounds__(PT_THREADS, 2) kv8_prompt_kernel(const AttnPar
             const float mu = m == -INFINITY ? 0.0f : m;                // a row that has seen no key yet
 #pragma unroll
             for (int hh = 0; hh < 2; ++hh) {
-                // (the weights of the first half take the place of its own scores, the second's too)
+                // (the weights of the first half take the place of its own scores, the second's too: 16
+                // columns of high terms, then 16 of low ones)
                 float s[32];
-                uint32_t pk[16];
+                uint32_t pk[16], pl[TERMS == 2 ? 16 : 1];
                 tc_ld32(tmem + lanes + (uint32_t)(64 * b + 32 * hh), s);
                 tc_wait_ld(s);
                 if (edge) {
@@ -276,15 +306,20 @@ __global__ void __launch_bounds__(PT_THREADS, 2) kv8_prompt_kernel(const AttnPar
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     const float c = ks[2 * hh + u], v = vs[2 * hh + u];
-                    const float w = v == vref ? 1.0f : v * vinv;
+                    const float w = v == vref ? PT_BOOST : v * vinv;
 #pragma unroll
                     for (int i = 16 * u; i < 16 * u + 16; i += 2) {
                         const float e0 = ex2(fmaf(s[i], c, -mu)), e1 = ex2(fmaf(s[i + 1], c, -mu));
                         l += e0 + e1;
                         pk[i / 2] = pack2<__half>(e0 * w, e1 * w);
+                        if constexpr (TERMS == 2) {
+                            const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&pk[i / 2]));
+                            pl[i / 2] = pack2<__half>(fmaf(e0, w, -h.x), fmaf(e1, w, -h.y));
+                        }
                     }
                 }
-                tc_st16(tmem + lanes + (uint32_t)(64 * b + 16 * hh), pk);
+                tc_st16(tmem + lanes + (uint32_t)(64 * b + 32 * hh), pk);
+                if constexpr (TERMS == 2) tc_st16(tmem + lanes + (uint32_t)(64 * b + 32 * hh + 16), pl);
             }
             tc_wait_st();
             tc_fence_before();
@@ -295,7 +330,7 @@ __global__ void __launch_bounds__(PT_THREADS, 2) kv8_prompt_kernel(const AttnPar
             const int b = (steps - 1) & 1;
             if (!__all_sync(0xffffffffu, mbar_wait(pv_done(b), (uint32_t)(((steps - 1) >> 1) & 1), abort_flag))) fail();
             tc_fence_after();
-            const float inv = 1.0f / l;
+            const float inv = 1.0f / (l * PT_BOOST);
             T *dst = static_cast<T *>(p.out) + row * p.ldo + (int64_t)head * D;
             const bool vec = (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
 #pragma unroll 1
@@ -307,12 +342,26 @@ __global__ void __launch_bounds__(PT_THREADS, 2) kv8_prompt_kernel(const AttnPar
                 if (!live) continue;
 #pragma unroll
                 for (int i = 0; i < 32; ++i) o[i] = o[i] * inv * vref;
-                if (vec) {
+                if (p.out_q) {
+                    uint32_t c[8];
 #pragma unroll
-                    for (int i = 0; i < 32; i += 8)
-                        *reinterpret_cast<uint4 *>(dst + d + i) =
-                            make_uint4(pack2<T>(o[i], o[i + 1]), pack2<T>(o[i + 2], o[i + 3]), pack2<T>(o[i + 4], o[i + 5]),
-                                       pack2<T>(o[i + 6], o[i + 7]));
+                    for (int i = 0; i < 8; ++i)
+                        c[i] = (uint32_t)(uint8_t)quant127(o[4 * i]) | (uint32_t)(uint8_t)quant127(o[4 * i + 1]) << 8 |
+                               (uint32_t)(uint8_t)quant127(o[4 * i + 2]) << 16 | (uint32_t)(uint8_t)quant127(o[4 * i + 3]) << 24;
+                    uint4 *dq = reinterpret_cast<uint4 *>(p.out_q + (row * p.H + head) * D + d);
+                    dq[0] = make_uint4(c[0], c[1], c[2], c[3]);
+                    dq[1] = make_uint4(c[4], c[5], c[6], c[7]);
+                } else if (vec) {
+                    if constexpr (TERMS == 2) {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4 *>(dst + d + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8)
+                            *reinterpret_cast<uint4 *>(dst + d + i) =
+                                make_uint4(pack2<T>(o[i], o[i + 1]), pack2<T>(o[i + 2], o[i + 3]), pack2<T>(o[i + 4], o[i + 5]),
+                                           pack2<T>(o[i + 6], o[i + 7]));
+                    }
                 } else {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) dst[d + i] = from_f32<T>(o[i]);
@@ -340,11 +389,11 @@ __global__ void __launch_bounds__(PT_THREADS, 2) kv8_prompt_kernel(const AttnPar
         };
         if (steps > 0) { load(0); load_scale(0); }
         for (int j = 0; j < steps && ok; ++j) {
-            const int b = j & 1;
-            if (!__all_sync(0xffffffffu, mbar_wait(k_empty(b), (uint32_t)((j >> 1) & 1) ^ 1u, abort_flag))) { fail(); break; }
+            const int b = j % ST;
+            if (!__all_sync(0xffffffffu, mbar_wait(k_empty(b), (uint32_t)((j / ST) & 1) ^ 1u, abort_flag))) { fail(); break; }
             const uint32_t dst = base + L::off_k + (uint32_t)b * L::K;
             const uint32_t blk = dst + (uint32_t)(ch / 4) * (PT_KEYS * 128);
-            const int odd = ch / 4;                                  // (the two 64-d blocks' lanes write the
+            const int odd = (ch / 4) & 1;                            // (neighbouring 64-d blocks' lanes write the
 #pragma unroll                                                       // halves in opposite order: no bank conflicts)
             for (int i = 0; i < LK; ++i) {
                 uint4 x, y;
@@ -367,41 +416,50 @@ __global__ void __launch_bounds__(PT_THREADS, 2) kv8_prompt_kernel(const AttnPar
         }
     } else if (warp < 8) {
         // ---------------- V: fp16, transposed ----------------
-        const int t = tid - 192, kg = t & 7, dg = t >> 3;            // keys 8 kg .., d 16 dg .. (8 groups at D = 128)
-        const uint8_t *vb = p.v + hb + 16 * dg;
-        uint4 c[8];
-        const bool live = dg < D / 16;
+        constexpr int VG = D > 128 ? D / 128 : 1;                    // pieces of 16 d x 8 keys a thread
+        const int t = tid - 192, kg = t & 7, dg0 = t >> 3;           // keys 8 kg .., d 16 dg .. (8 groups, D / 16 in all)
+        const uint8_t *vb = p.v + hb + 16 * dg0;
+        uint4 c[VG][8];
+        const bool live = dg0 < D / 16;
         auto load = [&](int j) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) c[i] = ldg16(vb + (int64_t)min(j * PT_KEYS + 8 * kg + i, kend - 1) * D);
+            for (int g = 0; g < VG; ++g)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) c[g][i] = ldg16(vb + 128 * g + (int64_t)min(j * PT_KEYS + 8 * kg + i, kend - 1) * D);
         };
         if (steps > 0 && live) load(0);
         for (int j = 0; j < steps && ok; ++j) {
-            const int b = j & 1;
-            if (!__all_sync(0xffffffffu, mbar_wait(pv_done(b), (uint32_t)((j >> 1) & 1) ^ 1u, abort_flag))) { fail(); break; }
+            const int b = j % ST;
+            // the stage is free: P V of step j - ST
+            if (j >= ST && !__all_sync(0xffffffffu, mbar_wait(pv_done((j - ST) & 1), (uint32_t)((j - ST) >> 1) & 1u, abort_flag))) { fail(); break; }
             if (live) {
                 // past the last key: whatever is stored there must not count
                 if ((j + 1) * PT_KEYS > kend) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                        if (j * PT_KEYS + 8 * kg + i >= kend) c[i] = make_uint4(0u, 0u, 0u, 0u);
+                        if (j * PT_KEYS + 8 * kg + i >= kend) {
+#pragma unroll
+                            for (int g = 0; g < VG; ++g) c[g][i] = make_uint4(0u, 0u, 0u, 0u);
+                        }
                 }
                 const uint32_t dst = base + L::off_v + (uint32_t)b * L::V;
                 auto word = [&](const uint4 &u, int w) { return w == 0 ? u.x : w == 1 ? u.y : w == 2 ? u.z : u.w; };
 #pragma unroll
-                for (int w = 0; w < 4; ++w)
+                for (int g = 0; g < VG; ++g)
 #pragma unroll
-                    for (int hh = 0; hh < 2; ++hh) {
-                        uint4 x, y;                                   // d = 16 dg + 4 w + 2 hh, and the next
-                        const uint32_t sel = hh ? 0x7362 : 0x5140;
-                        codes_f16<CODE>(__byte_perm(word(c[0], w), word(c[1], w), sel), x.x, y.x);
-                        codes_f16<CODE>(__byte_perm(word(c[2], w), word(c[3], w), sel), x.y, y.y);
-                        codes_f16<CODE>(__byte_perm(word(c[4], w), word(c[5], w), sel), x.z, y.z);
-                        codes_f16<CODE>(__byte_perm(word(c[6], w), word(c[7], w), sel), x.w, y.w);
-                        const int d = 16 * dg + 4 * w + 2 * hh;
-                        st_shared16(dst + swz(d, kg), x);
-                        st_shared16(dst + swz(d + 1, kg), y);
-                    }
+                    for (int w = 0; w < 4; ++w)
+#pragma unroll
+                        for (int hh = 0; hh < 2; ++hh) {
+                            uint4 x, y;                               // d = 16 dg + 4 w + 2 hh, and the next
+                            const uint32_t sel = hh ? 0x7362 : 0x5140;
+                            codes_f16<CODE>(__byte_perm(word(c[g][0], w), word(c[g][1], w), sel), x.x, y.x);
+                            codes_f16<CODE>(__byte_perm(word(c[g][2], w), word(c[g][3], w), sel), x.y, y.y);
+                            codes_f16<CODE>(__byte_perm(word(c[g][4], w), word(c[g][5], w), sel), x.z, y.z);
+                            codes_f16<CODE>(__byte_perm(word(c[g][6], w), word(c[g][7], w), sel), x.w, y.w);
+                            const int d = 16 * (dg0 + 8 * g) + 4 * w + 2 * hh;
+                            st_shared16(dst + swz(d, kg), x);
+                            st_shared16(dst + swz(d + 1, kg), y);
+                        }
                 if (j + 1 < steps) load(j + 1);
             }
             fence_async();
@@ -414,31 +472,36 @@ __global__ void __launch_bounds__(PT_THREADS, 2) kv8_prompt_kernel(const AttnPar
         const uint64_t qd = smem_desc_sw128(base);
         if (!mbar_wait(q_full, 0, abort_flag)) fail();
         auto scores = [&](int j) {
-            const int b = j & 1;
-            const uint32_t ph = (uint32_t)((j >> 1) & 1);
+            const int b = j & 1, sb = j % ST;
             // the buffer's weights have been read: P V of step j - 2
-            if (!mbar_wait(k_full(b), ph, abort_flag) || (j >= 2 && !mbar_wait(pv_done(b), ph ^ 1u, abort_flag))) { fail(); return; }
+            if (!mbar_wait(k_full(sb), (uint32_t)((j / ST) & 1), abort_flag) ||
+                (j >= 2 && !mbar_wait(pv_done(b), (uint32_t)((j >> 1) & 1) ^ 1u, abort_flag))) { fail(); return; }
             tc_fence_after();
-            const uint64_t kd = smem_desc_sw128(base + L::off_k + (uint32_t)b * L::K);
+            const uint64_t kd = smem_desc_sw128(base + L::off_k + (uint32_t)sb * L::K);
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i)
-                tc_mma_f16(tmem + (uint32_t)(64 * b), qd + (uint64_t)((i / 4) * (PT_ROWS * 128 >> 4) + 2 * (i % 4)),
-                           kd + (uint64_t)((i / 4) * (PT_KEYS * 128 >> 4) + 2 * (i % 4)), is, i > 0 ? 1u : 0u);
-            tc_commit(k_empty(b));
+            for (int term = 0; term < TERMS; ++term)
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i)
+                    tc_mma_f16(tmem + (uint32_t)(64 * b), qd + (uint64_t)((term * L::Q + (i / 4) * (PT_ROWS * 128)) / 16 + 2 * (i % 4)),
+                               kd + (uint64_t)((i / 4) * (PT_KEYS * 128 >> 4) + 2 * (i % 4)), is, term > 0 || i > 0 ? 1u : 0u);
+            tc_commit(k_empty(sb));
             tc_commit(s_full(b));
         };
         if (ok) scores(0);
         for (int j = 0; j < steps && ok; ++j) {
-            const int b = j & 1;
-            const uint32_t ph = (uint32_t)((j >> 1) & 1);
+            const int b = j & 1, sb = j % ST;
             if (j + 1 < steps) scores(j + 1);
             if (!ok) break;
-            if (!mbar_wait(p_full(b), ph, abort_flag) || !mbar_wait(v_full(b), ph, abort_flag)) { fail(); break; }
+            if (!mbar_wait(p_full(b), (uint32_t)((j >> 1) & 1), abort_flag) ||
+                !mbar_wait(v_full(sb), (uint32_t)((j / ST) & 1), abort_flag)) { fail(); break; }
             tc_fence_after();
-            const uint64_t vd = smem_desc_sw128(base + L::off_v + (uint32_t)b * L::V);
+            const uint64_t vd = smem_desc_sw128(base + L::off_v + (uint32_t)sb * L::V);
 #pragma unroll
             for (int i = 0; i < PT_KEYS / 16; ++i)
-                tc_mma_f16_ts(tmem + 128u, tmem + (uint32_t)(64 * b + 8 * i), vd + (uint64_t)(2 * i), io, j > 0 || i > 0 ? 1u : 0u);
+#pragma unroll
+                for (int term = 0; term < TERMS; ++term)
+                    tc_mma_f16_ts(tmem + 128u, tmem + (uint32_t)(64 * b + 32 * (i / 2) + 16 * term + 8 * (i % 2)),
+                                  vd + (uint64_t)(2 * i), io, j > 0 || i > 0 || term > 0 ? 1u : 0u);
             tc_commit(pv_done(b));
         }
         tc_commit(drain);
@@ -450,38 +513,45 @@ __global__ void __launch_bounds__(PT_THREADS, 2) kv8_prompt_kernel(const AttnPar
     tc_fence_after();
     if (warp == 8) {
         __syncwarp();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256u) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::tmem) : "memory");
     }
 }
 
 template <typename T, int CODE, int D> int launch_prompt(const AttnParams &p, int zs, cudaStream_t s) {
+    using L = Prompt<std::is_same<T, float>::value ? 2 : 1, D>;
     auto kern = kv8_prompt_kernel<T, CODE, D>;
     static bool configured[64] = {};
     int dev = 0;
     Q35_CUDA_TRY(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !configured[dev]) {
-        Q35_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Prompt<D>::smem));
+        Q35_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::smem));
         if (dev >= 0 && dev < 64) configured[dev] = true;
     }
     const dim3 grid((unsigned)ceil_div((int64_t)p.max_rows * p.G, PT_ROWS), (unsigned)zs);
-    Q35_CUDA_TRY(launch_dependent(kern, grid, PT_THREADS, Prompt<D>::smem, s, 1, p));
+    Q35_CUDA_TRY(launch_dependent(kern, grid, PT_THREADS, L::smem, s, 1, p));
     return Q35_OK;
 }
+template <typename T, int CODE> int launch_prompt(const AttnParams &p, int D, int zs, cudaStream_t s) {
+    return D == 64 ? launch_prompt<T, CODE, 64>(p, zs, s) : D == 128 ? launch_prompt<T, CODE, 128>(p, zs, s) : launch_prompt<T, CODE, 256>(p, zs, s);
+}
 template <typename T> int launch_prompt(const AttnParams &p, int code, int D, int zs, cudaStream_t s) {
-    if (code == Q35_CODE_INT8)
-        return D == 64 ? launch_prompt<T, Q35_CODE_INT8, 64>(p, zs, s) : launch_prompt<T, Q35_CODE_INT8, 128>(p, zs, s);
-    return D == 64 ? launch_prompt<T, Q35_CODE_E4M3, 64>(p, zs, s) : launch_prompt<T, Q35_CODE_E4M3, 128>(p, zs, s);
+    return code == Q35_CODE_INT8 ? launch_prompt<T, Q35_CODE_INT8>(p, D, zs, s) : launch_prompt<T, Q35_CODE_E4M3>(p, D, zs, s);
 }
 
 }  // namespace
 
-// 16-bit queries with head_dim 64 or 128, half a tile of (row, head) pairs at least: below that the
-// 16-row form has more CTAs and no idle rows
-bool kv8_prompt_takes(const q35_kv8_cache &c, int dtype, int32_t heads, int32_t max_rows) {
-    return dtype != Q35_DT_F32 && c.head_dim <= 128 && (int64_t)max_rows * (heads / c.kv_heads) >= PROMPT_PAIRS;
+// Half a tile of (row, head) pairs at least, and tiles for a good part of the SMs: the 16-row form
+// splits few tiles' keys over all SMs, this one walks them alone.  Append and attention over 4000
+// older tokens, 16-row form against this one: 8 tiles 48 / 84 us (bf16, head_dim 128), 57 / 113
+// (fp32), 89 / 119 (bf16, 256); 16 tiles 64 / 93, 85 / 115, 118 / 121; 32 tiles 94 / 89, 137 / 121,
+// 172 / 128; 160 tiles 330 / 135, 505 / 243, 600 / 262.
+bool kv8_prompt_takes(const q35_kv8_cache &c, int32_t heads, int32_t max_rows) {
+    const int64_t pairs = (int64_t)max_rows * (heads / c.kv_heads);
+    return pairs >= PT_ROWS / 2 && ceil_div(pairs, PT_ROWS) * c.seqs * c.kv_heads >= 32;
 }
 
 int launch_kv8_prompt(const AttnParams &p, int dtype, int code, int D, int zs, cudaStream_t s) {
+    if (dtype == Q35_DT_F32) return launch_prompt<float>(p, code, D, zs, s);
     return dtype == Q35_DT_BF16 ? launch_prompt<__nv_bfloat16>(p, code, D, zs, s) : launch_prompt<__half>(p, code, D, zs, s);
 }
 

@@ -181,10 +181,20 @@ PROMPTS = [  # heads, kv heads, D, block, max_seq, counts, past, scale, columns 
     (1, 1, 128, 64, 1300, [129], [1171], 0.0, 0),                         # 0: the mean of what a row sees
     (3, 1, 64, 16, 65, [64, 65, 1], [1, 0, 64], 0.125, 0),
     (16, 2, 128, 128, 2500, [9], [2491], 0.0884, 16),
+    # below: tiles of 128 rows for many SMs
+    (24, 24, 128, 64, 700, [64, 300, 0], [0, 333, 9], 0.09, 0),
+    (64, 16, 64, 16, 300, [33, 1, 129], [7, 299, 171], -0.09, 1),
+    (16, 16, 128, 64, 1300, [129], [1171], 0.0, 0),
+    (48, 16, 128, 16, 65, [64, 65, 1], [1, 0, 64], 0.125, 0),
+    (3, 3, 256, 64, 500, [190, 0, 70], [310, 40, 5], 0.0625, 0),
+    (8, 2, 256, 16, 300, [17, 33], [200, 0], -0.0625, 5),
+    (16, 16, 128, 64, 900, [140, 129, 131, 150], [700, 0, 3, 64], 0.0884, 0),
+    (40, 20, 64, 64, 1100, [300], [777], 0.125, 4),
+    (6, 6, 256, 128, 1000, [140, 257, 300, 128, 65, 129, 150, 200], [800, 0, 3, 64, 9, 129, 640, 1], 0.0625, 4),
 ]
 
 
-@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("code", ["int8", "e4m3"])
 @pytest.mark.parametrize("case", PROMPTS, ids=[str(i) for i in range(len(PROMPTS))])
 def test_attention_of_prompts(ctx, dtype, code, case):
@@ -214,14 +224,15 @@ def test_attention_of_prompts(ctx, dtype, code, case):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("heads,D,past,rows", [(1, 128, 13, 6), (1, 128, 5, 40), (2, 64, 5, 123), (1, 256, 7, 20)])
-def test_later_values_take_no_bits_from_earlier_rows(ctx, dtype, heads, D, past, rows):
+@pytest.mark.parametrize("heads,G,D,past,rows", [(1, 1, 128, 13, 6), (1, 1, 128, 5, 40), (2, 1, 64, 5, 123), (1, 1, 256, 7, 20),
+                                                 (40, 40, 128, 5, 123), (64, 32, 64, 5, 100), (32, 32, 256, 7, 80)])
+def test_later_values_take_no_bits_from_earlier_rows(ctx, dtype, heads, G, D, past, rows):
     """Values that grow by 2^7 from block to block: a row is as exact as what it sees is large."""
     rng = np.random.default_rng(heads * D + rows)
     S = past + rows
-    c = Cache(ctx, "int8", 1, 1, D, S, 16, 3)
+    c = Cache(ctx, "int8", 1, G, D, S, 16, 3)
     grow = 2.0 ** (-100 + 7 * (np.arange(S) // 16))[:, None] if dtype != "f16" else 2.0 ** (-14 + 3 * (np.arange(S) // 16))[:, None]
-    k, v = dev(rng.normal(0, 1, (S, D)), dtype), dev(rng.normal(0, 1, (S, D)) * grow, dtype)
+    k, v = dev(rng.normal(0, 1, (S, G * D)), dtype), dev(rng.normal(0, 1, (S, G * D)) * grow, dtype)
     c.append(k, v, [S], [0], dtype)
     q = dev(rng.normal(0, 1, (rows, heads * D)), dtype)
     out = c.attend(q, heads, [rows], [past], dtype, D ** -0.5)
@@ -234,30 +245,34 @@ def test_later_values_take_no_bits_from_earlier_rows(ctx, dtype, heads, D, past,
     check_attention(got, ref, mag, vmax, D, dtype)
 
 
-def test_values_of_the_smallest_numbers(ctx):
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("G", [1, 20])
+def test_values_of_the_smallest_numbers(ctx, G, dtype):
     """Block scales that are subnormal: no division by one makes an infinity."""
     D, S = 128, 200
     rng = np.random.default_rng(3)
     for rows in (1, 20, S):
-        c = Cache(ctx, "e4m3", 1, 1, D, S, 16, 4)
+        c = Cache(ctx, "e4m3", 1, G, D, S, 16, 4)
         size = np.choose(np.arange(S) // 16 % 3, [0.0, 1e-38, 3e-37])[:, None]
-        k, v = dev(rng.normal(0, 1, (S, D)), "bf16"), dev(rng.normal(0, 1, (S, D)) * size, "bf16")
-        c.append(k, v, [S], [0], "bf16")
-        q = dev(rng.normal(0, 1, (rows, D)), "bf16")
-        out = c.attend(q, 1, [rows], [S - rows], "bf16", 0.09)
+        k, v = dev(rng.normal(0, 1, (S, G * D)), dtype), dev(rng.normal(0, 1, (S, G * D)) * size, dtype)
+        c.append(k, v, [S], [0], dtype)
+        q = dev(rng.normal(0, 1, (rows, G * D)), dtype)
+        out = c.attend(q, G, [rows], [S - rows], dtype, 0.09)
         assert torch.isfinite(out).all() and float(out.abs().max()) <= 1.5e-36
 
 
-def test_prompt_rows_that_are_not_numbers_stay_alone(ctx):
-    heads, D, S = 2, 128, 200
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("G", [1, 16])
+def test_prompt_rows_that_are_not_numbers_stay_alone(ctx, G, dtype):
+    heads, D, S = 2 * G, 128, 200
     rng = np.random.default_rng(17)
-    c = Cache(ctx, "int8", 1, 1, D, S, 64, 8)
-    kv = {n: dev(rng.normal(0, 1, (S, D)), "bf16") for n in "kv"}
-    c.append(kv["k"], kv["v"], [S], [0], "bf16")
-    q = dev(rng.normal(0, 1, (S, heads * D)), "bf16")
-    clean = c.attend(q, heads, [S], [0], "bf16", 0.09)
+    c = Cache(ctx, "int8", 1, G, D, S, 64, 8)
+    kv = {n: dev(rng.normal(0, 1, (S, G * D)), dtype) for n in "kv"}
+    c.append(kv["k"], kv["v"], [S], [0], dtype)
+    q = dev(rng.normal(0, 1, (S, heads * D)), dtype)
+    clean = c.attend(q, heads, [S], [0], dtype, 0.09)
     q[50, 3] = float("nan")
-    out = c.attend(q, heads, [S], [0], "bf16", 0.09)
+    out = c.attend(q, heads, [S], [0], dtype, 0.09)
     assert torch.isnan(out[50, :D]).all()
     out[50, :D] = clean[50, :D]
     assert torch.equal(out, clean)
