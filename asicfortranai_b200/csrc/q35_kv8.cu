@@ -20,9 +20,9 @@
 // probabilities take two fp16 terms each (22 bits).  Maximum, sum and outputs are fp32.
 //
 // Measured, append and attention together: 16 sequences of 301 to 8100 tokens, 8 kv heads and 64
-// heads of 128 44 us (131 MB of codes, 3 TB/s), three of 40 to 65 thousand with 32 heads 74 us (306
-// MB, 4.1 TB/s); one token after 2000 12 to 18 us, three launches.  The append of 2048 tokens of
-// 40 heads 36 us (64 MB): its issue slots are 62 % busy.
+// heads of 128 45 us (130 MB of codes, 2.9 TB/s), three of 40 to 65 thousand with 32 heads 75 us (306
+// MB, 4.1 TB/s); one token after 2000 13 us, three launches.  The append of 2048 tokens of
+// 40 heads 28 us (64 MB): conversions and roundings, about 20 instructions an element.
 //
 // Prompts take 128-row tiles on tcgen05 instead (q35_kv8_prompt.cu).
 //
@@ -67,20 +67,19 @@ template <int CODE> __device__ __forceinline__ uint32_t encode_quotients(const f
     bool near = !fast;
     uint32_t word = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) t[i] = (x[i] != x[i] ? 0.0f : x[i]) * r;
+    for (int i = 0; i < 4; ++i) t[i] = x[i] * r;
     if (CODE == Q35_CODE_INT8) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float c = fminf(fmaxf(t[i], -127.0f), 127.0f);
-            const float k = __fadd_rn(c, 12582912.0f);        // 3 2^22: the sum's last bits are the whole number
-            near |= fabsf(c - __fadd_rn(k, -12582912.0f)) > 0.4999f;
+            const float k = __fadd_rn(t[i], 12582912.0f);     // 3 2^22: the sum's last bits are the whole number
+            near |= !(fabsf(t[i] - __fadd_rn(k, -12582912.0f)) <= 0.4999f);    // (infinities and NaN too)
             word |= (__float_as_uint(k) & 0xffu) << (8 * i);
         }
     } else {
         // boundaries lie half way between numbers of 3 fraction bits (from 2^-6 on)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            near |= fabsf(t[i]) < 0.015626f || ((__float_as_uint(t[i]) - 0x7fff8u) & 0xfffffu) < 16u;
+            near |= !(fabsf(t[i]) >= 0.015626f) || ((__float_as_uint(t[i]) - 0x7fff8u) & 0xfffffu) < 16u;
         word = encode8x4<CODE>(t[0], t[1], t[2], t[3]);
     }
     if (near) {
@@ -109,49 +108,69 @@ __global__ void __launch_bounds__(APPEND_THREADS) kv8_append_kernel(const Append
     const int held = first - t0, fresh = last - first;
 
     // four elements a thread and round, all of the block's rounds in flight (a whole block of 128
-    // tokens by 256 is 32 rounds: those take two passes over the input)
-    constexpr int R = TB * D / (4 * APPEND_THREADS) < 8 ? (TB * D / (4 * APPEND_THREADS) < 1 ? 1 : TB * D / (4 * APPEND_THREADS)) : 8;
+    // tokens by 256 is 32 rounds: those take several passes over the input)
+    constexpr int STEP = 4 * APPEND_THREADS, ROUNDS = TB * D / STEP, R = ROUNDS < 8 ? ROUNDS : 8;
+    static_assert(STEP % D == 0 && ROUNDS >= 1, "a round is whole tokens, a block whole rounds");
     const bool vec = p.vec;
-    auto load4 = [&](int e, float (&v)[4]) {
-        const T *s = x + (int64_t)(e / D) * p.ld + e % D;
-        if (vec) {
-            if constexpr (sizeof(T) == 4) {
-                const float4 u = *reinterpret_cast<const float4 *>(s);
-                v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
-            } else {
-                const uint2 u = *reinterpret_cast<const uint2 *>(s);
+    const int64_t next = (int64_t)(STEP / D) * p.ld;         // elements of x between rounds
+    const T *mine = x + (int64_t)(4 * threadIdx.x / D) * p.ld + 4 * threadIdx.x % D;
+    // (held as they stand in memory: half the registers for 16-bit types)
+    using Raw = typename std::conditional<sizeof(T) == 4, uint4, uint2>::type;
+    Raw raw[R];
+    const int total = fresh * D;
+    auto load = [&](int e0) {                                // rounds e0 / STEP .. of this thread's elements
+        const T *s = mine + e0 / STEP * next;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            raw[r] = Raw{};                                  // (zeros)
+            if (e0 + r * STEP + 4 * (int)threadIdx.x >= total) continue;
+            if (vec) raw[r] = *reinterpret_cast<const Raw *>(s + r * next);
+            else {
                 T w[4];
-                memcpy(w, &u, 8);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = to_f32<T>(w[i]);
+                for (int i = 0; i < 4; ++i) w[i] = s[r * next + i];
+                memcpy(&raw[r], w, sizeof(w));
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = to_f32<T>(s[i]);
         }
     };
-    float amax = 0.0f, v[R][4];
-    const int total = fresh * D;
-    for (int e0 = 4 * threadIdx.x; e0 < total; e0 += 4 * APPEND_THREADS * R) {
+    auto values = [&](int r, float (&v)[4]) {
+        T w[4];
+        memcpy(w, &raw[r], sizeof(w));
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-            if (e0 + 4 * APPEND_THREADS * r < total) load4(e0 + 4 * APPEND_THREADS * r, v[r]);
+        for (int i = 0; i < 4; ++i) v[i] = to_f32<T>(w[i]);
+    };
+    auto over_cta = [&](float amax) {
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-            if (e0 + 4 * APPEND_THREADS * r < total)
+        for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = amax;
+        __syncthreads();
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float a = fabsf(v[r][i]);
-                    if (a <= 3.402823466e38f) amax = fmaxf(amax, a);
-                }
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = amax;
+        for (int w = 0; w < APPEND_THREADS / 32; ++w) amax = fmaxf(amax, part[w]);
+        return amax;
+    };
     const float old = held ? *scale : 0.0f;
-    __syncthreads();
+    float amax = 0.0f;                                       // (fmaxf leaves NaN out)
+    for (int e0 = 0; e0 < total; e0 += R * STEP) {
+        load(e0);
 #pragma unroll
-    for (int w = 0; w < APPEND_THREADS / 32; ++w) amax = fmaxf(amax, part[w]);
+        for (int r = 0; r < R; ++r) {
+            float v[4];
+            values(r, v);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fabsf(v[i]));
+        }
+    }
+    amax = over_cta(amax);
+    if (amax > FLT_MAX) {                                    // infinities do not count: once more without
+        amax = 0.0f;
+#pragma unroll 1
+        for (int e = threadIdx.x; e < total; e += APPEND_THREADS) {
+            const float a = fabsf(to_f32<T>(x[(int64_t)(e / D) * p.ld + e % D]));
+            if (a <= FLT_MAX) amax = fmaxf(amax, a);
+        }
+        __syncthreads();
+        amax = over_cta(amax);
+    }
     const float now = fmaxf(old, __fmul_rn(amax, 1.0f / code_max<CODE>()));
     if (threadIdx.x == 0) *scale = now;
     if (held && now != old)
@@ -164,18 +183,14 @@ __global__ void __launch_bounds__(APPEND_THREADS) kv8_append_kernel(const Append
         }
     codes += held * D;
     const float recip = __fdiv_rn(1.0f, now);
-    const bool once = total <= 4 * APPEND_THREADS * R;       // the values are still here
-    for (int e0 = 4 * threadIdx.x; e0 < total; e0 += 4 * APPEND_THREADS * R) {
-        if (!once) {
-#pragma unroll
-            for (int r = 0; r < R; ++r)
-                if (e0 + 4 * APPEND_THREADS * r < total) load4(e0 + 4 * APPEND_THREADS * r, v[r]);
-        }
+    for (int e0 = 0; e0 < total; e0 += R * STEP) {
+        if (total > R * STEP) load(e0);                      // (else the values are still here)
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const int e = e0 + 4 * APPEND_THREADS * r;
-            if (e >= total) continue;
-            *reinterpret_cast<uint32_t *>(codes + e) = encode_quotients<CODE>(v[r], now, recip, now >= 1e-30f);
+            const int e = e0 + r * STEP + 4 * threadIdx.x;
+            float v[4];
+            values(r, v);
+            if (e < total) *reinterpret_cast<uint32_t *>(codes + e) = encode_quotients<CODE>(v, now, recip, now >= 1e-30f);
         }
     }
 }

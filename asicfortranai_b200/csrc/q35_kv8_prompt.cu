@@ -15,8 +15,8 @@
 //     as fp16 into S's buffer.
 // fp32 queries and their weights take two fp16 terms each (22 bits), with two MMAs for one.
 //
-// Sums and O are fp32.  Measured, 2048 rows of 40 heads of 128 over 2001 older tokens, bf16: 276 us
-// (of 75 for the operations at the fp16 rate), f32 about 400.  A CTA's step of 64 keys takes 3300
+// Sums and O are fp32.  Measured, 2048 rows of 40 heads of 128 over 2001 older tokens, bf16: 250 us
+// (75 are the operations at the fp16 rate), f32 about 445.  A CTA's step of 64 keys takes 3300
 // clocks, of which a softmax warp works 2000 (1500 of them on the weights: 16 exponentials a clock
 // and SM alone are 512 for each of the SM's two CTAs) and the tensor pipe is busy for 640.
 //
