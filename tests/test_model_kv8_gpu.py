@@ -32,7 +32,20 @@ def layer_model(ctx, cfg, seed):
 @pytest.mark.parametrize("code", ["int8", "e4m3"])
 @pytest.mark.parametrize("D,H,KVH,block", [(128, 4, 2, 64), (256, 2, 1, 16), (128, 8, 1, 32)])
 def test_layer_over_an_8_bit_cache(ctx, code, D, H, KVH, block):
-    cfg = dict(TINY, n_layers=2, n_heads=H, n_kv_heads=KVH, head_dim=D, hidden=512, wformat=1, max_batch=2, max_seq=100)
+    check_layer(ctx, code, D, H, KVH, block, 100,
+                [(1, 1, 9, 1.0), (0, 1, 3, 2.0), (1, 1, 1, 1.0), (1, 1, 1, 30.0), (1, 1, 40, 0.5), (0, 1, 1, 1.0)])
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("D,H,KVH,block", [(128, 16, 16, 64), (128, 32, 8, 32), (256, 12, 12, 16)])
+def test_layer_of_a_prompt_over_an_8_bit_cache(ctx, code, D, H, KVH, block):
+    """Rows for many 128-row tiles, first and behind others."""
+    check_layer(ctx, code, D, H, KVH, block, 410, [(0, 1, 260, 1.0), (0, 1, 131, 2.0), (1, 1, 300, 0.5), (0, 1, 1, 1.0)])
+
+
+def check_layer(ctx, code, D, H, KVH, block, max_seq, calls):
+    """calls: (sequence, layer, rows, size of the input)"""
+    cfg = dict(TINY, n_layers=2, n_heads=H, n_kv_heads=KVH, head_dim=D, hidden=512, wformat=1, max_batch=2, max_seq=max_seq)
     gm, w = layer_model(ctx, cfg, 31)
     gm.set_kv_cache(code, block=block)
     S, nblk, hid = cfg["max_seq"], -(-cfg["max_seq"] // block), cfg["hidden"]
@@ -41,7 +54,7 @@ def test_layer_over_an_8_bit_cache(ctx, code, D, H, KVH, block):
     scales = {n: np.zeros((2, 2, KVH, nblk), np.float32) for n in "kv"}
     past = [0, 0]
     wo = orc.matmul_int4_awq                                         # int32 accumulators of an int8 matrix
-    for seq, layer, n, size in [(1, 1, 9, 1.0), (0, 1, 3, 2.0), (1, 1, 1, 1.0), (1, 1, 1, 30.0), (1, 1, 40, 0.5), (0, 1, 1, 1.0)]:
+    for seq, layer, n, size in calls:
         x = (rng.normal(0, size, (n, hid)) * np.exp(rng.normal(0, 1, (n, 1)))).astype(np.float32)
         out = gm.apply_transformer_layer(layer, x, seq=seq)
         QN, KN = H * D, KVH * D
@@ -59,13 +72,12 @@ def test_layer_over_an_8_bit_cache(ctx, code, D, H, KVH, block):
             np.testing.assert_array_equal(gots[nm], scales[nm])
             val[nm] = decode(codes[nm][seq, layer], code) * np.repeat(scales[nm][seq, layer].astype(np.float64), block, 1)[:, :S, None]
         att = np.zeros((n, H, D))
-        for i in range(n):
-            L = past[seq] + i + 1
-            for h in range(H):
-                g = h * KVH // H
-                s = val["k"][g, :L] @ q[i, h].astype(np.float64) / np.sqrt(D)
-                p = np.exp(s - s.max())
-                att[i, h] = p @ val["v"][g, :L] / p.sum()
+        seen = np.arange(past[seq] + n)[None] <= past[seq] + np.arange(n)[:, None]
+        for h in range(H):
+            g = h * KVH // H
+            s = np.where(seen, q[:, h].astype(np.float64) @ val["k"][g, :past[seq] + n].T / np.sqrt(D), -np.inf)
+            p = np.exp(s - s.max(1, keepdims=True))
+            att[:, h] = p @ val["v"][g, :past[seq] + n] / p.sum(1, keepdims=True)
         a = np.clip(att.reshape(n, QN) * 127.0, -127, 127)
         ai = np.trunc(a).astype(np.int8)
         # an attention output within 2^-14 of a step of 127 a may fall on either side of it

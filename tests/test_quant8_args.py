@@ -174,3 +174,15 @@ def test_reference_sampler_on_known_rows():
     assert sample_ref(lg, 1.0, 0, 0.5, 0.0, 0.99)[0] == 3       # 0.4 does not reach 0.5, 0.7 does
     assert sample_ref(lg, 1.0, 0, 1.0, 0.6, 0.99)[0] == 3       # at least 0.24
     assert sample_ref(np.full(4, -np.inf), 1.0, 0, 1.0, 0.0, 0.5) == (0, 0.0)
+
+
+def test_the_program_takes_a_cache_format():
+    import os
+    import subprocess
+
+    from asicfortranai_b200 import build
+    build.build()
+    cli = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "asicfortranai_b200", "bin", "llama_generate")
+    assert "--kv-cache" in subprocess.run([cli, "--help"], capture_output=True, text=True).stdout
+    for bad in (["--kv-cache", "int7"], ["--kv-cache"]):
+        assert subprocess.run([cli, *bad], capture_output=True).returncode == 2
