@@ -509,18 +509,21 @@ __global__ void __launch_bounds__(ATT_THREADS, AttnShape<D>::CTAS) kv8_attn_kern
                         codes_f16<CODE>(__byte_perm(a0, a1, hh ? 0x7362 : 0x5140), b0, b1);
                         codes_f16<CODE>(__byte_perm(a2, a3, hh ? 0x7362 : 0x5140), b2, b3);
                         const int t = (j * VW + w4) * 4 + 2 * hh;
-                        mma16816(o[t], pa, b0, b2);
-                        mma16816(o[t + 1], pa, b1, b3);
                         if (TERMS == 2) {
-                            // the low terms carry a factor 2^11 that keeps them in fp16's normal range
+                            // the low terms carry a factor 2^11 that keeps them in fp16's normal range;
+                            // rounded additions over the steps
                             float lo0[4] = {0, 0, 0, 0}, lo1[4] = {0, 0, 0, 0};
                             mma16816(lo0, pl, b0, b2);
                             mma16816(lo1, pl, b1, b3);
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                o[t][i] = fmaf(lo0[i], 1.0f / 2048.0f, o[t][i]);
-                                o[t + 1][i] = fmaf(lo1[i], 1.0f / 2048.0f, o[t + 1][i]);
-                            }
+                            for (int i = 0; i < 4; ++i) { lo0[i] *= 1.0f / 2048.0f; lo1[i] *= 1.0f / 2048.0f; }
+                            mma16816(lo0, pa, b0, b2);
+                            mma16816(lo1, pa, b1, b3);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) { o[t][i] += lo0[i]; o[t + 1][i] += lo1[i]; }
+                        } else {
+                            mma16816(o[t], pa, b0, b2);
+                            mma16816(o[t + 1], pa, b1, b3);
                         }
                     }
                 }
@@ -723,11 +726,13 @@ __global__ void __launch_bounds__(ATT_THREADS, D == 256 ? 1 : 2) kv8_attn8_kerne
 
     for (; kk < k1; kk += ATT_WARPS * KC) {
         const int nk = kk + ATT_WARPS * KC;
-        float s[U][4];
+        // (the tensor cores' sums lose what lies below the accumulator's last bit, each time: the low
+        // terms of fp32 queries have a sum of their own)
+        float s[U][4], sl[U][4];
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[u][i] = 0.0f;
+            for (int i = 0; i < 4; ++i) s[u][i] = sl[u][i] = 0.0f;
 #pragma unroll
         for (int j = 0; j < KL; ++j)
 #pragma unroll
@@ -747,7 +752,7 @@ __global__ void __launch_bounds__(ATT_THREADS, D == 256 ? 1 : 2) kv8_attn8_kerne
                     codes_f16<CODE>(i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w, a.x, a.z);
                     codes_f16<CODE>(i == 0 ? y.x : i == 1 ? y.y : i == 2 ? y.z : y.w, a.y, a.w);
                     mma16816(s[u], a, q0, q1);
-                    if (TERMS == 2) mma16816(s[u], a, q2, q3);
+                    if (TERMS == 2) mma16816(sl[u], a, q2, q3);
                 }
             }
         float ksc[U], vsc[U][2], vtop[2] = {vref[0], vref[1]};
@@ -765,7 +770,7 @@ __global__ void __launch_bounds__(ATT_THREADS, D == 256 ? 1 : 2) kv8_attn8_kerne
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[u][i] *= qs[i & 1] * ksc[u];
+            for (int i = 0; i < 4; ++i) s[u][i] = (TERMS == 2 ? s[u][i] + sl[u][i] : s[u][i]) * (qs[i & 1] * ksc[u]);
         if (kk + KC > all_see) {                 // some row does not see some key of the step
 #pragma unroll
             for (int u = 0; u < U; ++u)
@@ -848,8 +853,13 @@ __global__ void __launch_bounds__(ATT_THREADS, D == 256 ? 1 : 2) kv8_attn8_kerne
                         codes_f16<CODE>(__byte_perm(vr[u][0][j][w4], vr[u][1][j][w4], hh ? 0x7362 : 0x5140), a.x, a.y);
                         codes_f16<CODE>(__byte_perm(vr[u][2][j][w4], vr[u][3][j][w4], hh ? 0x7362 : 0x5140), a.z, a.w);
                         const int t = (j * VW + w4) * 2 + hh;
-                        mma16816(o[t], a, b0, b1);
-                        if (TERMS == 2) mma16816(o[t], a, c0, c1);
+                        if (TERMS == 2) {
+                            float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};        // (rounded additions over the steps)
+                            mma16816(x, a, c0, c1);
+                            mma16816(x, a, b0, b1);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) o[t][i] += x[i];
+                        } else mma16816(o[t], a, b0, b1);
                     }
         }
         if (nk < k1) load_v(nk);
