@@ -173,16 +173,25 @@ __global__ void __launch_bounds__(APPEND_THREADS) kv8_append_kernel(const Append
     }
     const float now = fmaxf(old, __fmul_rn(amax, 1.0f / code_max<CODE>()));
     if (threadIdx.x == 0) *scale = now;
-    if (held && now != old)
-        for (int e = 4 * threadIdx.x; e < held * D; e += 4 * APPEND_THREADS) {
-            const uint32_t c = *reinterpret_cast<const uint32_t *>(codes + e);
-            float u[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) u[i] = __fdiv_rn(__fmul_rn(decode8<CODE>((uint8_t)(c >> (8 * i))), old), now);
-            *reinterpret_cast<uint32_t *>(codes + e) = encode8x4<CODE>(u[0], u[1], u[2], u[3]);
-        }
-    codes += held * D;
     const float recip = __fdiv_rn(1.0f, now);
+    const bool fast = now >= 1e-30f;
+    if (held && now != old) {
+        uint32_t *w = reinterpret_cast<uint32_t *>(codes) + threadIdx.x;
+        const int n = held * D / 4 - (int)threadIdx.x;       // words from this thread's first one on
+        for (int i0 = 0; i0 < n; i0 += R * APPEND_THREADS) {
+            uint32_t c[R];                                   // (a round's loads together: one latency)
+#pragma unroll
+            for (int r = 0; r < R; ++r) c[r] = i0 + r * APPEND_THREADS < n ? w[i0 + r * APPEND_THREADS] : 0u;
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                float v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = __fmul_rn(decode8<CODE>((uint8_t)(c[r] >> (8 * i))), old);
+                if (i0 + r * APPEND_THREADS < n) w[i0 + r * APPEND_THREADS] = encode_quotients<CODE>(v, now, recip, fast);
+            }
+        }
+    }
+    codes += held * D;
     for (int e0 = 0; e0 < total; e0 += R * STEP) {
         if (total > R * STEP) load(e0);                      // (else the values are still here)
 #pragma unroll
@@ -190,7 +199,7 @@ __global__ void __launch_bounds__(APPEND_THREADS) kv8_append_kernel(const Append
             const int e = e0 + r * STEP + 4 * threadIdx.x;
             float v[4];
             values(r, v);
-            if (e < total) *reinterpret_cast<uint32_t *>(codes + e) = encode_quotients<CODE>(v, now, recip, now >= 1e-30f);
+            if (e < total) *reinterpret_cast<uint32_t *>(codes + e) = encode_quotients<CODE>(v, now, recip, fast);
         }
     }
 }
