@@ -15,8 +15,9 @@
 // are one side of m16n8k16 tensor-core tiles -- the 8 columns (kv8_attn8_kernel, up to 8 pairs
 // in all: single tokens) or the 16 rows (kv8_attn_kernel).  Codes become fp16 exactly (both codes
 // fit its 11 bits), the scale multiplies the fp32 scores of its block, and v's scale the
-// probabilities, relative to the largest v scale that the row has seen (at most 1), so no range is
-// lost.  A query row is scaled by a power of two to use fp16's range; fp32 queries and their
+// probabilities, relative to the largest v scale that the row has seen (at most 1).  They are the
+// other operand in fp16: 11 bits of a weight, with a factor that spends fp16's range on small ones
+// (ATT_BOOST).  A query row is scaled by a power of two to use fp16's range; fp32 queries and their
 // probabilities take two fp16 terms each (22 bits).  Maximum, sum and outputs are fp32.
 //
 // Measured, append and attention together: 16 sequences of 301 to 8100 tokens, 8 kv heads and 64
@@ -210,6 +211,12 @@ constexpr int ATT_WARPS = 8;
 constexpr int ATT_THREADS = 32 * ATT_WARPS;
 constexpr int ATT_M = 16;                 // (row, head) pairs per CTA
 constexpr int ATT_MAX_SPLITS = 64;        // CTAs that share a tile's keys
+// Factor of the weights in fp16.  A weight is at most 1 (the row's largest score, the largest v scale) and
+// the ones that carry a row can be far below it: a key high above the others whose value is small, a block
+// of large values without weight.  With 2^15 a weight keeps its 11 bits down to 2^-29 and is off by 2^-40
+// at most below that (without: 2^-14 and 2^-25).  fp32 queries' second term, the rest of the first, carries
+// another 2^11: 22 bits, or 2^-51.
+constexpr float ATT_BOOST = 32768.0f, ATT_LOW = 2048.0f;
 
 __device__ __forceinline__ uint2 ldg8(const uint8_t *p) {
     uint2 v;
@@ -491,7 +498,8 @@ __global__ void __launch_bounds__(ATT_THREADS, AttnShape<D>::CTAS) kv8_attn_kern
         if (kk + KC > k1) clear_v(kk);
 #pragma unroll
         for (int u = 0; u < NT / 2; ++u) {
-            const float w[2] = {vsc[u][0] == vref[0] ? 1.0f : vsc[u][0] * vinv[0], vsc[u][1] == vref[1] ? 1.0f : vsc[u][1] * vinv[1]};
+            const float w[2] = {vsc[u][0] == vref[0] ? ATT_BOOST : vsc[u][0] * vinv[0] * ATT_BOOST,
+                                vsc[u][1] == vref[1] ? ATT_BOOST : vsc[u][1] * vinv[1] * ATT_BOOST};
             uint4 pa, pl;
             float x[8];
 #pragma unroll
@@ -503,7 +511,7 @@ __global__ void __launch_bounds__(ATT_THREADS, AttnShape<D>::CTAS) kv8_attn_kern
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float2 hf = __half22float2(*reinterpret_cast<const __half2 *>(&hp[i]));
-                    lp[i] = pack2<__half>((x[2 * i] - hf.x) * 2048.0f, (x[2 * i + 1] - hf.y) * 2048.0f);
+                    lp[i] = pack2<__half>((x[2 * i] - hf.x) * ATT_LOW, (x[2 * i + 1] - hf.y) * ATT_LOW);
                 }
             }
 #pragma unroll
@@ -519,13 +527,12 @@ __global__ void __launch_bounds__(ATT_THREADS, AttnShape<D>::CTAS) kv8_attn_kern
                         codes_f16<CODE>(__byte_perm(a2, a3, hh ? 0x7362 : 0x5140), b2, b3);
                         const int t = (j * VW + w4) * 4 + 2 * hh;
                         if (TERMS == 2) {
-                            // the low terms carry a factor 2^11 that keeps them in fp16's normal range;
-                            // rounded additions over the steps
+                            // (rounded additions over the steps)
                             float lo0[4] = {0, 0, 0, 0}, lo1[4] = {0, 0, 0, 0};
                             mma16816(lo0, pl, b0, b2);
                             mma16816(lo1, pl, b1, b3);
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) { lo0[i] *= 1.0f / 2048.0f; lo1[i] *= 1.0f / 2048.0f; }
+                            for (int i = 0; i < 4; ++i) { lo0[i] *= 1.0f / ATT_LOW; lo1[i] *= 1.0f / ATT_LOW; }
                             mma16816(lo0, pa, b0, b2);
                             mma16816(lo1, pa, b1, b3);
 #pragma unroll
@@ -554,7 +561,7 @@ __global__ void __launch_bounds__(ATT_THREADS, AttnShape<D>::CTAS) kv8_attn_kern
         for (int i = 0; i < 4; ++i) {
             const int n = 2 * c + (i & 1);      // column tile t, column n: see load_v
             const int d = D == 64 ? n * 8 + t : (t / 16) * 128 + n * 16 + t % 16;
-            mg[(warp * ATT_M + g + 8 * (i >> 1)) * RO + d] = o[t][i] * vref[i >> 1];
+            mg[(warp * ATT_M + g + 8 * (i >> 1)) * RO + d] = o[t][i] * (1.0f / ATT_BOOST) * vref[i >> 1];
         }
     __syncthreads();
     for (int r = warp; r < fn; r += ATT_WARPS) {
@@ -833,7 +840,8 @@ __global__ void __launch_bounds__(ATT_THREADS, D == 256 ? 1 : 2) kv8_attn8_kerne
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const float w[2] = {vsc[u][0] == vref[0] ? 1.0f : vsc[u][0] * vinv[0], vsc[u][1] == vref[1] ? 1.0f : vsc[u][1] * vinv[1]};
+            const float w[2] = {vsc[u][0] == vref[0] ? ATT_BOOST : vsc[u][0] * vinv[0] * ATT_BOOST,
+                                vsc[u][1] == vref[1] ? ATT_BOOST : vsc[u][1] * vinv[1] * ATT_BOOST};
             float x[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -848,8 +856,8 @@ __global__ void __launch_bounds__(ATT_THREADS, D == 256 ? 1 : 2) kv8_attn8_kerne
             if (TERMS == 2) {
                 const float2 f0 = __half22float2(*reinterpret_cast<const __half2 *>(&h0));
                 const float2 f1 = __half22float2(*reinterpret_cast<const __half2 *>(&h1));
-                c0 = transpose8x8(pack2<__half>(x[0] - f0.x, x[1] - f0.y));
-                c1 = transpose8x8(pack2<__half>(x[2] - f1.x, x[3] - f1.y));
+                c0 = transpose8x8(pack2<__half>((x[0] - f0.x) * ATT_LOW, (x[1] - f0.y) * ATT_LOW));
+                c1 = transpose8x8(pack2<__half>((x[2] - f1.x) * ATT_LOW, (x[3] - f1.y) * ATT_LOW));
             }
 #pragma unroll
             for (int j = 0; j < VL; ++j)
@@ -865,6 +873,8 @@ __global__ void __launch_bounds__(ATT_THREADS, D == 256 ? 1 : 2) kv8_attn8_kerne
                         if (TERMS == 2) {
                             float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};        // (rounded additions over the steps)
                             mma16816(x, a, c0, c1);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) x[i] *= 1.0f / ATT_LOW;
                             mma16816(x, a, b0, b1);
 #pragma unroll
                             for (int i = 0; i < 4; ++i) o[t][i] += x[i];
@@ -887,7 +897,7 @@ __global__ void __launch_bounds__(ATT_THREADS, D == 256 ? 1 : 2) kv8_attn8_kerne
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int d = (D == 64 ? 8 * g : (t / 8) * 128 + 16 * g) + 2 * (t % 8) + (i >> 1);
-            mg[(warp * TM + 2 * c + (i & 1)) * RO + d] = o[t][i] * vref[i & 1];
+            mg[(warp * TM + 2 * c + (i & 1)) * RO + d] = o[t][i] * (1.0f / ATT_BOOST) * vref[i & 1];
         }
     __syncthreads();
     if (warp < fn) {
