@@ -10,9 +10,9 @@
 //     O += P V with P from tensor memory;
 //   * softmax (warps 0..3, a row per thread): S from tensor memory, times the row's and the
 //     block's scale, masked; weights relative to a reference that follows the running maximum
-//     only when that has grown by 2^8 (weights stay below 2^8, fp16 holds them with 11 bits), so
-//     O is rarely moved; weights times the block's v scale over the largest one so far go back
-//     as fp16 into S's buffer.
+//     only when that has grown by 2^4 (fp32 queries: 2), so O is rarely moved; weights times the
+//     block's v scale over the largest one so far go back as fp16 into S's buffer, with a factor that
+//     spends fp16's range on small ones.
 // fp32 queries and their weights take two fp16 terms each (22 bits), with two MMAs for one.
 //
 // Sums and O are fp32.  Measured, 2048 rows of 40 heads of 128 over 2001 older tokens, bf16: 250 us
@@ -33,9 +33,6 @@ namespace {
 constexpr int PT_ROWS = 128;               // (row, head) pairs per CTA
 constexpr int PT_KEYS = 64;                // keys per step
 constexpr int PT_THREADS = 288;
-constexpr float PT_SLACK = 8.0f;           // log2 by which a row's maximum may pass its reference
-
-constexpr float PT_BOOST = 128.0f;         // factor of the weights in fp16: 2^8 2^7 is in its range, and 2^-31 not 0
 
 // TERMS: fp16 terms of a query element and of a weight (2 for fp32 queries: 22 bits)
 template <int TERMS, int D> struct Prompt {
@@ -45,6 +42,13 @@ template <int TERMS, int D> struct Prompt {
     static constexpr uint32_t tmem = D > 128 ? 512 : 256;              // columns: S 2 x 64, O
     static constexpr uint32_t off_k = TERMS * Q, off_v = off_k + stages * K, off_bar = off_v + stages * V;
     static constexpr size_t smem = 1024 + off_bar + 8 * 18 + 16 + 4 * 32;
+    // A row's maximum may pass its reference by 2^slack, and the weights carry a factor `boost` in fp16:
+    // 2^15 together.  The factor keeps the bits of weights far below the reference (a key high above the
+    // others whose value is small, a block of large values without weight): 11 bits down to 2^-25 of it and
+    // 2^-36 at most below, with fp32 queries 22 bits down to 2^-17 and 2^-39.  Measured with factors of
+    // 2^7 / 2^11 / 2^13 / 2^14 at 2048 rows of 40 heads of 128 over 2001 older tokens, append included: bf16 276 /
+    // 279 / 283 / 285 us (O moves more often), fp32 477 at all four.
+    static constexpr float slack = TERMS == 2 ? 1.0f : 4.0f, boost = TERMS == 2 ? 16384.0f : 2048.0f;
 };
 
 __device__ __forceinline__ void tc_mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -219,8 +223,8 @@ kv8_prompt_kernel(const AttnParams p) {
         const uint32_t lanes = (uint32_t)(32 * warp) << 16;
         float m = -INFINITY, l = 0.0f;            // reference of the weights, their sum
         // largest v scale that the row has seen and its reciprocal (a later row's would cost an earlier
-        // one bits of its weights); 2^-119 stands for less
-        float vref = PT_BOOST * FLT_MIN, vinv = 1.0f / FLT_MIN;        // (the reciprocal times PT_BOOST)
+        // one bits of its weights); 2^-126 times the weights' factor stands for less
+        float vref = L::boost * FLT_MIN, vinv = 1.0f / FLT_MIN;        // (the reciprocal times L::boost)
         for (int j = 0; j < steps && ok; ++j) {
             const int b = j & 1, kk = j * PT_KEYS;
             const uint32_t ph = (uint32_t)((j >> 1) & 1);
@@ -262,13 +266,13 @@ kv8_prompt_kernel(const AttnParams p) {
                     mx = fmaxf(mx, x * ks[2 * hh + u]);
                 }
             }
-            // O moves to new references only where a row's maximum has passed its own by 2^8, or for
+            // O moves to new references only where a row's maximum has passed its own by 2^slack, or for
             // a larger v scale
-            if (__any_sync(0xffffffffu, mx > m + PT_SLACK || vtop > vref)) {
-                if (vtop > vref) vinv = PT_BOOST / vtop;
-                const float vdown = vtop > vref ? vref * vinv * (1.0f / PT_BOOST) : 1.0f;
+            if (__any_sync(0xffffffffu, mx > m + L::slack || vtop > vref)) {
+                if (vtop > vref) vinv = L::boost / vtop;
+                const float vdown = vtop > vref ? vref * vinv * (1.0f / L::boost) : 1.0f;
                 vref = vtop;
-                const float to = mx > m + PT_SLACK ? mx : m;
+                const float to = mx > m + L::slack ? mx : m;
                 float down = to == -INFINITY ? 1.0f : ex2(m - to);
                 m = to;
                 l *= down;
@@ -306,7 +310,7 @@ kv8_prompt_kernel(const AttnParams p) {
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     const float c = ks[2 * hh + u], v = vs[2 * hh + u];
-                    const float w = v == vref ? PT_BOOST : v * vinv;
+                    const float w = v == vref ? L::boost : v * vinv;
 #pragma unroll
                     for (int i = 16 * u; i < 16 * u + 16; i += 2) {
                         const float e0 = ex2(fmaf(s[i], c, -mu)), e1 = ex2(fmaf(s[i + 1], c, -mu));
@@ -330,7 +334,7 @@ kv8_prompt_kernel(const AttnParams p) {
             const int b = (steps - 1) & 1;
             if (!__all_sync(0xffffffffu, mbar_wait(pv_done(b), (uint32_t)(((steps - 1) >> 1) & 1), abort_flag))) fail();
             tc_fence_after();
-            const float inv = 1.0f / (l * PT_BOOST);
+            const float inv = 1.0f / (l * L::boost);
             T *dst = static_cast<T *>(p.out) + row * p.ldo + (int64_t)head * D;
             const bool vec = (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
 #pragma unroll 1

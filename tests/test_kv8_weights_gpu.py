@@ -10,7 +10,8 @@ element of a query is not zero, so a score is an exact product times a scale.
  * its rounding to fp16: 2^-11 for 16-bit queries, 2^-22 for the two terms of fp32 queries;
  * sums in binary32: 64 steps of 2 u, and 8 u for the merge and the division.
 What lies below fp16's normal numbers is off by half their spacing, 2^-25, before the factor that the weights
-carry: 2^15 (with a second term: 2^26).  That is floor_of() times the largest |v| for every key.  Outputs are rounded once to their type (fp16 below
+carry: 2^15 for up to 8 and 16 pairs (with a second term: 2^26), 2^11 for prompts (fp32 queries: 2^14).
+That is floor_of() times the largest |v| for every key.  Outputs are rounded once to their type (fp16 below
 2^-14: 2^-25)."""
 import numpy as np
 import pytest
@@ -24,14 +25,16 @@ from tests.test_quant8_gpu import U, Cache, ctx, dev, half_step  # noqa: E402
 
 __all__ = ["ctx"]
 
-# heads, kv heads, rows: up to 8 pairs a tile, 16 pairs a tile; with 448 tiles the keys are not split, so
-# that every warp walks several steps of them
-FORMS = {"pairs8": (8, 1, 1), "pairs8_heads": (4, 4, 2), "pairs16": (8, 1, 3),
+# heads, kv heads, rows: up to 8 pairs a tile, 16 pairs a tile, 128 (32 tiles of half a tile at least); with
+# 448 tiles the keys are not split, so that every warp walks several steps of them
+FORMS = {"pairs8": (8, 1, 1), "pairs8_heads": (4, 4, 2), "pairs16": (8, 1, 3), "prompt": (32, 32, 64),
          "pairs8_whole": (448, 448, 1), "pairs16_whole": (448, 448, 9)}
 S, BLOCK = 700, 64
 
 
-def floor_of(dtype):
+def floor_of(form, dtype):
+    if form == "prompt":
+        return 2.0 ** -39 if dtype == "f32" else 2.0 ** -36
     return 2.0 ** -51 if dtype == "f32" else 2.0 ** -40
 
 
@@ -58,7 +61,7 @@ def check(ctx, form, dtype, code, D, scores, values):
     ref, mag = w @ val["v"], w @ np.abs(val["v"])
     s2 = 1.4427 * scores.max() * 2
     rel = 10 * U * s2 + 2.0 ** -21 + 4 * U + (2.0 ** -22 if dtype == "f32" else 2.0 ** -11) + (128 + 8) * U
-    tol = np.abs(ref) * half_step(dtype) + rel * mag + S * floor_of(dtype) * np.abs(val["v"]).max()
+    tol = np.abs(ref) * half_step(dtype) + rel * mag + S * floor_of(form, dtype) * np.abs(val["v"]).max()
     if dtype == "f16":
         tol = tol + 2.0 ** -25
     off = np.abs(got - ref)
