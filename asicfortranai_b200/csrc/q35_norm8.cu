@@ -14,9 +14,14 @@
 // the codes are round(y' (Q / max |y'|)) -- f cancels -- and f enters the scale alone, so a code
 // sees fewer roundings than y / scale has, and no division per element.
 //
-// Measured: 4099 rows of 5120 in bf16 with the residual and its sum 27 us (147 MB, 5.4 TB/s; a
+// A row with an element that is no number, or with squares next to the ends of binary32's range, takes a
+// path of its own (far_row): NaN scales in every group, or the row's codes with the sum of squares taken
+// once more behind a power of two.
+//
+// Measured: 4099 rows of 5120 in bf16 with the residual and its sum 28 us (147 MB, 5.2 TB/s; a
 // copy reaches 6.5); one row of 8192 6.5 us a call back to back, which is the host's time.
 #include <algorithm>
+#include <cfloat>
 #include <cstring>
 
 #include "q35_q8.cuh"
@@ -38,7 +43,7 @@ struct Norm8Params {
     bool vec;                      // rows start on vector boundaries and dim is a multiple of V
 };
 
-// the larger of a and b, NaN if either is: a row with a NaN or infinite element gets NaN scales
+// the larger of a and b, NaN if either is
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -76,13 +81,86 @@ __device__ __forceinline__ uint4 load_chunk(const T *p, int i, int dim) {
     return u;
 }
 
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+__device__ __forceinline__ float warp_max_nan(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
+// One row, read from memory again in every pass: the largest element, then the sum of squares behind the
+// power of two that brings it next to 1 (eps with it), then codes by groups of 128 elements, a warp each.
+// All threads of the CTA call it, behind the loop over the rows (within it, in line or as a call, it cost
+// that loop registers: 30.5 us at 4099 rows of 5120 in bf16, 28.4 here, 27.5 without it).
+template <typename T, int CODE, bool ROW>
+__device__ __forceinline__ void far_row(const Norm8Params &p, int64_t row, float (*part)[32]) {
+    constexpr float Q = code_max<CODE>();
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, nw = blockDim.x >> 5;
+    const T *x = static_cast<const T *>(p.x) + row * p.ldx;
+    const T *r = static_cast<const T *>(p.res) + (p.res ? row * p.ldr : 0);
+    T *ro = static_cast<T *>(p.res_out) + (p.res_out ? row * p.ldo : 0);
+    uint8_t *q = p.q + row * p.ldq;
+    auto sum = [&](int i) { return p.res ? to_f32<T>(x[i]) + to_f32<T>(r[i]) : to_f32<T>(x[i]); };
+    auto over_cta = [&](float v, int slot, auto join) {
+        v = join(v);
+        __syncthreads();
+        if (lane == 0) part[slot][warp] = v;
+        __syncthreads();
+        return join(lane < nw ? part[slot][lane] : 0.0f);
+    };
+    float m = 0.0f, ss = 0.0f, top = 0.0f;
+#pragma unroll 1
+    for (int i = t; i < p.dim; i += blockDim.x) m = max_nan(m, fabsf(sum(i)));
+    m = over_cta(m, 0, warp_max_nan);
+    const int e = max(-126, min(126, (int)(__float_as_uint(fmaxf(m, sqrtf(p.eps))) >> 23) - 127));
+    const float by = m <= FLT_MAX ? __uint_as_float((uint32_t)(127 - e) << 23) : NAN;   // (NaN for the whole row)
+#pragma unroll 1
+    for (int i = t; i < p.dim; i += blockDim.x) {
+        const float y = sum(i) * by;
+        ss = fmaf(y, y, ss);
+    }
+    ss = over_cta(ss, 1, warp_sum);
+    const float f = rsqrtf(fmaf(ss, p.inv_dim, p.eps * by * by));       // 1/rms = by f
+    if (ROW) {
+#pragma unroll 1
+        for (int i = t; i < p.dim; i += blockDim.x) top = max_nan(top, fabsf(sum(i) * by * p.w[i]));
+        top = over_cta(top, 0, warp_max_nan);
+    }
+#pragma unroll 1
+    for (int g = warp; g * Q8_BLOCK < p.dim; g += nw) {
+        float y[Q8_BLOCK / 32], amax = top;
+#pragma unroll
+        for (int j = 0; j < Q8_BLOCK / 32; ++j) {
+            const int i = g * Q8_BLOCK + 32 * j + lane;
+            y[j] = 0.0f;
+            if (i < p.dim) {
+                const float h = sum(i);
+                y[j] = h * by * p.w[i];
+                if (p.res_out) ro[i] = from_f32<T>(h);
+            }
+            if (!ROW) amax = max_nan(amax, fabsf(y[j]));
+        }
+        if (!ROW) amax = warp_max_nan(amax);
+        if (lane == 0 && (!ROW || g == 0)) p.scales[row * p.groups + g] = amax * f * (1.0f / Q);
+#pragma unroll
+        for (int j = 0; j < Q8_BLOCK / 32; ++j) {
+            const int i = g * Q8_BLOCK + 32 * j + lane;
+            if (i < p.dim) q[i] = encode8<CODE>(amax > 0.0f ? __fdiv_rn(y[j], __fdiv_rn(amax, Q)) : amax);
+        }
+    }
+}
+
 // NC chunks per thread: thread t's chunk c covers elements (c * blockDim + t) * V ...  A CTA takes
 // rows blockIdx, blockIdx + gridDim, ...; the next row's loads are issued before this row's
 // barrier, so that memory is busy through the reductions.  MT: the largest CTA, MB: CTAs an
 // SM should hold.  WS: the weights stand in shared memory (CTAs of several rows), four floats of
 // every chunk in a plane.
 template <typename T, int CODE, int NC, bool ROW, bool VEC, bool WS, int MT, int MB>
-__global__ void __launch_bounds__(MT, MB) norm8_kernel(const Norm8Params p) {
+__global__ void __launch_bounds__(MT, MB) norm8_kernel(const __grid_constant__ Norm8Params p) {
     constexpr int V = 16 / sizeof(T);
     constexpr int LANES = Q8_BLOCK / V;       // lanes of a group of 128: 32 (fp32) or 16
     constexpr float Q = code_max<CODE>();
@@ -115,13 +193,12 @@ __global__ void __launch_bounds__(MT, MB) norm8_kernel(const Norm8Params p) {
                 if (ch < chunks) weights[j * chunks + ch] = *reinterpret_cast<const float4 *>(p.w + ch * V + 4 * j);
         }
     }
+    bool any_far = false;
     for (int par = 0; row < p.rows; par ^= 1) {
         float h[NC][V];
         float ss = 0.0f;
-        T *ro = static_cast<T *>(p.res_out) + (p.res_out ? row * p.ldo : 0);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const int i = (c * blockDim.x + t) * V;
             const Chunk<T, V> x = chunk_of<T, V>(nx[c]);
 #pragma unroll
             for (int j = 0; j < V; ++j) h[c][j] = to_f32<T>(x.e[j]);
@@ -132,7 +209,25 @@ __global__ void __launch_bounds__(MT, MB) norm8_kernel(const Norm8Params p) {
             }
 #pragma unroll
             for (int j = 0; j < V; ++j) ss = fmaf(h[c][j], h[c][j], ss);
-            if (p.res_out) {
+        }
+        const int64_t next = row + gridDim.x;
+        if (next < p.rows) fetch(next);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (lane == 0) part[par][0][warp] = ss;
+        __syncthreads();
+        float tot = lane < nw ? part[par][0][lane] : 0.0f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) tot += __shfl_xor_sync(0xffffffffu, tot, o);
+        const float mean = fmaf(tot, p.inv_dim, p.eps);
+        // a row for far_row: marked in its first scale; what else is written of it here is written again
+        const bool far = !(tot < INFINITY) || mean < 0x1p-100f;
+        any_far |= far;
+        if (p.res_out && !far) {              // (not before: far_row reads the inputs, which this may be)
+            T *ro = static_cast<T *>(p.res_out) + row * p.ldo;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const int i = (c * blockDim.x + t) * V;
                 Chunk<T, V> o;
 #pragma unroll
                 for (int j = 0; j < V; ++j) o.e[j] = from_f32<T>(h[c][j]);
@@ -145,17 +240,7 @@ __global__ void __launch_bounds__(MT, MB) norm8_kernel(const Norm8Params p) {
                 }
             }
         }
-        const int64_t next = row + gridDim.x;
-        if (next < p.rows) fetch(next);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (lane == 0) part[par][0][warp] = ss;
-        __syncthreads();
-        float tot = lane < nw ? part[par][0][lane] : 0.0f;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) tot += __shfl_xor_sync(0xffffffffu, tot, o);
-        const float inv = rsqrtf(fmaf(tot, p.inv_dim, p.eps));      // within 2 ulp
-        // (0 and infinity, of infinite and of all-zero rows without eps, stay as they are)
+        const float inv = rsqrtf(mean);      // within 2 ulp
         const float pow2 = __uint_as_float(__float_as_uint(inv) & 0x7f800000u);
         const float f = __uint_as_float((__float_as_uint(inv) & 0x007fffffu) | 0x3f800000u);
 
@@ -209,7 +294,7 @@ __global__ void __launch_bounds__(MT, MB) norm8_kernel(const Norm8Params p) {
             const int i = (c * blockDim.x + t) * V;
             if (i >= p.dim) continue;
             const int g = ROW ? 0 : i / Q8_BLOCK;
-            if (ROW ? i == 0 : (i % Q8_BLOCK) == 0) p.scales[row * p.groups + g] = amax[c] * f * (1.0f / Q);
+            if (ROW ? i == 0 : (i % Q8_BLOCK) == 0) p.scales[row * p.groups + g] = far ? -1.0f : amax[c] * f * (1.0f / Q);
             uint32_t b[V / 4];
             if (amax[c] < 1e-30f) {                    // Q / amax would overflow (0: codes 0)
                 const float s = __fdiv_rn(amax[c], Q);
@@ -233,6 +318,11 @@ __global__ void __launch_bounds__(MT, MB) norm8_kernel(const Norm8Params p) {
             }
         }
         row = next;
+    }
+    if (any_far) {
+        __syncthreads();                      // (the marks of thread 0)
+        for (row = blockIdx.x; row < p.rows; row += gridDim.x)
+            if (p.scales[row * p.groups] == -1.0f) far_row<T, CODE, ROW>(p, row, part[0]);
     }
 }
 

@@ -250,7 +250,8 @@ int q35_sample_filtered_dev(q35_ctx ctx, int dtype, const void *logits, int64_t 
  *   (may be NULL; may be x or residual themselves);
  *   y = h / sqrt(mean(h^2) + eps) * weight;
  *   scales[row][g] = max |y| over group g / (127 or 448), q = the code nearest to y / scale
- *   (ties to even; scale 0: codes 0).  A row with a NaN or infinite element gets NaN scales.
+ *   (ties to even; scale 0: codes 0).  A row of h with a NaN or infinite element gets NaN
+ *   scales in all its groups.
  * x, residual, residual_out: dtype, [rows] of dim elements ldx, ldr, ldo apart; q: codes, ldq
  * apart; weight fp32 [dim]; group: 128 elements (scales [rows][ceil(dim/128)], the x_scales of
  * q35_fp8_gemm_dev) or 0, the whole row (scales [rows]).  dim <= 32768. */
