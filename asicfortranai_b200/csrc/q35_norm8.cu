@@ -351,7 +351,16 @@ int launch_norm8(const Norm8Params &p, cudaStream_t s) {
            : nc == 2 ? norm8_kernel<T, CODE, 2, ROW, VEC, VEC, 512, 2>
                      : norm8_kernel<T, CODE, 4, ROW, VEC, VEC, 512, 1>;
     const size_t smem = VEC ? (size_t)p.dim * 4 : 0;
-    if (smem > 48 * 1024) Q35_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (smem > 48 * 1024) {
+        // the limit is the function's, for every call of the process: the largest row of this branch, once
+        static bool configured[64] = {};
+        int dev = 0;
+        Q35_CUDA_TRY(cudaGetDevice(&dev));
+        if (dev < 0 || dev >= 64 || !configured[dev]) {
+            Q35_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * 512 * V * 4));
+            if (dev >= 0 && dev < 64) configured[dev] = true;
+        }
+    }
     int per = 0;                                   // resident CTAs per SM
     Q35_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kern, threads, smem));
     const int grid = (int)std::min<int64_t>(p.rows, (int64_t)std::max(1, per) * 148);

@@ -1,5 +1,7 @@
 """RMSNorm with 8-bit output at the edges of binary32: rows with elements that are no numbers, rows whose
 squares leave the range.  Tolerances are those of tests/test_quant8_gpu.py."""
+import threading
+
 import numpy as np
 import pytest
 
@@ -86,3 +88,40 @@ def test_sums_that_pass_the_range_are_infinite(ctx):
     h, q, s = norm(ctx, x, x, w, "f32", "int8", 128)
     assert torch.isnan(s[[0, 2]]).all() and (s[1] > 0).all()
     assert (decode(q[1].cpu().numpy(), "int8") == 127).all()
+
+
+def test_two_threads_with_rows_of_different_length():
+    """Two contexts of one process, rows whose weights take 64 and 52 KB of shared memory."""
+    from asicfortranai_b200 import quant8
+    from asicfortranai_b200.quantized import Context
+    rows = 152
+    jobs = []
+    for dim in (16384, 13312):
+        c = Context(0)
+        x = torch.randn(rows, dim, device="cuda").bfloat16()
+        w = torch.ones(dim, device="cuda")
+        q = torch.zeros(rows, dim, dtype=torch.uint8, device="cuda")
+        s = torch.zeros(rows, dim // 128, device="cuda")
+        jobs.append((c, x, w, q, s, dim))
+    torch.cuda.synchronize()
+    failed = []
+
+    def go(c, x, w, q, s, dim):
+        try:
+            for i in range(3000):
+                quant8.rms_norm_quant(c, x.data_ptr(), w.data_ptr(), q.data_ptr(), s.data_ptr(), rows, dim)
+                if i % 100 == 99:
+                    c.synchronize()
+        except Exception as e:      # noqa: BLE001  (raised in the thread: reported by the test)
+            failed.append((dim, i, str(e)))
+
+    threads = [threading.Thread(target=go, args=j) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+    for c, x, w, q, s, dim in jobs:
+        c.synchronize()
+        check_norm(x, None, w, x, q.cpu().numpy(), s, "bf16", "e4m3", 128)
+        c.close()
