@@ -404,12 +404,12 @@ extern "C" int q35_rms_norm_quant_dev(q35_ctx ctx, int dtype, const void *x, int
         !aligned_to(scales, 4))
         return set_error(Q35_ERR_INVALID, "rms_norm_quant: a pointer is not aligned to its elements");
     // residual_out may be x or residual themselves (each thread reads its elements before it
-    // writes them); a shifted overlap would read sums
+    // writes them; one row has no stride); a shifted overlap would read sums
     if (residual_out) {
         auto overlaps = [&](const void *p, int64_t ld) {
             const char *a = static_cast<const char *>(p), *o = static_cast<const char *>(residual_out);
             const size_t na = ((size_t)(rows - 1) * ld + dim) * es, no = ((size_t)(rows - 1) * ldo + dim) * es;
-            return p && a < o + no && o < a + na && !(a == o && ld == ldo);
+            return p && a < o + no && o < a + na && !(a == o && (ld == ldo || rows == 1));
         };
         if (overlaps(x, ldx) || overlaps(residual, ldr))
             return set_error(Q35_ERR_INVALID, "rms_norm_quant: residual_out partly overlaps an input");

@@ -125,3 +125,18 @@ def test_two_threads_with_rows_of_different_length():
         c.synchronize()
         check_norm(x, None, w, x, q.cpu().numpy(), s, "bf16", "e4m3", 128)
         c.close()
+
+
+def test_one_row_in_place_whatever_the_strides(ctx):
+    """A single row has no stride that could make the sum's buffer another one than its input."""
+    from asicfortranai_b200 import quant8
+    dim = 640
+    x, r = (torch.randn(1, dim, device="cuda").bfloat16() for _ in "xr")
+    w = torch.ones(dim, device="cuda")
+    h, q, s = norm(ctx, x, r, w, "bf16", "e4m3", 128)
+    q2, s2 = torch.zeros_like(q), torch.zeros_like(s)
+    torch.cuda.synchronize()
+    quant8.rms_norm_quant(ctx, x.data_ptr(), w.data_ptr(), q2.data_ptr(), s2.data_ptr(), 1, dim, residual=r.data_ptr(),
+                          residual_out=r.data_ptr(), ldr=dim, ldo=4 * dim)
+    ctx.synchronize()
+    assert torch.equal(r, h) and torch.equal(q, q2) and torch.equal(s, s2)
