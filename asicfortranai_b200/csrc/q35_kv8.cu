@@ -1080,6 +1080,18 @@ int check_rows(const q35_kv8_cache &c, const Kv8Rows &r) {
     return Q35_OK;
 }
 
+int check_heads(const q35_kv8_cache &c, int32_t heads) {
+    if (heads < 1 || heads % c.kv_heads)
+        return set_error(Q35_ERR_INVALID, "kv8_attention: heads must be a multiple of kv_heads");
+    return Q35_OK;
+}
+// the kernels count a sequence's (row, head) pairs of a kv head in 32 bits
+int check_pairs(const q35_kv8_cache &c, int32_t heads, int32_t max_rows) {
+    if ((int64_t)max_rows * (heads / c.kv_heads) > INT32_MAX - 128)
+        return set_error(Q35_ERR_INVALID, "kv8_attention: max_rows * heads / kv_heads above 2^31 - 129");
+    return Q35_OK;
+}
+
 }  // namespace
 
 int kv8_check(const q35_kv8_cache *c) {
@@ -1129,7 +1141,7 @@ int launch_kv8_append(const q35_kv8_cache &c, int dtype, const void *k, const vo
 }
 
 size_t kv8_attention_workspace(const q35_kv8_cache &c, int32_t heads, int32_t rows, int32_t max_rows) {
-    if (rows <= 0) return 0;
+    if (rows <= 0 || kv8_prompt_takes(c, heads, max_rows)) return 0;
     const AttnPlan pl = attn_plan(c, heads, max_rows);
     return pl.ml_bytes + pl.o_bytes;
 }
@@ -1146,7 +1158,6 @@ int launch_kv8_attention(const q35_kv8_cache &c, int dtype, const void *q, int64
     if (r.rows == 0) return Q35_OK;
     const bool prompt = kv8_prompt_takes(c, heads, r.max_rows);
     const AttnPlan pl = attn_plan(c, heads, r.max_rows);
-    if (pl.mtiles > 65535) return set_error(Q35_ERR_INVALID, "kv8: too many rows in one call");
     AttnParams p;
     p.q = q; p.out = out; p.out_q = out_q;
     p.k = static_cast<const uint8_t *>(c.k); p.v = static_cast<const uint8_t *>(c.v);
@@ -1164,6 +1175,7 @@ int launch_kv8_attention(const q35_kv8_cache &c, int dtype, const void *q, int64
     p.err = err;
     const int zs = c.seqs * c.kv_heads;
     if (prompt) return launch_kv8_prompt(p, dtype, c.code, c.head_dim, zs, s);
+    // (tiles along grid.y: fewer than 32 of 128 pairs)
     switch (dtype) {
     case Q35_DT_F32: return launch_attn<float>(p, pl, c.code, c.head_dim, zs, s);
     case Q35_DT_BF16: return launch_attn<__nv_bfloat16>(p, pl, c.code, c.head_dim, zs, s);
@@ -1200,12 +1212,10 @@ int q35_kv8_append_dev(q35_ctx ctx, const q35_kv8_cache *cache, int dtype, const
 
 int64_t q35_kv8_attention_workspace(const q35_kv8_cache *cache, int32_t heads, int32_t rows, int32_t max_rows) {
     if (kv8_check(cache)) return -1;
-    if (heads < 1 || heads % cache->kv_heads) {
-        set_error(Q35_ERR_INVALID, "kv8_attention: heads must be a multiple of kv_heads");
-        return -1;
-    }
     const int32_t dummy = 0;
-    if (check_rows(*cache, Kv8Rows{&dummy, &dummy, rows, max_rows})) return -1;
+    if (check_heads(*cache, heads) || check_rows(*cache, Kv8Rows{&dummy, &dummy, rows, max_rows}) ||
+        check_pairs(*cache, heads, max_rows))
+        return -1;
     return (int64_t)kv8_attention_workspace(*cache, heads, rows, max_rows);
 }
 
@@ -1216,10 +1226,10 @@ int q35_kv8_attention_dev(q35_ctx ctx, const q35_kv8_cache *cache, int dtype, co
     int st = kv8_check(cache);
     if (!st) st = check_dtype(dtype);
     if (st) return st;
-    if (heads < 1 || heads % cache->kv_heads)
-        return set_error(Q35_ERR_INVALID, "kv8_attention: heads must be a multiple of kv_heads");
+    st = check_heads(*cache, heads);
     const Kv8Rows r{row_start, past, rows, max_rows};
-    st = check_rows(*cache, r);
+    if (!st) st = check_rows(*cache, r);
+    if (!st) st = check_pairs(*cache, heads, max_rows);
     if (st) return st;
     if (rows == 0) return Q35_OK;
     if (!q || !out) return set_error(Q35_ERR_INVALID, "kv8_attention: NULL argument");

@@ -302,7 +302,8 @@ int q35_kv8_append_dev(q35_ctx ctx, const q35_kv8_cache *cache, int dtype, const
  * over positions j up to the row's own.  q, out: dtype, [rows] of heads * head_dim elements, ldq
  * and ldo apart; heads a multiple of kv_heads.  workspace: device memory of
  * q35_kv8_attention_workspace bytes (16-byte aligned; may be NULL when that is 0), used by this
- * call alone while it runs.  Nothing behind a sequence's last token counts, whatever it holds. */
+ * call alone while it runs.  Nothing behind a sequence's last token counts, whatever it holds.
+ * max_rows * heads / kv_heads is at most 2^31 - 129. */
 int q35_kv8_attention_dev(q35_ctx ctx, const q35_kv8_cache *cache, int dtype, const void *q, int64_t ldq,
                           int32_t heads, void *out, int64_t ldo, const int32_t *row_start,
                           const int32_t *past, int32_t rows, int32_t max_rows, float scale,
