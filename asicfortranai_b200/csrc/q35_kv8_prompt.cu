@@ -13,11 +13,19 @@
 //     only when that has grown by 2^4 (fp32 queries: 2), so O is rarely moved; weights times the
 //     block's v scale over the largest one so far go back as fp16 into S's buffer, with a factor that
 //     spends fp16's range on small ones.
-// fp32 queries and their weights take two fp16 terms each (22 bits), with two MMAs for one.
+// fp32 queries and their weights take two fp16 terms each (22 bits), with two MMAs for one, the low terms
+// first.
 //
-// Sums and O are fp32.  Measured, 2048 rows of 40 heads of 128 over 2001 older tokens, bf16: 250 us
-// (75 are the operations at the fp16 rate), f32 about 445.  A CTA's step of 64 keys takes 3300
-// clocks, of which a softmax warp works 2000 (1500 of them on the weights: 16 exponentials a clock
+// Sums and O are fp32.  The tensor cores' additions do not round to nearest: each loses up to a bit of what
+// has been summed so far, always towards zero.  With 16-bit queries that is 7e-5 of an output over 20
+// thousand keys of like weight, below the outputs' own rounding (half a step of fp16: 4.9e-4).  With fp32
+// queries (1.4e-4: two products a key) P V adds up two steps at a time, in one of two buffers, and the
+// softmax warps add these to sums in registers, rounded; a head_dim of 256 is two CTAs then, 128 d of the
+// values each.
+//
+// Measured, 2048 rows of 40 heads of 128 over 2001 older tokens, bf16: 250 us (75 are the operations at
+// the fp16 rate), f32 555 (445 with all of O in the tensor cores' accumulators).  A CTA's step of 64 keys
+// (bf16) takes 3300 clocks, of which a softmax warp works 2000 (1500 of them on the weights: 16 exponentials a clock
 // and SM alone are 512 for each of the SM's two CTAs) and the tensor pipe is busy for 640.
 //
 // Waits are bounded as in q35_fp8.cu.
@@ -36,10 +44,19 @@ constexpr int PT_THREADS = 288;
 
 // TERMS: fp16 terms of a query element and of a weight (2 for fp32 queries: 22 bits)
 template <int TERMS, int D> struct Prompt {
-    static constexpr uint32_t Q = PT_ROWS * D * 2, K = PT_KEYS * D * 2, V = D * PT_KEYS * 2;   // Q: one term
+    // d of the values a CTA takes (fp32 queries of 256: two CTAs, each with all scores), and whether a group of
+    // steps' outputs is added up outside the tensor cores
+    static constexpr int DV = TERMS == 2 && D > 128 ? 128 : D;
+    static constexpr bool apart = TERMS == 2;
+    static constexpr int group = 2;                                    // steps that P V adds up in its accumulator
+    static constexpr uint32_t Q = PT_ROWS * D * 2, K = PT_KEYS * D * 2, V = DV * PT_KEYS * 2;  // Q: one term
     static constexpr int stages = TERMS * D > 256 ? 1 : 2;             // of K and V: what the memory takes
-    static constexpr int ctas = TERMS * D > 128 ? 1 : 2;               // per SM
-    static constexpr uint32_t tmem = D > 128 ? 512 : 256;              // columns: S 2 x 64, O
+    static constexpr int ctas = apart || D > 128 ? 1 : 2;              // per SM
+    // (sums outside the tensor cores take registers, which the converters give up: 232 + 96 of twice 168.  The
+    // issuer's warpgroup is filled up with idle warps, so that each is whole)
+    static constexpr int threads = apart ? 384 : PT_THREADS;
+    static constexpr int softmax_regs = 232, converter_regs = 96, launch_regs = (softmax_regs + converter_regs) / 2;
+    static constexpr uint32_t tmem = 128 + (apart ? 2 : 1) * DV > 256 ? 512 : 256;    // columns: S 2 x 64, O (2 of a step)
     static constexpr uint32_t off_k = TERMS * Q, off_v = off_k + stages * K, off_bar = off_v + stages * V;
     static constexpr size_t smem = 1024 + off_bar + 8 * 18 + 16 + 4 * 32;
     // A row's maximum may pass its reference by 2^slack, and the weights carry a factor `boost` in fp16:
@@ -96,11 +113,12 @@ __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.
 __device__ __forceinline__ uint32_t swz(int row, int chunk) { return (uint32_t)(row * 128 + ((chunk ^ (row & 7)) << 4)); }
 
 template <typename T, int CODE, int D>
-__global__ void __launch_bounds__(PT_THREADS, (Prompt<std::is_same<T, float>::value ? 2 : 1, D>::ctas))
+__global__ void __launch_bounds__((Prompt<std::is_same<T, float>::value ? 2 : 1, D>::threads), (Prompt<std::is_same<T, float>::value ? 2 : 1, D>::ctas))
 kv8_prompt_kernel(const AttnParams p) {
     constexpr int TERMS = std::is_same<T, float>::value ? 2 : 1;
     using L = Prompt<TERMS, D>;
-    constexpr int ST = L::stages;
+    constexpr int ST = L::stages, DV = L::DV;
+    const int d0 = DV < D ? (int)blockIdx.z * DV : 0;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     uint8_t *sbase = smem_raw + (base - raw);
@@ -153,6 +171,8 @@ kv8_prompt_kernel(const AttnParams p) {
     const int steps = (kend + PT_KEYS - 1) / PT_KEYS;                  // (0: nothing to do)
     const int64_t hb = seq * p.seq_stride + (int64_t)kvh * p.max_seq * D;
     const int64_t sb = seq * p.scale_seq_stride + (int64_t)kvh * p.nblk;
+    // where P V of step j adds up
+    auto o_at = [&](int j) { return 128u + (uint32_t)(L::apart ? j / L::group % 2 * DV : 0); };
     bool ok = true;
     auto fail = [&]() {
         ok = false;
@@ -162,6 +182,7 @@ kv8_prompt_kernel(const AttnParams p) {
 
     if (warp < 4) {
         // ---------------- Q, softmax, output: row `tid` of the tile ----------------
+        if constexpr (L::apart) regs_up<L::softmax_regs>();
         const int r = tid, f = f0 + r;
         const bool live = r < fn;
         const int lim = live ? sr.past + f / p.G + 1 : 0;
@@ -225,6 +246,26 @@ kv8_prompt_kernel(const AttnParams p) {
         // largest v scale that the row has seen and its reciprocal (a later row's would cost an earlier
         // one bits of its weights); 2^-126 times the weights' factor stands for less
         float vref = L::boost * FLT_MIN, vinv = 1.0f / FLT_MIN;        // (the reciprocal times L::boost)
+        float acc[L::apart ? DV : 1];             // outputs of the steps before the last one
+        if constexpr (L::apart) {
+#pragma unroll
+            for (int i = 0; i < DV; ++i) acc[i] = 0.0f;
+        }
+        // adds the outputs of the steps up to j, which are relative to the references that acc has
+        auto add_step = [&](int j) {
+            if (!__all_sync(0xffffffffu, mbar_wait(pv_done(j & 1), (uint32_t)((j >> 1) & 1), abort_flag))) { fail(); return; }
+            tc_fence_after();
+            if constexpr (L::apart) {
+#pragma unroll
+                for (int d = 0; d < DV; d += 32) {
+                    float o[32];
+                    tc_ld32(tmem + lanes + o_at(j) + (uint32_t)d, o);
+                    tc_wait_ld(o);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) acc[d + i] += o[i];
+                }
+            }
+        };
         for (int j = 0; j < steps && ok; ++j) {
             const int b = j & 1, kk = j * PT_KEYS;
             const uint32_t ph = (uint32_t)((j >> 1) & 1);
@@ -268,27 +309,32 @@ kv8_prompt_kernel(const AttnParams p) {
             }
             // O moves to new references only where a row's maximum has passed its own by 2^slack, or for
             // a larger v scale
+            float down = 1.0f;
             if (__any_sync(0xffffffffu, mx > m + L::slack || vtop > vref)) {
                 if (vtop > vref) vinv = L::boost / vtop;
                 const float vdown = vtop > vref ? vref * vinv * (1.0f / L::boost) : 1.0f;
                 vref = vtop;
                 const float to = mx > m + L::slack ? mx : m;
-                float down = to == -INFINITY ? 1.0f : ex2(m - to);
+                down = to == -INFINITY ? 1.0f : ex2(m - to);
                 m = to;
                 l *= down;
                 down *= vdown;
-                if (j > 0) {
+                if (L::apart ? j % L::group > 0 : j > 0) {
                     if (!__all_sync(0xffffffffu, mbar_wait(pv_done(b ^ 1), (uint32_t)(((j - 1) >> 1) & 1), abort_flag))) { fail(); break; }
                     tc_fence_after();
+                    constexpr int W = L::apart ? 16 : 32;              // (registers)
 #pragma unroll 1
-                    for (int d = 0; d < D; d += 32) {
-                        float o[32];
-                        uint32_t w[32];
-                        tc_ld32(tmem + lanes + 128u + (uint32_t)d, o);
+                    for (int d = 0; d < DV; d += W) {
+                        float o[W];
+                        uint32_t w[W];
+                        const uint32_t at = tmem + lanes + o_at(j) + (uint32_t)d;
+                        if constexpr (W == 16) tc_ld16(at, o);
+                        else tc_ld32(at, o);
                         tc_wait_ld(o);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(o[i] * down);
-                        tc_st32(tmem + lanes + 128u + (uint32_t)d, w);
+                        for (int i = 0; i < W; ++i) w[i] = __float_as_uint(o[i] * down);
+                        if constexpr (W == 16) tc_st16(at, w);
+                        else tc_st32(at, w);
                     }
                     tc_wait_st();
                 }
@@ -300,6 +346,7 @@ kv8_prompt_kernel(const AttnParams p) {
                 // columns of high terms, then 16 of low ones)
                 float s[32];
                 uint32_t pk[16], pl[TERMS == 2 ? 16 : 1];
+                float sum = 0.0f;                                      // (of 32: l takes two additions a step)
                 tc_ld32(tmem + lanes + (uint32_t)(64 * b + 32 * hh), s);
                 tc_wait_ld(s);
                 if (edge) {
@@ -314,7 +361,7 @@ kv8_prompt_kernel(const AttnParams p) {
 #pragma unroll
                     for (int i = 16 * u; i < 16 * u + 16; i += 2) {
                         const float e0 = ex2(fmaf(s[i], c, -mu)), e1 = ex2(fmaf(s[i + 1], c, -mu));
-                        l += e0 + e1;
+                        sum += e0 + e1;
                         pk[i / 2] = pack2<__half>(e0 * w, e1 * w);
                         if constexpr (TERMS == 2) {
                             const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&pk[i / 2]));
@@ -322,6 +369,7 @@ kv8_prompt_kernel(const AttnParams p) {
                         }
                     }
                 }
+                l += sum;
                 tc_st16(tmem + lanes + (uint32_t)(64 * b + 32 * hh), pk);
                 if constexpr (TERMS == 2) tc_st16(tmem + lanes + (uint32_t)(64 * b + 32 * hh + 16), pl);
             }
@@ -329,20 +377,32 @@ kv8_prompt_kernel(const AttnParams p) {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(p_full(b));
+            if constexpr (L::apart) {
+                // (P V does not come back to the buffer before the next arrivals on p_full)
+                if (j > 0 && j % L::group == 0) add_step(j - 1);
+                if (__any_sync(0xffffffffu, down != 1.0f)) {
+#pragma unroll
+                    for (int i = 0; i < DV; ++i) acc[i] *= down;
+                }
+            }
         }
         if (steps > 0 && ok) {
-            const int b = (steps - 1) & 1;
-            if (!__all_sync(0xffffffffu, mbar_wait(pv_done(b), (uint32_t)(((steps - 1) >> 1) & 1), abort_flag))) fail();
-            tc_fence_after();
+            add_step(steps - 1);
             const float inv = 1.0f / (l * L::boost);
-            T *dst = static_cast<T *>(p.out) + row * p.ldo + (int64_t)head * D;
+            T *dst = static_cast<T *>(p.out) + row * p.ldo + (int64_t)head * D + d0;
             const bool vec = (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
-#pragma unroll 1
-            for (int d = 0; d < D && ok; d += 32) {
+#pragma unroll(L::apart ? DV / 32 : 1)
+            for (int d = 0; d < DV; d += 32) {
                 float o[32];
-                __syncwarp();
-                tc_ld32(tmem + lanes + 128u + (uint32_t)d, o);
-                tc_wait_ld(o);
+                if (!ok) break;
+                if constexpr (L::apart) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = acc[d + i];
+                } else {
+                    __syncwarp();
+                    tc_ld32(tmem + lanes + 128u + (uint32_t)d, o);
+                    tc_wait_ld(o);
+                }
                 if (!live) continue;
 #pragma unroll
                 for (int i = 0; i < 32; ++i) o[i] = o[i] * inv * vref;
@@ -352,7 +412,7 @@ kv8_prompt_kernel(const AttnParams p) {
                     for (int i = 0; i < 8; ++i)
                         c[i] = (uint32_t)(uint8_t)quant127(o[4 * i]) | (uint32_t)(uint8_t)quant127(o[4 * i + 1]) << 8 |
                                (uint32_t)(uint8_t)quant127(o[4 * i + 2]) << 16 | (uint32_t)(uint8_t)quant127(o[4 * i + 3]) << 24;
-                    uint4 *dq = reinterpret_cast<uint4 *>(p.out_q + (row * p.H + head) * D + d);
+                    uint4 *dq = reinterpret_cast<uint4 *>(p.out_q + (row * p.H + head) * D + d0 + d);
                     dq[0] = make_uint4(c[0], c[1], c[2], c[3]);
                     dq[1] = make_uint4(c[4], c[5], c[6], c[7]);
                 } else if (vec) {
@@ -372,107 +432,110 @@ kv8_prompt_kernel(const AttnParams p) {
                 }
             }
         }
-    } else if (warp < 6) {
-        // ---------------- K: fp16 rows ----------------
-        // D / 16 neighbouring lanes take a key's row (whole lines); a thread has D / 16 pieces of 16 codes
-        constexpr int LK = D / 16, KR = 64 / LK;                     // lanes per key, keys per round of 64 threads
-        const int t = tid - 128, ch = t % LK, key0 = t / LK;
-        const uint8_t *kb = p.k + hb + 16 * ch;
-        uint4 c[LK];
-        auto load = [&](int j) {
-#pragma unroll
-            for (int i = 0; i < LK; ++i) c[i] = ldg16(kb + (int64_t)min(j * PT_KEYS + KR * i + key0, kend - 1) * D);
-        };
-        // lanes 0..3 of warp 4 the step's k scales, 4..7 its v scales
-        const float *sp = (t < 4 ? p.ks : p.vs) + sb;
-        float sc = 0.0f;
-        auto load_scale = [&](int j) {
-            const int key = j * PT_KEYS + 16 * (t & 3);
-            sc = 0.0f;
-            if (t < 8 && key < kend) sc = ldg(sp + (key >> p.block_shift));
-        };
-        if (steps > 0) { load(0); load_scale(0); }
-        for (int j = 0; j < steps && ok; ++j) {
-            const int b = j % ST;
-            if (!__all_sync(0xffffffffu, mbar_wait(k_empty(b), (uint32_t)((j / ST) & 1) ^ 1u, abort_flag))) { fail(); break; }
-            const uint32_t dst = base + L::off_k + (uint32_t)b * L::K;
-            const uint32_t blk = dst + (uint32_t)(ch / 4) * (PT_KEYS * 128);
-            const int odd = (ch / 4) & 1;                            // (neighbouring 64-d blocks' lanes write the
-#pragma unroll                                                       // halves in opposite order: no bank conflicts)
-            for (int i = 0; i < LK; ++i) {
-                uint4 x, y;
-                codes_f16<CODE>(c[i].x, x.x, x.y);
-                codes_f16<CODE>(c[i].y, x.z, x.w);
-                codes_f16<CODE>(c[i].z, y.x, y.y);
-                codes_f16<CODE>(c[i].w, y.z, y.w);
-                const int key = KR * i + key0;
-                st_shared16(blk + swz(key, 2 * (ch % 4) + odd), odd ? y : x);
-                st_shared16(blk + swz(key, 2 * (ch % 4) + 1 - odd), odd ? x : y);
-            }
-            if (t < 8) scales[8 * (j & 3) + t] = sc;
-            if (j + 1 < steps) { load(j + 1); load_scale(j + 1); }
-            fence_async();
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(k_full(b));
-                if (warp == 4) mbar_arrive(sc_full(j & 3));
-            }
-        }
     } else if (warp < 8) {
-        // ---------------- V: fp16, transposed ----------------
-        constexpr int VG = D > 128 ? D / 128 : 1;                    // pieces of 16 d x 8 keys a thread
-        const int t = tid - 192, kg = t & 7, dg0 = t >> 3;           // keys 8 kg .., d 16 dg .. (8 groups, D / 16 in all)
-        const uint8_t *vb = p.v + hb + 16 * dg0;
-        uint4 c[VG][8];
-        const bool live = dg0 < D / 16;
-        auto load = [&](int j) {
+        if constexpr (L::apart) regs_down<L::converter_regs>();
+        if (warp < 6) {
+            // ---------------- K: fp16 rows ----------------
+            // D / 16 neighbouring lanes take a key's row (whole lines); a thread has D / 16 pieces of 16 codes
+            constexpr int LK = D / 16, KR = 64 / LK;                     // lanes per key, keys per round of 64 threads
+            const int t = tid - 128, ch = t % LK, key0 = t / LK;
+            const uint8_t *kb = p.k + hb + 16 * ch;
+            uint4 c[LK];
+            auto load = [&](int j) {
 #pragma unroll
-            for (int g = 0; g < VG; ++g)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) c[g][i] = ldg16(vb + 128 * g + (int64_t)min(j * PT_KEYS + 8 * kg + i, kend - 1) * D);
-        };
-        if (steps > 0 && live) load(0);
-        for (int j = 0; j < steps && ok; ++j) {
-            const int b = j % ST;
-            // the stage is free: P V of step j - ST
-            if (j >= ST && !__all_sync(0xffffffffu, mbar_wait(pv_done((j - ST) & 1), (uint32_t)((j - ST) >> 1) & 1u, abort_flag))) { fail(); break; }
-            if (live) {
-                // past the last key: whatever is stored there must not count
-                if ((j + 1) * PT_KEYS > kend) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (j * PT_KEYS + 8 * kg + i >= kend) {
-#pragma unroll
-                            for (int g = 0; g < VG; ++g) c[g][i] = make_uint4(0u, 0u, 0u, 0u);
-                        }
+                for (int i = 0; i < LK; ++i) c[i] = ldg16(kb + (int64_t)min(j * PT_KEYS + KR * i + key0, kend - 1) * D);
+            };
+            // lanes 0..3 of warp 4 the step's k scales, 4..7 its v scales
+            const float *sp = (t < 4 ? p.ks : p.vs) + sb;
+            float sc = 0.0f;
+            auto load_scale = [&](int j) {
+                const int key = j * PT_KEYS + 16 * (t & 3);
+                sc = 0.0f;
+                if (t < 8 && key < kend) sc = ldg(sp + (key >> p.block_shift));
+            };
+            if (steps > 0) { load(0); load_scale(0); }
+            for (int j = 0; j < steps && ok; ++j) {
+                const int b = j % ST;
+                if (!__all_sync(0xffffffffu, mbar_wait(k_empty(b), (uint32_t)((j / ST) & 1) ^ 1u, abort_flag))) { fail(); break; }
+                const uint32_t dst = base + L::off_k + (uint32_t)b * L::K;
+                const uint32_t blk = dst + (uint32_t)(ch / 4) * (PT_KEYS * 128);
+                const int odd = (ch / 4) & 1;                            // (neighbouring 64-d blocks' lanes write the
+#pragma unroll                                                       // halves in opposite order: no bank conflicts)
+                for (int i = 0; i < LK; ++i) {
+                    uint4 x, y;
+                    codes_f16<CODE>(c[i].x, x.x, x.y);
+                    codes_f16<CODE>(c[i].y, x.z, x.w);
+                    codes_f16<CODE>(c[i].z, y.x, y.y);
+                    codes_f16<CODE>(c[i].w, y.z, y.w);
+                    const int key = KR * i + key0;
+                    st_shared16(blk + swz(key, 2 * (ch % 4) + odd), odd ? y : x);
+                    st_shared16(blk + swz(key, 2 * (ch % 4) + 1 - odd), odd ? x : y);
                 }
-                const uint32_t dst = base + L::off_v + (uint32_t)b * L::V;
-                auto word = [&](const uint4 &u, int w) { return w == 0 ? u.x : w == 1 ? u.y : w == 2 ? u.z : u.w; };
+                if (t < 8) scales[8 * (j & 3) + t] = sc;
+                if (j + 1 < steps) { load(j + 1); load_scale(j + 1); }
+                fence_async();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(k_full(b));
+                    if (warp == 4) mbar_arrive(sc_full(j & 3));
+                }
+            }
+        } else {
+            // ---------------- V: fp16, transposed ----------------
+            constexpr int VG = DV > 128 ? DV / 128 : 1;                    // pieces of 16 d x 8 keys a thread
+            const int t = tid - 192, kg = t & 7, dg0 = t >> 3;           // keys 8 kg .., d 16 dg .. (8 groups, DV / 16 in all)
+            const uint8_t *vb = p.v + hb + d0 + 16 * dg0;
+            uint4 c[VG][8];
+            const bool live = dg0 < DV / 16;
+            auto load = [&](int j) {
 #pragma unroll
                 for (int g = 0; g < VG; ++g)
 #pragma unroll
-                    for (int w = 0; w < 4; ++w)
+                    for (int i = 0; i < 8; ++i) c[g][i] = ldg16(vb + 128 * g + (int64_t)min(j * PT_KEYS + 8 * kg + i, kend - 1) * D);
+            };
+            if (steps > 0 && live) load(0);
+            for (int j = 0; j < steps && ok; ++j) {
+                const int b = j % ST;
+                // the stage is free: P V of step j - ST
+                if (j >= ST && !__all_sync(0xffffffffu, mbar_wait(pv_done((j - ST) & 1), (uint32_t)((j - ST) >> 1) & 1u, abort_flag))) { fail(); break; }
+                if (live) {
+                    // past the last key: whatever is stored there must not count
+                    if ((j + 1) * PT_KEYS > kend) {
 #pragma unroll
-                        for (int hh = 0; hh < 2; ++hh) {
-                            uint4 x, y;                               // d = 16 dg + 4 w + 2 hh, and the next
-                            const uint32_t sel = hh ? 0x7362 : 0x5140;
-                            codes_f16<CODE>(__byte_perm(word(c[g][0], w), word(c[g][1], w), sel), x.x, y.x);
-                            codes_f16<CODE>(__byte_perm(word(c[g][2], w), word(c[g][3], w), sel), x.y, y.y);
-                            codes_f16<CODE>(__byte_perm(word(c[g][4], w), word(c[g][5], w), sel), x.z, y.z);
-                            codes_f16<CODE>(__byte_perm(word(c[g][6], w), word(c[g][7], w), sel), x.w, y.w);
-                            const int d = 16 * (dg0 + 8 * g) + 4 * w + 2 * hh;
-                            st_shared16(dst + swz(d, kg), x);
-                            st_shared16(dst + swz(d + 1, kg), y);
-                        }
-                if (j + 1 < steps) load(j + 1);
+                        for (int i = 0; i < 8; ++i)
+                            if (j * PT_KEYS + 8 * kg + i >= kend) {
+#pragma unroll
+                                for (int g = 0; g < VG; ++g) c[g][i] = make_uint4(0u, 0u, 0u, 0u);
+                            }
+                    }
+                    const uint32_t dst = base + L::off_v + (uint32_t)b * L::V;
+                    auto word = [&](const uint4 &u, int w) { return w == 0 ? u.x : w == 1 ? u.y : w == 2 ? u.z : u.w; };
+#pragma unroll
+                    for (int g = 0; g < VG; ++g)
+#pragma unroll
+                        for (int w = 0; w < 4; ++w)
+#pragma unroll
+                            for (int hh = 0; hh < 2; ++hh) {
+                                uint4 x, y;                               // d = 16 dg + 4 w + 2 hh, and the next
+                                const uint32_t sel = hh ? 0x7362 : 0x5140;
+                                codes_f16<CODE>(__byte_perm(word(c[g][0], w), word(c[g][1], w), sel), x.x, y.x);
+                                codes_f16<CODE>(__byte_perm(word(c[g][2], w), word(c[g][3], w), sel), x.y, y.y);
+                                codes_f16<CODE>(__byte_perm(word(c[g][4], w), word(c[g][5], w), sel), x.z, y.z);
+                                codes_f16<CODE>(__byte_perm(word(c[g][6], w), word(c[g][7], w), sel), x.w, y.w);
+                                const int d = 16 * (dg0 + 8 * g) + 4 * w + 2 * hh;
+                                st_shared16(dst + swz(d, kg), x);
+                                st_shared16(dst + swz(d + 1, kg), y);
+                            }
+                    if (j + 1 < steps) load(j + 1);
+                }
+                fence_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(v_full(b));
             }
-            fence_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(v_full(b));
         }
-    } else if (lane == 0 && steps > 0) {
+    } else if (warp == 8 && lane == 0 && steps > 0) {
         // ---------------- MMA issuer ----------------
-        const uint32_t is = idesc_f16(PT_ROWS, PT_KEYS), io = idesc_f16(PT_ROWS, D);
+        const uint32_t is = idesc_f16(PT_ROWS, PT_KEYS), io = idesc_f16(PT_ROWS, DV);
         const uint64_t qd = smem_desc_sw128(base);
         if (!mbar_wait(q_full, 0, abort_flag)) fail();
         auto scores = [&](int j) {
@@ -483,11 +546,11 @@ kv8_prompt_kernel(const AttnParams p) {
             tc_fence_after();
             const uint64_t kd = smem_desc_sw128(base + L::off_k + (uint32_t)sb * L::K);
 #pragma unroll
-            for (int term = 0; term < TERMS; ++term)
+            for (int term = TERMS - 1; term >= 0; --term)              // (small sums first: they lose less)
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i)
                     tc_mma_f16(tmem + (uint32_t)(64 * b), qd + (uint64_t)((term * L::Q + (i / 4) * (PT_ROWS * 128)) / 16 + 2 * (i % 4)),
-                               kd + (uint64_t)((i / 4) * (PT_KEYS * 128 >> 4) + 2 * (i % 4)), is, term > 0 || i > 0 ? 1u : 0u);
+                               kd + (uint64_t)((i / 4) * (PT_KEYS * 128 >> 4) + 2 * (i % 4)), is, term < TERMS - 1 || i > 0 ? 1u : 0u);
             tc_commit(k_empty(sb));
             tc_commit(s_full(b));
         };
@@ -501,11 +564,11 @@ kv8_prompt_kernel(const AttnParams p) {
             tc_fence_after();
             const uint64_t vd = smem_desc_sw128(base + L::off_v + (uint32_t)sb * L::V);
 #pragma unroll
-            for (int i = 0; i < PT_KEYS / 16; ++i)
+            for (int term = TERMS - 1; term >= 0; --term)
 #pragma unroll
-                for (int term = 0; term < TERMS; ++term)
-                    tc_mma_f16_ts(tmem + 128u, tmem + (uint32_t)(64 * b + 32 * (i / 2) + 16 * term + 8 * (i % 2)),
-                                  vd + (uint64_t)(2 * i), io, j > 0 || i > 0 || term > 0 ? 1u : 0u);
+                for (int i = 0; i < PT_KEYS / 16; ++i)
+                    tc_mma_f16_ts(tmem + o_at(j), tmem + (uint32_t)(64 * b + 32 * (i / 2) + 16 * term + 8 * (i % 2)),
+                                  vd + (uint64_t)(2 * i), io, (L::apart ? j % L::group : j) > 0 || i > 0 || term < TERMS - 1 ? 1u : 0u);
             tc_commit(pv_done(b));
         }
         tc_commit(drain);
@@ -529,10 +592,16 @@ template <typename T, int CODE, int D> int launch_prompt(const AttnParams &p, in
     Q35_CUDA_TRY(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !configured[dev]) {
         Q35_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::smem));
+        if (L::apart) {
+            // the split of the registers takes what the CTA has at launch: with less it would wait for ever
+            cudaFuncAttributes a;
+            Q35_CUDA_TRY(cudaFuncGetAttributes(&a, kern));
+            if (a.numRegs < L::launch_regs) return set_error(Q35_ERR_INVALID, "kv8_attention: the prompt kernel was built with too few registers");
+        }
         if (dev >= 0 && dev < 64) configured[dev] = true;
     }
-    const dim3 grid((unsigned)ceil_div((int64_t)p.max_rows * p.G, PT_ROWS), (unsigned)zs);
-    Q35_CUDA_TRY(launch_dependent(kern, grid, PT_THREADS, L::smem, s, 1, p));
+    const dim3 grid((unsigned)ceil_div((int64_t)p.max_rows * p.G, PT_ROWS), (unsigned)zs, (unsigned)(D / L::DV));
+    Q35_CUDA_TRY(launch_dependent(kern, grid, L::threads, L::smem, s, 1, p));
     return Q35_OK;
 }
 template <typename T, int CODE> int launch_prompt(const AttnParams &p, int D, int zs, cudaStream_t s) {
@@ -546,9 +615,10 @@ template <typename T> int launch_prompt(const AttnParams &p, int code, int D, in
 
 // Half a tile of (row, head) pairs at least, and tiles for a good part of the SMs: the 16-row form
 // splits few tiles' keys over all SMs, this one walks them alone.  Append and attention over 4000
-// older tokens, 16-row form against this one: 8 tiles 48 / 84 us (bf16, head_dim 128), 57 / 113
-// (fp32), 89 / 119 (bf16, 256); 16 tiles 64 / 93, 85 / 115, 118 / 121; 32 tiles 94 / 89, 137 / 121,
-// 172 / 128; 160 tiles 330 / 135, 505 / 243, 600 / 262.
+// older tokens, 16-row form against this one: bf16 8 tiles 48 / 84 us (head_dim 128), 89 / 119 (256);
+// 16 tiles 64 / 93, 118 / 121; 32 tiles 94 / 89, 172 / 128; 160 tiles 330 / 135, 600 / 262.  fp32 with head_dim
+// 64, 128, 256: 32 tiles 68 / 86, 119 / 124, 251 / 184; 64 tiles 99 / 90, 192 / 149, 415 / 240; 160 tiles
+// 227 / 180, 478 / 257, 944 / 647.
 bool kv8_prompt_takes(const q35_kv8_cache &c, int32_t heads, int32_t max_rows) {
     const int64_t pairs = (int64_t)max_rows * (heads / c.kv_heads);
     return pairs >= PT_ROWS / 2 && ceil_div(pairs, PT_ROWS) * c.seqs * c.kv_heads >= 32;
