@@ -32,7 +32,7 @@
 // Measured: 1 x 10240 x 8192 20 us (84 MB of w, 4.2 TB/s), 16 x 8192 x 28672 43 us (236 MB, 5.5
 // TB/s): w's bytes through HBM bound both, less the start and the cluster's exchange.
 // 197 x 5120 x 13824 44 us: 20 tiles of 256 x 256 split three ways, each pair's chain of k-blocks.
-// 2048 x 28672 x 8192 520 us alone, 600 under the power cap (1.6 PFLOP/s): the promotion, 1230
+// 2048 x 28672 x 8192 600 us back to back (1.6 PFLOP/s, at the power cap): the promotion, 1230
 // clocks a k-block of a pair's tile, against 512 of MMAs.
 //
 // Every wait is bounded: a wait that gives up records Q35_ERR_TIMEOUT in the context's error

@@ -2,10 +2,11 @@
 // q35_sample_filtered.cu): element types, the two 8-bit codes and their rounding,
 // argument checks.
 //
-// A code stands for code * scale.  scale = amax / Q in binary32 (Q = 127 for int8, 448 for
-// e4m3), and a value x is stored as the code nearest to x / scale: the binary32 quotient,
-// correctly rounded, then rounded to the code with ties to even and clamped to [-Q, Q].
-// Every step is an IEEE operation, so a plain program in binary32 gets the same codes.
+// A code stands for code * scale, with the largest magnitude of the block at +-Q (127 for int8, 448 for
+// e4m3).  encode8 rounds a binary32 quotient to the nearest code, ties to even, clamped to [-Q, Q]; how
+// the scale and the quotient are formed is each operator's own: the append's are IEEE operations that a plain program
+// repeats bit for bit (q35_kv8.cu), the norm's have other roundings than a division (q35_norm8.cu), so a
+// value next to a rounding boundary may get the code on its other side.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

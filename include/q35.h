@@ -265,8 +265,9 @@ int q35_rms_norm_quant_dev(q35_ctx ctx, int dtype, const void *x, int64_t ldx, c
  * x [M] rows of K codes ldx apart with x_scales [M][ceil(K/128)]; w [N] rows of K codes ldw
  * apart with w_scales [ceil(N/128)][ceil(K/128)]; y dtype, [M] rows of N elements ldy apart.
  * Rows of x and w start on 16-byte boundaries (base and stride); K need not be a multiple of
- * anything (bytes between K and the stride are not used).  M <= 65536, K <= 131072,
- * N <= 2^24; M = 0 or N = 0 does nothing. */
+ * anything (bytes between K and the stride are not used).  The two scales are multiplied first: a
+ * product below binary32's normal numbers loses bits.  M <= 65536, K <= 131072, N <= 2^24; M = 0 or
+ * N = 0 does nothing. */
 int q35_fp8_gemm_dev(q35_ctx ctx, const void *x, int64_t ldx, const float *x_scales, const void *w,
                      int64_t ldw, const float *w_scales, int dtype, void *y, int64_t ldy, int32_t M,
                      int32_t N, int32_t K);
@@ -303,7 +304,8 @@ int q35_kv8_append_dev(q35_ctx ctx, const q35_kv8_cache *cache, int dtype, const
  * and ldo apart; heads a multiple of kv_heads.  workspace: device memory of
  * q35_kv8_attention_workspace bytes (16-byte aligned; may be NULL when that is 0), used by this
  * call alone while it runs.  Nothing behind a sequence's last token counts, whatever it holds.
- * max_rows * heads / kv_heads is at most 2^31 - 129. */
+ * max_rows * heads / kv_heads is at most 2^31 - 129.  max_rows decides how the call is laid out:
+ * prompts and single tokens are faster in a call each. */
 int q35_kv8_attention_dev(q35_ctx ctx, const q35_kv8_cache *cache, int dtype, const void *q, int64_t ldq,
                           int32_t heads, void *out, int64_t ldo, const int32_t *row_start,
                           const int32_t *past, int32_t rows, int32_t max_rows, float scale,
@@ -409,9 +411,11 @@ typedef struct {
 int q35_model_set_sampling(q35_model m, const q35_sampling *cfg);
 /* how the model keeps its KV cache (no counterpart in the reference; default Q35_KV_FP32): in
  * 8 bits with a scale for each block of `block` tokens (16, 32, 64 or 128; ignored for fp32) and
- * head, by q35_kv8_append_dev's and q35_kv8_attention_dev's rules.  A quarter of the memory, and
- * a rounding of every key and value to 8 bits.  Empties every sequence (as q35_model_reset);
- * under tensor parallelism every rank makes the same call. */
+ * head, by q35_kv8_append_dev's and q35_kv8_attention_dev's rules.  A quarter of the memory
+ * afterwards (a model is created with the fp32 cache, and both are held during the call, which
+ * leaves the model as it was where the new one cannot be had), and a rounding of every key and
+ * value to 8 bits.  Empties every sequence (as q35_model_reset); under tensor parallelism every
+ * rank makes the same call. */
 enum { Q35_KV_FP32 = 0, Q35_KV_INT8 = 1, Q35_KV_E4M3 = 2 };
 int q35_model_set_kv_format(q35_model m, int format, int32_t block);
 /* apply_transformer_layer (transformer_layer.f90:527-565) of one layer on host x(S,hidden)
